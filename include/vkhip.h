@@ -441,6 +441,102 @@ int vkhip_resize_nearest(const void *x, void *y, int64_t N, int64_t C, int64_t H
 int vkhip_resize_nearest_view(const void *x, int64_t x_pstride, void *y, int64_t y_pstride, int64_t N, int64_t C, int64_t H, int64_t W,
                               int64_t OH, int64_t OW, vkhip_stream_t s);
 
+/* ---------------------------------------------------------------- from feature maps to tokens
+ * Operators that hand the networks' feature maps on to token models: a norm whose output is one row
+ * of channels per pixel (a [T, C] row matrix with C % 4 == 0 is also an NC4HW4 tensor with N = T and
+ * H = W = 1, so vkhip_conv_forward projects it), attention over sequences of such rows, an 8-bit
+ * cache of their keys and values in pages, and attention over it. No counterpart in the reference's
+ * backends. Forward only, like the rest of the library. Strides are in elements. Every sum, mean,
+ * softmax statistic and accumulator is fp32; outputs are rounded once, to nearest even. */
+#define VKHIP_DT_F16 0
+#define VKHIP_DT_BF16 1
+#define VKHIP_DT_F32 2
+
+/* Group norm with an activation: y = act((x - mean) * rstd * gamma[c] + beta[c]), mean and biased
+ * variance over the H*W pixels and C/groups channels of a group of one image, rstd = 1/sqrt(var + eps).
+ *   x_fmt / y_fmt: 1 NHWC (rows of C channels, one per pixel) or 2 NC4HW4 (F16 only; channels past C
+ *           are not read and written +0), independently.
+ *   x_row / y_row: elements from one NHWC row to the next (0 = C), for rows that are slices of wider ones.
+ *   gamma, beta: fp32 [C] on the device; NULL = 1 and 0.
+ * y may be x where format and rows agree. workspace: vkhip_group_norm_workspace_bytes (0 for a
+ * descriptor that is refused), 16-byte aligned, contents undefined before and after. N or H*W of 0 is no work. */
+typedef struct vkhip_group_norm_desc {
+    int32_t N, C, H, W, groups;
+    int32_t x_fmt, y_fmt, dtype;
+    int32_t act;
+    float   act_lo, act_hi, eps;
+    int64_t x_row, y_row;
+} vkhip_group_norm_desc;
+size_t vkhip_group_norm_workspace_bytes(const vkhip_group_norm_desc *d);
+int    vkhip_group_norm(const vkhip_group_norm_desc *d, const void *x, const float *gamma, const float *beta, void *y, void *workspace,
+                        vkhip_stream_t s);
+
+/* Attention over packed sequences: sequence b has the query rows cu_q[b] .. cu_q[b+1] and the key and
+ * value rows cu_k[b] .. cu_k[b+1] (device int32 [batch + 1], rising; values outside [0, total] are
+ * clamped to it). Head h of q_heads reads key/value head h / (q_heads / kv_heads).
+ *   o = sum_j softmax_j(scale * q . k_j) v_j over every key of the sequence or, with causal, over the keys
+ *   j <= i + nk - nq for query i of nq (the last query sees the last key).
+ * A query that sees no key gives zeros. What a query does not see never reaches it, NaN and
+ * infinities included. F16 or BF16; head_dim a multiple of 8 up to 128; scale > 0; every row of every
+ * head starts on a 16-byte boundary. o must not overlap q, k or v. workspace:
+ * vkhip_attention_workspace_bytes (may be 0: then NULL is taken). */
+typedef struct vkhip_attention_desc {
+    int32_t batch, q_heads, kv_heads, head_dim;
+    int32_t total_q, total_k; /* rows of q and o, and of k and v */
+    int32_t dtype, causal;
+    float   scale;
+    int64_t q_row, q_head, k_row, k_head, v_row, v_head, o_row, o_head;
+} vkhip_attention_desc;
+size_t vkhip_attention_workspace_bytes(const vkhip_attention_desc *d);
+int    vkhip_attention_packed(const vkhip_attention_desc *d, const void *q, const void *k, const void *v, const int32_t *cu_q,
+                              const int32_t *cu_k, void *o, void *workspace, vkhip_stream_t s);
+
+/* A cache of keys and values in 8 bits. A page holds page_tokens consecutive tokens of one sequence for
+ * every head, with one fp32 scale per page and head for the keys and one for the values:
+ *   k int8 [pages][kv_heads][page_tokens][Dp], v int8 [pages][kv_heads][Dp][page_tokens] (a head's tokens
+ *   side by side, as the second product reads them), k_scale / v_scale fp32 [pages][kv_heads];
+ *   value = int8 * scale; Dp = vkhip_kv_row(head_dim), what lies past head_dim is never used.
+ * table int32 [batch][max_blocks] names the page of every block of page_tokens tokens of a sequence.
+ * Sequences may share pages that are only read. A table entry outside [0, pages) is a block without
+ * memory: nothing is written there, it reads as zeros and no query sees it. Lengths are clamped to
+ * max_blocks * page_tokens. head_dim: a multiple of 8 up to 128; page_tokens 32, 64, 128 or 256; k and v
+ * 16-byte aligned. */
+typedef struct vkhip_kv_cache {
+    void          *k, *v;
+    float         *k_scale, *v_scale;
+    const int32_t *table;
+    int32_t        pages, page_tokens, kv_heads, head_dim, batch, max_blocks;
+} vkhip_kv_cache;
+int32_t vkhip_kv_row(int32_t head_dim); /* Dp: 64 or 128; 0 for a head_dim that is not taken */
+/* Rows of keys and values in F16 or BF16, `total` of them, each head's row on a 16-byte boundary. */
+typedef struct vkhip_kv_rows {
+    int32_t dtype, total;
+    int64_t k_row, k_head, v_row, v_head;
+} vkhip_kv_rows;
+/* Sequence b holds lens[b] tokens; the rows cu[b] .. cu[b+1] become its next ones (cu int32 [batch + 1]
+ * rising and clamped to [0, total], lens int32 [batch], both on the device; the caller advances lens).
+ * Per page and head: s = max(s0, max|x| / 127) over the rows x that join it, s0 the scale of the tokens
+ * already there (0 for none); if the scale grew those become rint(q * (s0 / s)), the new ones
+ * rint(x / s). A NaN or infinity among the rows makes the scale NaN: all that the page holds reads as NaN
+ * until it begins anew. A page that two sequences share must not be appended to. */
+int vkhip_kv_append(const vkhip_kv_cache *c, const vkhip_kv_rows *r, const void *k, const void *v, const int32_t *cu, const int32_t *lens,
+                    vkhip_stream_t s);
+/* The tokens start[b] .. start[b] + cu[b+1] - cu[b] of sequence b as the rows cu[b] .. cu[b+1]: what prompt
+ * attention behind a cached prefix takes. */
+int vkhip_kv_read(const vkhip_kv_cache *c, const vkhip_kv_rows *r, const int32_t *start, const int32_t *cu, void *k, void *v, vkhip_stream_t s);
+/* Attention over the cache: the last q_tokens (1 .. 64) tokens of each sequence of lens[b] tokens, query t at
+ * position lens[b] - q_tokens + t, over the tokens up to its own position. q and o: row b * q_tokens + t,
+ * F16 or BF16, 16-byte aligned rows per head. max_len: no length is larger (0: max_blocks * page_tokens);
+ * it sizes the launch, longer sequences are cut to it. A query that sees no token gives zeros. */
+typedef struct vkhip_kv_attention_desc {
+    int32_t q_heads, q_tokens, dtype, max_len;
+    float   scale;
+    int64_t q_row, q_head, o_row, o_head;
+} vkhip_kv_attention_desc;
+size_t vkhip_kv_attention_workspace_bytes(const vkhip_kv_attention_desc *d, const vkhip_kv_cache *c);
+int    vkhip_kv_attention(const vkhip_kv_attention_desc *d, const vkhip_kv_cache *c, const void *q, const int32_t *lens, void *o,
+                          void *workspace, vkhip_stream_t s);
+
 #ifdef __cplusplus
 }
 #endif

@@ -24,6 +24,7 @@ c_int, c_i32, c_i64, c_u64, c_f, c_vp, c_sz, c_char_p = (
 c_dbl = ctypes.c_double
 
 ACT = {"none": 0, "relu": 1, "relu6": 2, "clip": 3, "hardswish": 4, "silu": 5}
+DT_F16, DT_BF16, DT_F32 = 0, 1, 2
 CONV_AUTO, CONV_GEMM, CONV_SPLITK, CONV_WINOGRAD, CONV_DEPTHWISE, CONV_SPLITK_LAST = 0, 1, 2, 3, 4, 5
 
 
@@ -54,6 +55,30 @@ class ConvPw2Desc(ctypes.Structure):
 
 class PoolDesc(ctypes.Structure):
     _fields_ = [(n, c_i32) for n in ("N", "C", "H", "W", "OH", "OW", "KH", "KW", "SH", "SW", "PT", "PL")]
+
+
+class GroupNormDesc(ctypes.Structure):
+    _fields_ = [(n, c_i32) for n in ("N", "C", "H", "W", "groups", "x_fmt", "y_fmt", "dtype", "act")] + \
+               [("act_lo", c_f), ("act_hi", c_f), ("eps", c_f), ("x_row", c_i64), ("y_row", c_i64)]
+
+
+class AttentionDesc(ctypes.Structure):
+    _fields_ = [(n, c_i32) for n in ("batch", "q_heads", "kv_heads", "head_dim", "total_q", "total_k", "dtype", "causal")] + \
+               [("scale", c_f)] + [(n, c_i64) for n in ("q_row", "q_head", "k_row", "k_head", "v_row", "v_head", "o_row", "o_head")]
+
+
+class KvCache(ctypes.Structure):
+    _fields_ = [(n, c_vp) for n in ("k", "v", "k_scale", "v_scale", "table")] + \
+               [(n, c_i32) for n in ("pages", "page_tokens", "kv_heads", "head_dim", "batch", "max_blocks")]
+
+
+class KvRows(ctypes.Structure):
+    _fields_ = [("dtype", c_i32), ("total", c_i32)] + [(n, c_i64) for n in ("k_row", "k_head", "v_row", "v_head")]
+
+
+class KvAttentionDesc(ctypes.Structure):
+    _fields_ = [(n, c_i32) for n in ("q_heads", "q_tokens", "dtype", "max_len")] + [("scale", c_f)] + \
+               [(n, c_i64) for n in ("q_row", "q_head", "o_row", "o_head")]
 
 
 P = ctypes.POINTER
@@ -148,6 +173,15 @@ VKHIP_API = {
     "vkhip_concat_channels": (c_int, [P(c_vp), P(c_i64), c_i32, c_vp, c_i64, c_i64, c_vp]),
     "vkhip_slice_channels": (c_int, [c_vp, c_vp, c_i64, c_i64, c_i64, c_i64, c_i64, c_vp]),
     "vkhip_resize_nearest": (c_int, [c_vp, c_vp, c_i64, c_i64, c_i64, c_i64, c_i64, c_i64, c_vp]),
+    "vkhip_group_norm_workspace_bytes": (c_sz, [P(GroupNormDesc)]),
+    "vkhip_group_norm": (c_int, [P(GroupNormDesc), c_vp, c_vp, c_vp, c_vp, c_vp, c_vp]),
+    "vkhip_attention_workspace_bytes": (c_sz, [P(AttentionDesc)]),
+    "vkhip_attention_packed": (c_int, [P(AttentionDesc), c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp]),
+    "vkhip_kv_row": (c_i32, [c_i32]),
+    "vkhip_kv_append": (c_int, [P(KvCache), P(KvRows), c_vp, c_vp, c_vp, c_vp, c_vp]),
+    "vkhip_kv_read": (c_int, [P(KvCache), P(KvRows), c_vp, c_vp, c_vp, c_vp, c_vp]),
+    "vkhip_kv_attention_workspace_bytes": (c_sz, [P(KvAttentionDesc), P(KvCache)]),
+    "vkhip_kv_attention": (c_int, [P(KvAttentionDesc), P(KvCache), c_vp, c_vp, c_vp, c_vp, c_vp]),
 }
 
 VKNN_API = {

@@ -1,0 +1,373 @@
+// Attention of a few query tokens per sequence over the 8-bit cache.
+//
+// Bound by the cache's bytes, so every byte is read once, straight into the registers that feed the matrix
+// cores, and all query heads and tokens that share a key/value head are rows of one product:
+//   S^T = K Q^T (16x16x32 tiles: 16 tokens x 16 rows), softmax per row with a running maximum, O^T += V^T P^T.
+// A token tile's output registers are the other product's operand as they are: which token sits in which
+// contraction slot is free as long as both operands agree, so K's rows are taken in the order that leaves each
+// lane with the tokens whose values its V load brings (16 tokens of one channel, side by side in the page).
+// int8 becomes fp16 exactly; a page's key scale multiplies its scores, its value scale the fp32 product of the
+// page, so weights are rounded to fp16 unscaled (at most 1, the largest of a row exactly 1).
+// The tokens of a sequence are split over workgroups and a workgroup's four waves; partial results
+// (maximum, sum, product) join in LDS and, across workgroups, in a second kernel.
+#include "kv_cache.h"
+
+namespace vkhip {
+
+    struct KvAttnArgs {
+        KvArgs         c;
+        const void    *q;
+        void          *o;
+        const int32_t *lens;
+        float         *part; // [batch][head][row][split]: row values, then (maximum, sum)
+        float          scale;
+        int            group, rows, q_tokens; // query heads per kv head; rows = group * q_tokens
+        int            blocks;                // blocks of 16 * RT rows
+        int            max_len, span, splits; // tokens per workgroup
+        int64_t        q_row, q_head, o_row, o_head;
+    };
+
+    // 4 int8 (as bits) -> 4 fp16, exactly: the byte with its sign flipped is the low byte of 1024 + (b + 128).
+    __device__ __forceinline__ void i8_to_h4(unsigned b, half2v &lo, half2v &hi) {
+        b ^= 0x80808080u;
+        const half2v off = {(half_t) 1152.f, (half_t) 1152.f};
+        lo = __builtin_bit_cast(half2v, __builtin_amdgcn_perm(0x64646464u, b, 0x04010400u)) - off;
+        hi = __builtin_bit_cast(half2v, __builtin_amdgcn_perm(0x64646464u, b, 0x04030402u)) - off;
+    }
+    __device__ __forceinline__ half8 i8_to_h8(unsigned a, unsigned b) {
+        half2v x, y, z, w;
+        i8_to_h4(a, x, y);
+        i8_to_h4(b, z, w);
+        return half8 {x[0], x[1], y[0], y[1], z[0], z[1], w[0], w[1]};
+    }
+
+    constexpr int kStep = 64; // tokens a wave takes at a time
+
+    // DJ = row / 64 channels, RT tiles of 16 rows, P32: pages of 32 tokens (two to a step).
+    template <typename T, int DJ, int RT, bool P32>
+    __global__ __launch_bounds__(256) void kv_attention_kernel(KvAttnArgs a) {
+        constexpr int Dp = DJ * 64, DT = DJ * 4;
+        __shared__ float wave_m[4][RT * 16], wave_l[4][RT * 16];
+        __shared__ float acc_lds[4][16][Dp + 4];
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, nn = lane & 15;
+        const int split = blockIdx.x, head = blockIdx.y / a.blocks, row0 = blockIdx.y % a.blocks * (16 * RT), b = blockIdx.z;
+        const int P   = a.c.page_tokens, D = a.c.head_dim;
+        const int len = clampi(a.lens[b], 0, min(a.max_len, a.c.max_blocks * P));
+        const int t0 = split * a.span, t1 = min(len, t0 + a.span);
+        if (t0 >= len && split > 0) return; // split 0 also answers for a sequence without tokens
+
+        // queries: lane holds row nn, channels 64 j + 16 g + 8 e .. + 7; bf16 rows are brought into fp16's range by
+        // a power of two each (their 8 bits fit its 11; what falls below 2^-24 of a row's largest is lost)
+        half8 qf[RT][DJ][2];
+        int   limit[RT]; // tokens below it are seen
+        float c2[RT];    // factor from a score to the exponent of 2
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            const int  row = row0 + rt * 16 + nn, t = row / a.group, h = head * a.group + row % a.group;
+            const bool in  = row < a.rows;
+            limit[rt]      = in ? len - a.q_tokens + t + 1 : 0;
+            const T *src   = (const T *) a.q + ((int64_t) b * a.q_tokens + t) * a.q_row + h * a.q_head;
+            float    v[DJ][2][8], big = 0.f;
+#pragma unroll
+            for (int j = 0; j < DJ; ++j)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int d = 64 * j + 16 * g + 8 * e;
+                    typedef T V __attribute__((ext_vector_type(8)));
+                    V         x;
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) x[k] = (T) 0.f;
+                    if (in && d < D) x = *reinterpret_cast<const V *>(src + d);
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        v[j][e][k] = (float) x[k];
+                        big        = fmaxf(big, fabsf(v[j][e][k]));
+                    }
+                }
+            float mul = 1.f;
+            c2[rt]    = a.scale * 1.44269504088896f;
+            if constexpr (!__is_same(T, half_t)) {
+                big          = fmaxf(big, __shfl_xor(big, 16));
+                big          = fmaxf(big, __shfl_xor(big, 32));
+                const int ex = clampi((int) (__float_as_uint(big) >> 23), 7, 247);
+                if (big > 0.f && big < __builtin_inff()) {
+                    mul = __uint_as_float((unsigned) (254 - ex) << 23);
+                    c2[rt] *= __uint_as_float((unsigned) ex << 23);
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < DJ; ++j)
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) qf[rt][j][e][k] = (half_t) (v[j][e][k] * mul);
+        }
+
+        float4v acc[RT][DT];
+        float   m[RT], l[RT];
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            m[rt] = -__builtin_inff(), l[rt] = 0.f;
+#pragma unroll
+            for (int d = 0; d < DT; ++d) acc[rt][d] = float4v {0.f, 0.f, 0.f, 0.f};
+        }
+
+        const int32_t *table = a.c.table + (int64_t) b * a.c.max_blocks;
+        const int64_t  page_bytes = (int64_t) P * Dp;
+        for (int tok = t0 + wave * kStep; tok < t1; tok += 4 * kStep) {
+            // the step's page, or its two; a block without memory is a page that no query sees
+            const unsigned char *kp[2], *vp[2];
+            float                ks[2], vs[2];
+            bool                 has[2];
+#pragma unroll
+            for (int u = 0; u < (P32 ? 2 : 1); ++u) {
+                const int at = tok + 32 * u, id = at < t1 ? __builtin_amdgcn_readfirstlane(table[at / P]) : -1;
+                has[u]       = id >= 0 && id < a.c.pages;
+                const int64_t hp = (int64_t) (has[u] ? id : 0) * a.c.heads + head;
+                kp[u] = a.c.k + hp * page_bytes + (int64_t) (at % P) * Dp;
+                vp[u] = a.c.v + hp * page_bytes + at % P;
+                ks[u] = has[u] ? a.c.k_scale[hp] : 0.f;
+                vs[u] = has[u] ? a.c.v_scale[hp] : 0.f;
+            }
+            if (!has[0] && !(P32 && has[1])) continue;
+            tk_u32x4 kr[4][DJ], vr[DT];
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int j = 0; j < DJ; ++j) {
+                    // row nn = 4 (nn / 4) + i of tile t is the token that lane group nn / 4 multiplies
+                    const int r = P32 ? 8 * (nn >> 2) + 4 * (t & 1) + (nn & 3) : 16 * (nn >> 2) + 4 * t + (nn & 3);
+                    kr[t][j]    = *reinterpret_cast<const tk_u32x4 *>(kp[P32 ? t >> 1 : 0] + r * Dp + 64 * j + 16 * g);
+                }
+#pragma unroll
+            for (int d = 0; d < DT; ++d) {
+                if constexpr (P32) {
+                    const tk_u32x2 x = *reinterpret_cast<const tk_u32x2 *>(vp[0] + (int64_t) (16 * d + nn) * P + 8 * g);
+                    const tk_u32x2 y = *reinterpret_cast<const tk_u32x2 *>(vp[1] + (int64_t) (16 * d + nn) * P + 8 * g);
+                    vr[d]            = tk_u32x4 {x[0], x[1], y[0], y[1]};
+                } else {
+                    vr[d] = *reinterpret_cast<const tk_u32x4 *>(vp[0] + (int64_t) (16 * d + nn) * P + 16 * g);
+                }
+            }
+            float4v s[RT][4];
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) s[rt][t] = float4v {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int j = 0; j < DJ; ++j)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const half8 kf = i8_to_h8(kr[t][j][2 * e], kr[t][j][2 * e + 1]);
+#pragma unroll
+                        for (int rt = 0; rt < RT; ++rt) s[rt][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[rt][j][e], s[rt][t], 0, 0, 0);
+                    }
+            }
+            half8 pf[RT][2];
+            float alpha[RT];
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+                float top = -__builtin_inff();
+#pragma unroll
+                for (int t = 0; t < 4; ++t) {
+                    const float f = ks[P32 ? t >> 1 : 0] * c2[rt];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int at = tok + (P32 ? 32 * (t >> 1) + 8 * g + 4 * (t & 1) + i : 16 * g + 4 * t + i);
+                        float     x  = s[rt][t][i] * f;
+                        x            = at < limit[rt] && has[P32 ? t >> 1 : 0] ? x : -__builtin_inff();
+                        s[rt][t][i]  = x;
+                        top          = fmaxf(top, x);
+                    }
+                }
+                top               = fmaxf(top, __shfl_xor(top, 16));
+                top               = fmaxf(top, __shfl_xor(top, 32));
+                const float to    = fmaxf(m[rt], top), base = to == -__builtin_inff() ? 0.f : to;
+                alpha[rt]         = exp2_hw(m[rt] - base);
+                m[rt]             = to;
+                float sum         = 0.f;
+#pragma unroll
+                for (int t = 0; t < 4; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float p = exp2_hw(s[rt][t][i] - base);
+                        sum += p;
+                        pf[rt][t >> 1][(t & 1) * 4 + i] = (half_t) p;
+                    }
+                l[rt] = l[rt] * alpha[rt] + sum;
+            }
+#pragma unroll
+            for (int d = 0; d < DT; ++d) {
+                const half8   v0 = i8_to_h8(vr[d][0], vr[d][1]), v1 = i8_to_h8(vr[d][2], vr[d][3]);
+                const float4v zero = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) {
+                    float4v x = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, pf[rt][0], zero, 0, 0, 0);
+                    // a row that sees nothing of a page takes nothing from it, whatever its scale
+                    const float f0 = limit[rt] > tok ? vs[0] : 0.f;
+                    if constexpr (P32) {
+                        const float4v y = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, pf[rt][1], zero, 0, 0, 0);
+                        const float   f1 = limit[rt] > tok + 32 ? vs[1] : 0.f;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) acc[rt][d][i] = acc[rt][d][i] * alpha[rt] + (x[i] * f0 + y[i] * f1);
+                    } else {
+                        x = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, pf[rt][1], x, 0, 0, 0);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) acc[rt][d][i] = acc[rt][d][i] * alpha[rt] + x[i] * f0;
+                    }
+                }
+            }
+        }
+
+        // join the four waves, a tile of rows at a time
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            l[rt] += __shfl_xor(l[rt], 16);
+            l[rt] += __shfl_xor(l[rt], 32);
+            if (g == 0) wave_m[wave][rt * 16 + nn] = m[rt], wave_l[wave][rt * 16 + nn] = l[rt];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            const int   r   = rt * 16 + nn;
+            const float top = fmaxf(fmaxf(wave_m[0][r], wave_m[1][r]), fmaxf(wave_m[2][r], wave_m[3][r]));
+            const float f   = exp2_hw(m[rt] - (top == -__builtin_inff() ? 0.f : top));
+#pragma unroll
+            for (int d = 0; d < DT; ++d) {
+                float4v x = acc[rt][d];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x[i] *= f;
+                *reinterpret_cast<float4v *>(&acc_lds[wave][nn][16 * d + 4 * g]) = x;
+            }
+            __syncthreads();
+            for (int i = threadIdx.x; i < 16 * Dp; i += 256) {
+                const int   n = i / Dp, d = i % Dp, row = row0 + rt * 16 + n, q = rt * 16 + n;
+                const float tm  = fmaxf(fmaxf(wave_m[0][q], wave_m[1][q]), fmaxf(wave_m[2][q], wave_m[3][q]));
+                const float tb  = tm == -__builtin_inff() ? 0.f : tm;
+                float       sum = 0.f, x = 0.f;
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    sum += wave_l[w][q] * exp2_hw(wave_m[w][q] - tb);
+                    x += acc_lds[w][n][d];
+                }
+                if (row >= a.rows || d >= D) continue;
+                if (a.splits == 1) {
+                    const int t = row / a.group, h = head * a.group + row % a.group;
+                    ((T *) a.o)[((int64_t) b * a.q_tokens + t) * a.o_row + h * a.o_head + d] = (T) (sum == 0.f ? 0.f : x / sum);
+                } else {
+                    float *p = a.part + (((int64_t) b * a.c.heads + head) * a.rows + row) * a.splits * (D + 2) + (int64_t) split * (D + 2);
+                    p[d]     = x;
+                    if (d == 0) p[D] = tm, p[D + 1] = sum;
+                }
+            }
+            __syncthreads();
+        }
+    }
+
+    // Joins the splits of one row: one wave, two channels a lane.
+    template <typename T>
+    __global__ __launch_bounds__(64) void kv_join_kernel(KvAttnArgs a) {
+        const int row = blockIdx.x, head = blockIdx.y, b = blockIdx.z, D = a.c.head_dim, lane = threadIdx.x;
+        const int len = clampi(a.lens[b], 0, min(a.max_len, a.c.max_blocks * a.c.page_tokens));
+        const int n   = max(1, (len + a.span - 1) / a.span);
+        const float *p = a.part + (((int64_t) b * a.c.heads + head) * a.rows + row) * a.splits * (D + 2);
+        float top = -__builtin_inff();
+        for (int k = lane; k < n; k += 64) top = fmaxf(top, p[(int64_t) k * (D + 2) + D]);
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) top = fmaxf(top, __shfl_xor(top, o));
+        const float base = top == -__builtin_inff() ? 0.f : top;
+        float       sum = 0.f, x0 = 0.f, x1 = 0.f;
+        for (int k = 0; k < n; ++k) {
+            const float *e = p + (int64_t) k * (D + 2);
+            const float  f = exp2_hw(e[D] - base);
+            sum += e[D + 1] * f;
+            if (lane < D) x0 += e[lane] * f;
+            if (lane + 64 < D) x1 += e[lane + 64] * f;
+        }
+        T *o = (T *) a.o + ((int64_t) b * a.q_tokens + row / a.group) * a.o_row + (head * a.group + row % a.group) * a.o_head;
+        if (lane < D) o[lane] = (T) (sum == 0.f ? 0.f : x0 / sum);
+        if (lane + 64 < D) o[lane + 64] = (T) (sum == 0.f ? 0.f : x1 / sum);
+    }
+
+    static int row_tiles(int rows) { return rows <= 16 ? 1 : (rows <= 32 ? 2 : 4); }
+
+    static const char *kv_attention_refusal(const vkhip_kv_attention_desc *d, const vkhip_kv_cache *c) {
+        if (const char *why = kv_refusal(c)) return why;
+        if (!d || d->q_heads <= 0 || d->q_heads % c->kv_heads) return "q_heads is not a multiple of kv_heads";
+        if (d->q_tokens < 1 || d->q_tokens > 64) return "q_tokens is not 1 .. 64";
+        if (d->q_heads > 65535) return "q_heads over 65535";
+        if (d->dtype != VKHIP_DT_F16 && d->dtype != VKHIP_DT_BF16) return "q and o are F16 or BF16";
+        if (!(d->scale > 0.f) || d->scale > 1e30f || d->max_len < 0) return "scale is not positive or max_len negative";
+        if (d->q_row < 0 || d->q_head < 0 || d->o_row < 0 || d->o_head < 0 || (d->q_row | d->q_head | d->o_row | d->o_head) % 8) return "strides are not multiples of 8";
+        return nullptr;
+    }
+
+    // How the call is cut: rows into blocks of up to 64, tokens into spans of whole rounds of the four waves.
+    static KvAttnArgs kv_attention_cut(const vkhip_kv_attention_desc *d, const vkhip_kv_cache *c) {
+        KvAttnArgs a {};
+        a.c        = kv_args(c);
+        a.group    = d->q_heads / c->kv_heads;
+        a.q_tokens = d->q_tokens;
+        a.rows     = a.group * d->q_tokens;
+        a.blocks   = (int) ceil_div(a.rows, 16 * row_tiles(a.rows));
+        const int64_t most = (int64_t) c->max_blocks * c->page_tokens;
+        a.max_len  = (int) (d->max_len > 0 && d->max_len < most ? d->max_len : most);
+        const int64_t base = (int64_t) c->batch * c->kv_heads * a.blocks, rounds = ceil_div(a.max_len > 0 ? a.max_len : 1, 4 * kStep);
+        int64_t       splits = base > 0 ? ceil_div(1024, base) : 1;
+        if (splits > rounds) splits = rounds;
+        a.span   = (int) (ceil_div(rounds, splits) * 4 * kStep);
+        a.splits = (int) ceil_div(a.max_len > 0 ? a.max_len : 1, a.span);
+        return a;
+    }
+
+    template <typename T, int DJ, int RT>
+    static void kv_attention_launch(const KvAttnArgs &a, hipStream_t s) {
+        const dim3 grid((unsigned) a.splits, (unsigned) (a.c.heads * a.blocks), (unsigned) a.c.batch);
+        if (a.c.page_tokens == 32) kv_attention_kernel<T, DJ, RT, true><<<grid, 256, 0, s>>>(a);
+        else kv_attention_kernel<T, DJ, RT, false><<<grid, 256, 0, s>>>(a);
+    }
+    template <typename T>
+    static int kv_attention_run(const KvAttnArgs &a, hipStream_t s) {
+        const int rt = row_tiles(a.rows);
+        if (a.c.row == 64) {
+            if (rt == 1) kv_attention_launch<T, 1, 1>(a, s);
+            else if (rt == 2) kv_attention_launch<T, 1, 2>(a, s);
+            else kv_attention_launch<T, 1, 4>(a, s);
+        } else {
+            if (rt == 1) kv_attention_launch<T, 2, 1>(a, s);
+            else if (rt == 2) kv_attention_launch<T, 2, 2>(a, s);
+            else kv_attention_launch<T, 2, 4>(a, s);
+        }
+        int rc = check_launch("kv_attention");
+        if (rc || a.splits == 1) return rc;
+        kv_join_kernel<T><<<dim3((unsigned) a.rows, (unsigned) a.c.heads, (unsigned) a.c.batch), 64, 0, s>>>(a);
+        return check_launch("kv_attention join");
+    }
+
+} // namespace vkhip
+
+using namespace vkhip;
+
+extern "C" {
+
+size_t vkhip_kv_attention_workspace_bytes(const vkhip_kv_attention_desc *d, const vkhip_kv_cache *c) {
+    if (kv_attention_refusal(d, c)) return 0;
+    const KvAttnArgs a = kv_attention_cut(d, c);
+    return a.splits == 1 ? 0 : (size_t) c->batch * c->kv_heads * a.rows * a.splits * (c->head_dim + 2) * sizeof(float);
+}
+
+int vkhip_kv_attention(const vkhip_kv_attention_desc *d, const vkhip_kv_cache *c, const void *q, const int32_t *lens, void *o, void *workspace,
+                       vkhip_stream_t s) {
+    if (const char *why = kv_attention_refusal(d, c)) return set_error(VKHIP_ERR_INVALID, "kv_attention: %s", why);
+    if (c->batch == 0) return VKHIP_OK;
+    if (const char *why = kv_bad_pointers(c)) return set_error(VKHIP_ERR_INVALID, "kv_attention: %s", why);
+    KvAttnArgs a = kv_attention_cut(d, c);
+    if (!q || !lens || !o || (a.splits > 1 && !workspace)) return set_error(VKHIP_ERR_INVALID, "kv_attention: null pointer");
+    if (misaligned16(q) || misaligned16(o) || misaligned16(workspace) || ((uintptr_t) lens) % 4) return set_error(VKHIP_ERR_INVALID, "kv_attention: misaligned pointer");
+    if ((int64_t) c->kv_heads * a.blocks > 65535) return set_error(VKHIP_ERR_INVALID, "kv_attention: too many heads and query tokens");
+    a.q = q, a.o = o, a.lens = lens, a.part = (float *) workspace, a.scale = d->scale;
+    a.q_row = d->q_row, a.q_head = d->q_head, a.o_row = d->o_row, a.o_head = d->o_head;
+    return d->dtype == VKHIP_DT_F16 ? kv_attention_run<half_t>(a, resolve_stream(s)) : kv_attention_run<bf16_t>(a, resolve_stream(s));
+}
+
+} // extern "C"
