@@ -4,7 +4,14 @@
 // and the squared deviations M2 of a few loaded values, and parts (n, mean, M2) merge as
 //   d = mean_b - mean_a,  mean = mean_a + d n_b / n,  M2 = M2_a + M2_b + d^2 n_a n_b / n
 // so a mean far from zero costs no digits of the variance, as the difference of two sums would.
+//
+// Bound by memory. What a workgroup can hold in its registers (a group of one image) is read once, in one
+// launch (gn_slab_kernel). Larger groups take two launches, statistics of chunks of pixels and the output, and
+// read x twice: 64 x 256 x 56 x 56 fp16 74 us, the statistics 28 (103 MB at 3.7 TB/s) and the output 41 (206 MB at
+// 5.1 TB/s, a large copy's rate); one launch of slabs takes 102 there, since 16-byte pieces of 512-byte rows cost
+// whole cache lines. The smallest calls are a launch: 1 x 128 x 40 x 40 6.0 us.
 #include "tokens.h"
+#include <type_traits>
 
 namespace vkhip {
 
@@ -15,9 +22,25 @@ namespace vkhip {
         float2      *part; // (mean, M2) per image, chunk, group
         int          N, C, CV, HW, G, Cg, chunk, chunks;
         int64_t      x_row, y_row;
-        int          act;
-        float        lo, hi, eps;
+        int          kind; // of activation, see gn_act
+        float        s, t, lo, hi, eps;
     };
+
+    // Every activation is one of three forms, so that a loop over a batch branches once:
+    // 0 clamp(s z + t, lo, hi), 1 z clamp(s z + t, lo, hi), 2 z sigmoid(z). NaN passes.
+    template <int KIND>
+    __device__ __forceinline__ float gn_act(const GnArgs &a, float z) {
+        if constexpr (KIND == 2) return z * __builtin_amdgcn_rcpf(1.f + __expf(-z));
+        float g = __builtin_fmaf(a.s, z, a.t);
+        g       = g < a.lo ? a.lo : (g > a.hi ? a.hi : g);
+        return KIND ? z * g : g;
+    }
+    template <typename F>
+    __device__ __forceinline__ void gn_by_kind(int kind, F f) {
+        if (kind == 0) f(std::integral_constant<int, 0>());
+        else if (kind == 1) f(std::integral_constant<int, 1>());
+        else f(std::integral_constant<int, 2>());
+    }
 
     struct Moments {
         float n, mean, m2;
@@ -25,7 +48,7 @@ namespace vkhip {
     __device__ __forceinline__ Moments merge(Moments a, Moments b) {
         const float n = a.n + b.n;
         if (n == 0.f) return a;
-        const float r = b.n / n, d = b.mean - a.mean;
+        const float r = b.n * __builtin_amdgcn_rcpf(n), d = b.mean - a.mean; // 1 ulp of the share: 1e-7 of a part's weight
         return {n, a.mean + d * r, a.m2 + b.m2 + d * d * a.n * r};
     }
 
@@ -45,16 +68,13 @@ namespace vkhip {
             return NC4 ? (((int64_t) n * a.CV + cv) * a.HW + p) * 4 : ((int64_t) n * a.HW + p) * row + cv * VEC;
         }
         typedef T V __attribute__((ext_vector_type(VEC)));
-        static __device__ __forceinline__ void load(const GnArgs &a, int n, int p, int cv, float *v) {
+        static __device__ __forceinline__ V raw(const GnArgs &a, int n, int p, int cv) {
             const T *s = (const T *) a.x + at(a, a.x_row, n, p, cv);
-            if constexpr (NC4 || AL) {
-                const V t = *reinterpret_cast<const V *>(s);
+            if constexpr (NC4 || AL) return *reinterpret_cast<const V *>(s);
+            V t;
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) v[j] = (float) t[j];
-            } else {
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) v[j] = cv * VEC + j < a.C ? (float) s[j] : 0.f;
-            }
+            for (int j = 0; j < VEC; ++j) t[j] = cv * VEC + j < a.C ? s[j] : (T) 0.f;
+            return t;
         }
         static __device__ __forceinline__ void store(const GnArgs &a, int n, int p, int cv, const float *v) {
             T *d = (T *) a.y + at(a, a.y_row, n, p, cv);
@@ -72,7 +92,7 @@ namespace vkhip {
     };
 
     constexpr int kGnThreads = 256;
-    constexpr int kGnBatch   = 4; // pixels a thread has in flight
+    constexpr int kGnBatch   = 8; // pixels a thread has in flight
 
     // Threads over (channel vectors, pixels): neighbouring threads read neighbouring memory, which is the
     // channels of an NHWC row and the pixels of an NC4HW4 plane.
@@ -87,58 +107,98 @@ namespace vkhip {
         return {t % cvs, cvs, t / cvs, pls};
     }
 
+    // Moments of a thread's channels over the chunk's pixels pl, pl + pls, ...: eight pixels at a time, whose
+    // mean and deviations are formed in registers and merged with equal counts.
+    template <typename T, int VEC, bool XN4, bool XAL>
+    __device__ __forceinline__ void gn_thread_moments(const GnArgs &a, int n, int p0, int np, int cv, int pl, int pls, float (&mean)[VEC], float (&m2)[VEC]) {
+        using X = GnIo<T, VEC, XN4, XAL>;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) mean[j] = m2[j] = 0.f;
+        float     count = 0.f;
+        int       base  = 0;
+        const int step  = pls * kGnBatch;
+        for (; base + step <= np; base += step) {
+            typename X::V v[kGnBatch];
+#pragma unroll
+            for (int u = 0; u < kGnBatch; ++u) v[u] = X::raw(a, n, p0 + base + pl + u * pls, cv);
+            __builtin_amdgcn_sched_barrier(0); // the loads stay ahead of the first use
+            const float share = kGnBatch * __builtin_amdgcn_rcpf(count + kGnBatch), cross = count * share;
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                float s = 0.f, q = 0.f;
+#pragma unroll
+                for (int u = 0; u < kGnBatch; ++u) s += (float) v[u][j];
+                s *= 1.f / kGnBatch;
+#pragma unroll
+                for (int u = 0; u < kGnBatch; ++u) q = __builtin_fmaf((float) v[u][j] - s, (float) v[u][j] - s, q);
+                const float d = s - mean[j];
+                mean[j]       = __builtin_fmaf(d, share, mean[j]);
+                m2[j] += __builtin_fmaf(d * d, cross, q);
+            }
+            count += kGnBatch;
+        }
+        const int left = (np - base - pl + pls - 1) / pls; // pixels of this thread's last, shorter batch
+        if (left <= 0) return;
+        typename X::V v[kGnBatch];
+#pragma unroll
+        for (int u = 0; u < kGnBatch; ++u) v[u] = X::raw(a, n, p0 + min(base + pl + u * pls, np - 1), cv);
+        __builtin_amdgcn_sched_barrier(0);
+        const float k = (float) left, share = k * __builtin_amdgcn_rcpf(count + k), cross = count * share, ik = 1.f / k;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+            float s = 0.f, q = 0.f;
+#pragma unroll
+            for (int u = 0; u < kGnBatch; ++u) s += u < left ? (float) v[u][j] : 0.f;
+            s *= ik;
+#pragma unroll
+            for (int u = 0; u < kGnBatch; ++u) q += u < left ? ((float) v[u][j] - s) * ((float) v[u][j] - s) : 0.f;
+            const float d = s - mean[j];
+            mean[j]       = __builtin_fmaf(d, share, mean[j]);
+            m2[j] += __builtin_fmaf(d * d, cross, q);
+        }
+    }
+    __device__ __forceinline__ float gn_thread_count(int np, int pl, int pls) { return pl < np ? (float) ((np - pl + pls - 1) / pls) : 0.f; }
+
+    // Statistics of a chunk of pixels into a.part: (mean, M2) of every channel from NC4HW4, where a wave is 64
+    // pixels of one block of channels, and of every group from NHWC, where the threads' channels meet in LDS.
     template <typename T, int VEC, bool XN4, bool XAL>
     __global__ __launch_bounds__(kGnThreads) void gn_stats_kernel(GnArgs a) {
         extern __shared__ float sm[];
-        Moments *ent = reinterpret_cast<Moments *>(sm);                    // [pixel lane][channel of the pass]
-        float2  *ch  = reinterpret_cast<float2 *>(sm + 3 * kGnThreads * VEC); // (mean, M2) of every channel over the chunk
+        float2      *ent = reinterpret_cast<float2 *>(sm);
         const int    n = blockIdx.y, p0 = blockIdx.x * a.chunk, np = min(a.chunk, a.HW - p0);
         const GnLane L = gn_lane<XN4>(a);
-        for (int base = 0; base < a.CV; base += L.cvs) {
-            const int cv = base + L.cv;
-            if (L.pl < L.pls) {
-                Moments m[VEC];
+        float        mean[VEC], m2[VEC];
+        if constexpr (XN4) {
+            const int cv = blockIdx.z * L.cvs + L.cv;
+            if (cv >= a.CV) return;
+            gn_thread_moments<T, VEC, XN4, XAL>(a, n, p0, np, cv, L.pl, L.pls, mean, m2);
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) m[j] = {0.f, 0.f, 0.f};
-                if (cv < a.CV)
-                    for (int p = L.pl; p < np; p += L.pls * kGnBatch) {
-                        float v[kGnBatch][VEC];
-                        int   k = 0;
-#pragma unroll
-                        for (int u = 0; u < kGnBatch; ++u) {
-                            const bool in = p + u * L.pls < np;
-                            k += in;
-                            GnIo<T, VEC, XN4, XAL>::load(a, n, p0 + (in ? p + u * L.pls : p), cv, v[u]);
-                        }
-#pragma unroll
-                        for (int j = 0; j < VEC; ++j) {
-                            float s = 0.f, q = 0.f;
-#pragma unroll
-                            for (int u = 0; u < kGnBatch; ++u) s += u < k ? v[u][j] : 0.f;
-                            const float mean = s / (float) k;
-#pragma unroll
-                            for (int u = 0; u < kGnBatch; ++u) q += u < k ? (v[u][j] - mean) * (v[u][j] - mean) : 0.f;
-                            m[j] = merge(m[j], {(float) k, mean, q});
-                        }
-                    }
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) ent[(L.pl * L.cvs + L.cv) * VEC + j] = m[j];
+            for (int j = 0; j < VEC; ++j) {
+                const Moments m = merge_lanes({gn_thread_count(np, L.pl, L.pls), mean[j], m2[j]}, 64);
+                if (L.pl == 0 && cv * VEC + j < a.C) a.part[((int64_t) n * a.chunks + blockIdx.x) * a.C + cv * VEC + j] = make_float2(m.mean, m.m2);
             }
-            __syncthreads();
-            for (int c = threadIdx.x; c < L.cvs * VEC && base * VEC + c < a.C; c += kGnThreads) {
-                Moments m = {0.f, 0.f, 0.f};
-                for (int r = 0; r < L.pls; ++r) m = merge(m, ent[r * L.cvs * VEC + c]);
-                ch[base * VEC + c] = make_float2(m.mean, m.m2);
-            }
-            __syncthreads();
+            return;
         }
-        int lanes = 64;
+        const int width = (a.CV < kGnThreads ? L.cvs : a.CV) * VEC; // channels of a row of entries
+        for (int cv = L.cv; cv < a.CV; cv += L.cvs) {
+            if (L.pl >= L.pls) break;
+            gn_thread_moments<T, VEC, XN4, XAL>(a, n, p0, np, cv, L.pl, L.pls, mean, m2);
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) ent[L.pl * width + cv * VEC + j] = make_float2(mean[j], m2[j]);
+        }
+        __syncthreads();
+        const int rows = L.pls;
+        int       lanes = 64;
         while (lanes > 1 && lanes * a.G > kGnThreads) lanes >>= 1;
         for (int g0 = 0; g0 < a.G; g0 += kGnThreads / lanes) {
             const int g = g0 + threadIdx.x / lanes;
             Moments   m = {0.f, 0.f, 0.f};
             if (g < a.G)
-                for (int c = threadIdx.x % lanes; c < a.Cg; c += lanes) m = merge(m, {(float) np, ch[g * a.Cg + c].x, ch[g * a.Cg + c].y});
+                for (int i = threadIdx.x % lanes; i < rows * a.Cg; i += lanes) {
+                    const int    r = i / a.Cg, c = g * a.Cg + i - r * a.Cg;
+                    const float2 e = ent[r * width + c];
+                    m              = merge(m, {gn_thread_count(np, r, rows), e.x, e.y});
+                }
             m = merge_lanes(m, lanes);
             if (g < a.G && threadIdx.x % lanes == 0) a.part[((int64_t) n * a.chunks + blockIdx.x) * a.G + g] = make_float2(m.mean, m.m2);
         }
@@ -148,64 +208,226 @@ namespace vkhip {
     __global__ __launch_bounds__(kGnThreads) void gn_apply_kernel(GnArgs a) {
         extern __shared__ float sm[];
         float2   *st = reinterpret_cast<float2 *>(sm); // (mean, rstd) of every group
-        const int n = blockIdx.y, p0 = blockIdx.x * a.chunk, np = min(a.chunk, a.HW - p0);
+        // last image first: what the statistics read last is still in the caches
+        const int n = gridDim.y - 1 - blockIdx.y, p0 = (gridDim.x - 1 - blockIdx.x) * a.chunk, np = min(a.chunk, a.HW - p0);
+        // the groups of the workgroup's channels
+        const int g_first = XN4 ? blockIdx.z * (kGnThreads / 64) * VEC / a.Cg : 0;
+        const int gs      = XN4 ? min(a.G - 1, (((int) blockIdx.z + 1) * (kGnThreads / 64) * VEC - 1) / a.Cg) - g_first + 1 : a.G;
+        const int per = XN4 ? a.Cg : 1, row = XN4 ? a.C : a.G; // entries of a group in a chunk, of a chunk
         int       lanes = 64;
-        while (lanes > 1 && lanes * a.G > kGnThreads) lanes >>= 1;
-        for (int g0 = 0; g0 < a.G; g0 += kGnThreads / lanes) {
+        while (lanes > 1 && lanes * gs > kGnThreads) lanes >>= 1;
+        for (int g0 = 0; g0 < gs; g0 += kGnThreads / lanes) {
             const int g = g0 + threadIdx.x / lanes;
             Moments   m = {0.f, 0.f, 0.f};
-            if (g < a.G)
-                for (int k = threadIdx.x % lanes; k < a.chunks; k += lanes) {
-                    const float2 q = a.part[((int64_t) n * a.chunks + k) * a.G + g];
-                    m              = merge(m, {(float) min(a.chunk, a.HW - k * a.chunk) * (float) a.Cg, q.x, q.y});
+            if (g < gs)
+                for (int i = threadIdx.x % lanes; i < a.chunks * per; i += lanes) {
+                    const int    k = i / per;
+                    const float2 q = a.part[((int64_t) n * a.chunks + k) * row + (g_first + g) * per + i - k * per];
+                    m              = merge(m, {(float) min(a.chunk, a.HW - k * a.chunk) * (XN4 ? 1.f : (float) a.Cg), q.x, q.y});
                 }
             m = merge_lanes(m, lanes);
-            if (g < a.G && threadIdx.x % lanes == 0) st[g] = make_float2(m.mean, 1.f / sqrtf(m.m2 / m.n + a.eps));
+            if (g < gs && threadIdx.x % lanes == 0) st[g] = make_float2(m.mean, 1.f / sqrtf(m.m2 / m.n + a.eps));
         }
         __syncthreads();
         const GnLane L = gn_lane<XN4>(a);
         if (L.pl >= L.pls) return;
-        for (int cv = L.cv; cv < a.CV; cv += L.cvs) {
+        for (int cv = XN4 ? blockIdx.z * L.cvs + L.cv : L.cv; cv < (XN4 ? min(a.CV, ((int) blockIdx.z + 1) * L.cvs) : a.CV); cv += L.cvs) {
             float mean[VEC], mul[VEC], add[VEC];
 #pragma unroll
             for (int j = 0; j < VEC; ++j) {
-                const int c = min(cv * VEC + j, a.C - 1), g = c / a.Cg;
+                const int c = min(cv * VEC + j, a.C - 1), g = c / a.Cg - g_first;
                 mean[j]     = st[g].x;
                 mul[j]      = st[g].y * (a.gamma ? a.gamma[c] : 1.f);
                 add[j]      = a.beta ? a.beta[c] : 0.f;
             }
-            for (int p = L.pl; p < np; p += L.pls * kGnBatch) {
-                float v[kGnBatch][VEC];
+            gn_by_kind(a.kind, [&](auto kind) __attribute__((always_inline)) {
+                using X        = GnIo<T, VEC, XN4, XAL>;
+                const int step = L.pls * kGnBatch;
+                const auto put = [&](const typename X::V &x, int p) __attribute__((always_inline)) {
+                    float v[VEC];
 #pragma unroll
-                for (int u = 0; u < kGnBatch; ++u) GnIo<T, VEC, XN4, XAL>::load(a, n, p0 + (p + u * L.pls < np ? p + u * L.pls : p), cv, v[u]);
+                    for (int j = 0; j < VEC; ++j) v[j] = gn_act<decltype(kind)::value>(a, ((float) x[j] - mean[j]) * mul[j] + add[j]);
+                    GnIo<T, VEC, YN4, YAL>::store(a, n, p0 + p, cv, v);
+                };
+                int base = 0;
+                for (; base + step <= np; base += step) {
+                    typename X::V x[kGnBatch];
 #pragma unroll
-                for (int u = 0; u < kGnBatch; ++u) {
-                    if (p + u * L.pls >= np) break;
+                    for (int u = 0; u < kGnBatch; ++u) x[u] = X::raw(a, n, p0 + base + L.pl + u * L.pls, cv);
+                    __builtin_amdgcn_sched_barrier(0); // the loads stay ahead of the first use
 #pragma unroll
-                    for (int j = 0; j < VEC; ++j) v[u][j] = apply_act((v[u][j] - mean[j]) * mul[j] + add[j], a.act, a.lo, a.hi);
-                    GnIo<T, VEC, YN4, YAL>::store(a, n, p0 + p + u * L.pls, cv, v[u]);
+                    for (int u = 0; u < kGnBatch; ++u) put(x[u], base + L.pl + u * L.pls);
                 }
-            }
+                if (base + L.pl >= np) return;
+                typename X::V x[kGnBatch]; // fewer than eight are left
+#pragma unroll
+                for (int u = 0; u < kGnBatch; ++u) x[u] = X::raw(a, n, p0 + min(base + L.pl + u * L.pls, np - 1), cv);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int u = 0; u < kGnBatch; ++u)
+                    if (base + L.pl + u * L.pls < np) put(x[u], base + L.pl + u * L.pls);
+            });
         }
+    }
+
+    // Sums of a wave and of a workgroup; the latter in a fixed order, the same in every thread.
+    template <int CTRL>
+    __device__ __forceinline__ float dpp_add(float x) {
+        return x + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xF, 0xF, true));
+    }
+    __device__ __forceinline__ float wave_sum(float x) {
+        x = dpp_add<0x111>(x); // row_shr 1, 2, 4, 8: lane 15 of each 16 has its row
+        x = dpp_add<0x112>(x);
+        x = dpp_add<0x114>(x);
+        x = dpp_add<0x118>(x);
+        x = dpp_add<0x142>(x); // row_bcast 15, 31: lane 63 has them all
+        x = dpp_add<0x143>(x);
+        return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), 63));
+    }
+    template <int THREADS, int GS>
+    __device__ __forceinline__ void block_sums(float (&x)[GS], float (*red)[GS]) {
+#pragma unroll
+        for (int g = 0; g < GS; ++g) {
+            x[g] = wave_sum(x[g]);
+            if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6][g] = x[g];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int g = 0; g < GS; ++g) {
+            x[g] = red[0][g];
+#pragma unroll
+            for (int w = 1; w < THREADS / 64; ++w) x[g] += red[w][g];
+        }
+    }
+
+    // One launch: a workgroup owns a slab of one image and keeps all of its pixels in registers: mean, then
+    // deviations from it, then the output, x read once. A slab is a group of SV whole vectors of channels or
+    // (GV > 1) a vector of GV whole groups. Slabs of several groups side by side, whose rows' pieces are longer,
+    // were slower (64 x 256 x 28 x 28: 34 us with four groups, 24 with one): one workgroup a compute unit has nothing
+    // to read while it writes.
+    template <typename T, int VEC, bool XN4, bool YN4, bool XAL, bool YAL, int THREADS, int R, int GV>
+    __global__ __launch_bounds__(THREADS) void gn_slab_kernel(GnArgs a, int SV, int slabs, int spread) {
+        using X             = GnIo<T, VEC, XN4, XAL>;
+        constexpr int SHARE = VEC / GV; // channels of a vector in one group
+        __shared__ float red[2][THREADS / 64][GV];
+        // images over the XCDs, the slabs of one on the same: their pieces of a cache line meet in its L2
+        const int n = blockIdx.x / (slabs * spread) * spread + blockIdx.x % spread, slab = blockIdx.x / spread % slabs;
+        if (n >= a.N) return;
+        const int pls = THREADS / SV, v = XN4 ? threadIdx.x / pls : threadIdx.x % SV, pl = XN4 ? threadIdx.x % pls : threadIdx.x / SV;
+        const int cv = slab * SV + v;
+        // pixels of this thread; the loads of the others repeat the last pixel
+        const int mine = (int) threadIdx.x < pls * SV && cv < a.CV && pl < a.HW ? (a.HW - pl + pls - 1) / pls : 0;
+        typename X::V x[R];
+#pragma unroll
+        for (int k = 0; k < R; ++k) x[k] = X::raw(a, n, min(pl + k * pls, a.HW - 1), min(cv, a.CV - 1));
+        __builtin_amdgcn_sched_barrier(0); // the loads stay ahead of the first use
+        float       mean[GV], m2[GV];
+        const float count = (float) a.HW * (float) a.Cg;
+#pragma unroll
+        for (int pass = 0; pass < 2; ++pass) {
+            float sum[GV];
+#pragma unroll
+            for (int g = 0; g < GV; ++g) sum[g] = 0.f;
+#pragma unroll
+            for (int k = 0; k < R; ++k)
+#pragma unroll
+                for (int g = 0; g < GV; ++g) {
+                    float part = 0.f;
+#pragma unroll
+                    for (int j = 0; j < SHARE; ++j) {
+                        const bool  lost = XN4 && SHARE * g + j + cv * VEC >= a.C; // past the channels
+                        const float d    = lost ? 0.f : (float) x[k][SHARE * g + j] - (pass ? mean[g] : 0.f);
+                        part             = pass ? __builtin_fmaf(d, d, part) : part + d;
+                    }
+                    sum[g] += k < mine ? part : 0.f;
+                }
+            block_sums<THREADS, GV>(sum, red[pass]);
+#pragma unroll
+            for (int g = 0; g < GV; ++g) (pass ? m2 : mean)[g] = sum[g] / count;
+        }
+        float mul[VEC], be[VEC];
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+            const int c = min(cv * VEC + j, a.C - 1);
+            mul[j]      = (a.gamma ? a.gamma[c] : 1.f) / sqrtf(m2[j / SHARE] + a.eps);
+            be[j]       = a.beta ? a.beta[c] : 0.f;
+        }
+        gn_by_kind(a.kind, [&](auto kind) __attribute__((always_inline)) {
+#pragma unroll
+            for (int k = 0; k < R; ++k) {
+                float o[VEC];
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) o[j] = gn_act<decltype(kind)::value>(a, ((float) x[k][j] - mean[j / SHARE]) * mul[j] + be[j]);
+                if (k < mine) GnIo<T, VEC, YN4, YAL>::store(a, n, pl + k * pls, cv, o);
+            }
+        });
+    }
+
+    // How the one-launch kernel cuts a norm; threads 0: two launches.
+    struct GnSlab {
+        int vectors, groups, threads, pixels; // SV, GV, and a thread's pixels
+    };
+    // Where a slab fits, it is taken from NC4HW4 always (its planes are contiguous; 8 x 108 x 75 x 75 to rows 12.1 us
+    // against 18.3 with two launches, 16 x 128 x 80 x 80 19.5 against 23.4), and from NHWC by the two sides' times as
+    // measured, in us: 4 and 1 + 3 / SV ns a vector and compute unit (a row's piece of SV vectors costs whole cache
+    // lines), against 11.5 and three passes over the tensor at 5.5 TB/s. Measured slab / two launches:
+    // 1 x 128 x 40 x 40 5.7 / 13.0, 8 x 512 x 28 x 28 6.8 / 15.0, 64 x 256 x 28 x 28 23.8 / 27.4,
+    // 1 x 64 x 80 x 80 20.9 / 14.9, 64 x 256 x 56 x 56 101.6 / 75.1.
+    static GnSlab gn_slab(const GnArgs &a, int vec, int size, bool planes) {
+        if (a.Cg % vec && vec % a.Cg) return {0, 0, 0, 0};
+        const int    sv      = a.Cg < vec ? 1 : a.Cg / vec;
+        const double vectors = (double) a.HW * sv * (double) ceil_div((int64_t) a.N * ceil_div(a.CV, sv), 256);
+        if (!planes && 4 + vectors * (1 + 3. / sv) * 1e-3 > 11.5 + 3. * size * a.N * a.C * (double) a.HW / 5.5e6) return {0, 0, 0, 0};
+        for (int threads: {256, 1024}) {
+            const int r = sv > threads ? 99 : (int) ceil_div(a.HW, threads / sv);
+            if (r <= (threads == 256 ? 8 : 16)) return {sv, a.Cg < vec ? vec / a.Cg : 1, threads, r <= 8 ? 8 : 16};
+        }
+        return {0, 0, 0, 0};
+    }
+
+    template <typename T, int VEC, bool XN4, bool YN4, bool XAL, bool YAL, int GV>
+    static int gn_slab_launch(const GnArgs &a, const GnSlab &c, hipStream_t s) {
+        const int  slabs = (int) ceil_div(a.CV, c.vectors), spread = a.N >= 8 ? 8 : 1;
+        const dim3 grid((unsigned) (round_up(a.N, spread) * slabs));
+        if (c.threads == 256) gn_slab_kernel<T, VEC, XN4, YN4, XAL, YAL, 256, 8, GV><<<grid, 256, 0, s>>>(a, c.vectors, slabs, spread);
+        else if (c.pixels == 8) gn_slab_kernel<T, VEC, XN4, YN4, XAL, YAL, 1024, 8, GV><<<grid, 1024, 0, s>>>(a, c.vectors, slabs, spread);
+        else gn_slab_kernel<T, VEC, XN4, YN4, XAL, YAL, 1024, 16, GV><<<grid, 1024, 0, s>>>(a, c.vectors, slabs, spread);
+        return check_launch("group_norm");
     }
 
     template <typename T, int VEC, bool XN4, bool YN4, bool XAL, bool YAL>
     static int gn_launch(const GnArgs &a, hipStream_t s) {
-        const dim3 grid((unsigned) a.chunks, (unsigned) a.N);
-        gn_stats_kernel<T, VEC, XN4, XAL><<<grid, kGnThreads, (3 * kGnThreads * VEC + 2 * a.C) * sizeof(float), s>>>(a);
+        const GnSlab c = gn_slab(a, VEC, (int) sizeof(T), XN4);
+        if (c.threads) {
+            if (c.groups == 1) return gn_slab_launch<T, VEC, XN4, YN4, XAL, YAL, 1>(a, c, s);
+            if constexpr (VEC >= 4) {
+                if (c.groups == 2) return gn_slab_launch<T, VEC, XN4, YN4, XAL, YAL, 2>(a, c, s);
+                if (c.groups == 4) return gn_slab_launch<T, VEC, XN4, YN4, XAL, YAL, 4>(a, c, s);
+            }
+            if constexpr (VEC >= 8) return gn_slab_launch<T, VEC, XN4, YN4, XAL, YAL, 8>(a, c, s);
+        }
+        const dim3   grid((unsigned) a.chunks, (unsigned) a.N, XN4 ? (unsigned) ceil_div(a.CV, kGnThreads / 64) : 1u);
+        const size_t lds = XN4 ? 0 : (size_t) (a.CV > kGnThreads ? a.CV : kGnThreads) * VEC; // entries
+        gn_stats_kernel<T, VEC, XN4, XAL><<<grid, kGnThreads, lds * sizeof(float2), s>>>(a);
         int rc = check_launch("group_norm statistics");
         if (rc) return rc;
         gn_apply_kernel<T, VEC, XN4, YN4, XAL, YAL><<<grid, kGnThreads, 2 * a.G * sizeof(float), s>>>(a);
         return check_launch("group_norm");
     }
 
-    static int gn_chunks(const vkhip_group_norm_desc *d) {
-        const int64_t hw = (int64_t) d->H * d->W;
-        int64_t       k  = ceil_div(1024, d->N);
+    // Pixels of a chunk: workgroups for every compute unit, whole batches of the threads' pixels where there are
+    // enough, and no more than 128 chunks or so, since each workgroup of the second launch joins them all.
+    static int gn_chunk(const vkhip_group_norm_desc *d) {
+        const int64_t hw = (int64_t) d->H * d->W, vectors = ceil_div((int64_t) d->C * (d->dtype == VKHIP_DT_F32 ? 4 : 2), 16);
+        const int64_t batch = kGnBatch * (d->x_fmt == 2 ? 64 : kGnThreads / (vectors < kGnThreads ? vectors : kGnThreads));
+        int64_t       k = ceil_div(1024, d->N);
         if (k > 128) k = 128;
-        if (k > ceil_div(hw, 32)) k = ceil_div(hw, 32);
-        const int64_t chunk = ceil_div(hw, k);
-        return (int) ceil_div(hw, chunk);
+        const int64_t least = d->x_fmt == 2 ? batch : 32;
+        if (k > ceil_div(hw, least)) k = ceil_div(hw, least);
+        int64_t chunk = ceil_div(hw, k);
+        if (chunk >= batch) chunk -= chunk % batch;
+        else if (chunk * 2 > batch) chunk = batch;
+        return (int) chunk;
     }
 
     static const char *gn_refusal(const vkhip_group_norm_desc *d) {
@@ -229,7 +451,7 @@ extern "C" {
 
 size_t vkhip_group_norm_workspace_bytes(const vkhip_group_norm_desc *d) {
     if (gn_refusal(d) || d->N == 0 || d->H == 0 || d->W == 0) return 0;
-    return (size_t) d->N * gn_chunks(d) * d->groups * sizeof(float2);
+    return (size_t) d->N * ceil_div((int64_t) d->H * d->W, gn_chunk(d)) * (d->x_fmt == 2 ? d->C : d->groups) * sizeof(float2);
 }
 
 int vkhip_group_norm(const vkhip_group_norm_desc *d, const void *x, const float *gamma, const float *beta, void *y, void *workspace,
@@ -245,9 +467,19 @@ int vkhip_group_norm(const vkhip_group_norm_desc *d, const void *x, const float 
     a.x = x, a.y = y, a.gamma = gamma, a.beta = beta, a.part = (float2 *) workspace;
     a.N = d->N, a.C = d->C, a.HW = d->H * d->W, a.G = d->groups, a.Cg = d->C / d->groups;
     a.x_row = d->x_row ? d->x_row : d->C, a.y_row = d->y_row ? d->y_row : d->C;
-    a.act = d->act, a.lo = d->act_lo, a.hi = d->act_hi, a.eps = d->eps;
-    a.chunks      = gn_chunks(d);
-    a.chunk       = (int) ceil_div(a.HW, a.chunks);
+    const float inf = __builtin_inff();
+    a.kind = 0, a.s = 1.f, a.t = 0.f, a.lo = -inf, a.hi = inf, a.eps = d->eps;
+    switch (d->act) {
+        case VKHIP_ACT_RELU: a.lo = 0.f; break;
+        case VKHIP_ACT_RELU6: a.lo = 0.f, a.hi = 6.f; break;
+        case VKHIP_ACT_CLIP: a.lo = d->act_lo, a.hi = d->act_hi; break;
+        case VKHIP_ACT_HARDSWISH: a.kind = 1, a.s = 1.f / 6.f, a.t = 0.5f, a.lo = 0.f, a.hi = 1.f; break;
+        case VKHIP_ACT_SILU: a.kind = 2; break;
+        case VKHIP_ACT_HARDSIGMOID: a.s = d->act_lo, a.t = d->act_hi, a.lo = 0.f, a.hi = 1.f; break;
+        default: break;
+    }
+    a.chunk       = gn_chunk(d);
+    a.chunks      = (int) ceil_div(a.HW, a.chunk);
     hipStream_t q = resolve_stream(s);
     // the widest vector that divides the channels and that both sides' rows start on
     const auto fits = [&](int vec, bool side_x, bool side_y) {
