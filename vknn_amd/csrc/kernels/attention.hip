@@ -9,6 +9,7 @@
 // K and V tiles of 64 keys go from memory into LDS without passing registers, one tile ahead; rows are stored
 // with their 16-byte pieces permuted (xor with the row) so that neither read pattern meets a bank twice.
 #include "tokens.h"
+#include <type_traits>
 
 namespace vkhip {
 
@@ -27,7 +28,7 @@ namespace vkhip {
     struct AttnType<half_t> {
         typedef half8 V8;
         typedef half4 V4;
-        static constexpr unsigned kExp = 0x7C00u;
+        static constexpr unsigned kExp = 0x7C00u; // bits of infinity
         static __device__ __forceinline__ float16v mfma(V8 a, V8 b, float16v c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
     };
     template <>
@@ -40,38 +41,44 @@ namespace vkhip {
 
     constexpr int kAttnQ = 128, kAttnK = 64;
 
-    typedef short attn_s4 __attribute__((ext_vector_type(4)));
-    // 4 x 16 values of 16 bits per 16 lanes, transposed: lane i of the 16 points at 4 values of row i / 4 (columns
-    // 4 (i % 4) ..) and gets column i, rows 0 .. 3.
-    __device__ __forceinline__ uint2 lds_read_tr(const unsigned char *p) {
-#if defined(__HIP_DEVICE_COMPILE__) // the host pass rejects a generic pointer's cast to the LDS space
-        const attn_s4 t = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) attn_s4 *) (p));
-        return __builtin_bit_cast(uint2, t);
-#else
-        return {};
-#endif
-    }
-    // 16 bytes a lane from `off` past the resource's base to `dst` + 16 * lane
-    __device__ __forceinline__ void copy_to_lds(__amdgpu_buffer_rsrc_t r, unsigned char *dst, unsigned off) {
-#if defined(__HIP_DEVICE_COMPILE__)
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void *) dst, 16, off, 0, 0, 0);
-#endif
-    }
-
-    // Where a 16-byte piece of a row lies in a tile's LDS image. K is read by 32 rows at one piece, V by 8 rows at 4.
+    // Which 16-byte piece of a tile's LDS row `row` holds the row's piece `piece`. K is read by 32 rows at one piece,
+    // V by 8 rows at 4 neighbouring ones.
     template <int DP>
     __device__ __forceinline__ int k_swizzle(int row) { return DP == 128 ? row & 15 : row >> 1 & 7; }
     template <int DP>
     __device__ __forceinline__ int v_swizzle(int row) { return DP == 128 ? (row & 3) << 2 | (row >> 2 & 3) : (row >> 1 & 1) << 2; }
 
+    // The larger of a lane's value and that of lane ^ 32.
+    __device__ __forceinline__ float max_halves(float x) {
+        const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+        return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    }
+
+#if defined(__HIP_DEVICE_COMPILE__) // the host pass knows neither the LDS address space of these nor the reads
+    typedef __attribute__((address_space(3))) unsigned char *LdsPtr;
+    typedef short attn_s4 __attribute__((ext_vector_type(4)));
+
+    // 4 x 16 values of 16 bits per 16 lanes, transposed: lane i of the 16 points at 4 values of row i / 4 (columns
+    // 4 (i % 4) ..) and gets column i, rows 0 .. 3.
+    __device__ __forceinline__ tk_u32x2 lds_read_tr(LdsPtr p) {
+        return __builtin_bit_cast(tk_u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) attn_s4 *) p));
+    }
+    __device__ __forceinline__ tk_u32x4 lds_read16(LdsPtr p) { return *(__attribute__((address_space(3))) const tk_u32x4 *) p; }
+
+#endif
+
     template <typename T, int DP>
     __global__ __launch_bounds__(256, 2) void attn_packed_kernel(AttnArgs a) {
+#if defined(__HIP_DEVICE_COMPILE__)
         using A              = AttnType<T>;
+        using V8             = typename A::V8;
         constexpr int PIECES = DP / 8;            // 16-byte pieces of a row
-        constexpr int TILE   = kAttnK * DP * 2;   // bytes of a K or V tile
+        constexpr int ROW    = DP * 2;            // bytes of a row
+        constexpr int TILE   = kAttnK * ROW;      // bytes of a K or V tile
         constexpr int LOADS  = TILE / 1024 / 4;   // wave loads of 1 KB per wave and tile
         constexpr int KS = DP / 16, DB = DP / 32; // contraction steps of a score, 32-channel blocks of the output
-        __shared__ __attribute__((aligned(1024))) unsigned char sm[2][2][TILE];
+        __shared__ __attribute__((aligned(1024))) unsigned char sm[4 * TILE + 4 * kAttnK * 64]; // K, V of even tiles, K, V of odd ones, a wave's weights
+        LdsPtr lds = (LdsPtr) sm;
 
         const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, col = lane & 31;
         // heads of one key/value head next to each other in the grid: workgroups go to the 8 XCDs in turn
@@ -91,14 +98,15 @@ namespace vkhip {
 
         const int qi    = i0 + wave * 32 + col;
         const int limit = qi < nq ? (a.causal ? qi + shift + 1 : nk) : 0; // keys below it are seen
-        const int i_last = min(i0 + kAttnQ, nq) - 1;
-        const int k_end  = max(0, a.causal ? min(nk, i_last + shift + 1) : nk);
-        // the wave's own range: all its queries see keys below `low`, none sees any from `high`
-        const int w_first = i0 + wave * 32, w_last = min(w_first + 32, nq) - 1;
+        const int k_end = max(0, a.causal ? min(nk, min(i0 + kAttnQ, nq) + shift) : nk);
+        const int tiles = (k_end + kAttnK - 1) / kAttnK;
+        // the wave's own tiles: `plain` of them seen whole by all its queries, none of use from `used` on
+        const int w_first = __builtin_amdgcn_readfirstlane(i0 + wave * 32), w_last = min(w_first + 32, nq) - 1;
         const int low = w_first + 31 < nq ? (a.causal ? w_first + shift + 1 : nk) : 0;
         const int high = w_first < nq ? (a.causal ? min(nk, w_last + shift + 1) : nk) : 0;
+        const int plain = max(0, low) / kAttnK, used = (max(0, high) + kAttnK - 1) / kAttnK;
 
-        typename A::V8 qf[KS];
+        V8 qf[KS];
         {
             const T *src = (const T *) a.q + (int64_t) (q0 + qi) * a.q_row + (int64_t) head_q * a.q_head;
 #pragma unroll
@@ -106,82 +114,87 @@ namespace vkhip {
                 const int d = 16 * s + 8 * h;
 #pragma unroll
                 for (int j = 0; j < 8; ++j) qf[s][j] = (T) 0.f;
-                if (qi < nq && d < D) qf[s] = *reinterpret_cast<const typename A::V8 *>(src + d);
+                if (qi < nq && d < D) qf[s] = *reinterpret_cast<const V8 *>(src + d);
             }
         }
 
-        const T *kb = (const T *) a.k + (int64_t) k0 * a.k_row + (int64_t) head_kv * a.k_head;
-        const T *vb = (const T *) a.v + (int64_t) k0 * a.v_row + (int64_t) head_kv * a.v_head;
+        const char *kb = (const char *) ((const T *) a.k + (int64_t) k0 * a.k_row + (int64_t) head_kv * a.k_head);
+        const char *vb = (const char *) ((const T *) a.v + (int64_t) k0 * a.v_row + (int64_t) head_kv * a.v_head);
+        const int   k_bytes = (int) a.k_row * 2, v_bytes = (int) a.v_row * 2;
         // this lane's source offsets: piece p of the LDS image is row p / PIECES, piece (p % PIECES) ^ swizzle(row)
         unsigned off_k[LOADS], off_v[LOADS];
-        int      row_of[LOADS];
 #pragma unroll
         for (int r = 0; r < LOADS; ++r) {
             const int p = (wave * LOADS + r) * 64 + lane, row = p / PIECES, at = p % PIECES;
             const int ck = at ^ k_swizzle<DP>(row), cv = at ^ v_swizzle<DP>(row);
-            row_of[r]    = row;
-            off_k[r]     = ck * 8 < D ? (unsigned) (row * a.k_row * 2 + ck * 16) : 0x80000000u;
-            off_v[r]     = cv * 8 < D ? (unsigned) (row * a.v_row * 2 + cv * 16) : 0x80000000u;
+            off_k[r]     = ck * 8 < D ? (unsigned) (row * k_bytes + ck * 16) : 0x80000000u;
+            off_v[r]     = cv * 8 < D ? (unsigned) (row * v_bytes + cv * 16) : 0x80000000u;
         }
-        // past the last row of the sequence, and past the head's channels, the copy writes zeros
+        // past the sequence's last row, where the resource ends, and past the head's channels the copy writes zeros
         auto issue = [&](int t) __attribute__((always_inline)) {
-            const int valid = min(kAttnK, nk - t * kAttnK);
-            const __amdgpu_buffer_rsrc_t kr = __builtin_amdgcn_make_buffer_rsrc((void *) (kb + (int64_t) t * kAttnK * a.k_row), (short) 0, 0x7FFFFFFF, 0x00020000);
-            const __amdgpu_buffer_rsrc_t vr = __builtin_amdgcn_make_buffer_rsrc((void *) (vb + (int64_t) t * kAttnK * a.v_row), (short) 0, 0x7FFFFFFF, 0x00020000);
+            const int rows = min(kAttnK, nk - t * kAttnK) - 1;
+            const __amdgpu_buffer_rsrc_t kr =
+                __builtin_amdgcn_make_buffer_rsrc((void *) (kb + (int64_t) t * kAttnK * k_bytes), (short) 0, rows * k_bytes + D * 2, 0x00020000);
+            const __amdgpu_buffer_rsrc_t vr =
+                __builtin_amdgcn_make_buffer_rsrc((void *) (vb + (int64_t) t * kAttnK * v_bytes), (short) 0, rows * v_bytes + D * 2, 0x00020000);
+            LdsPtr dst = lds + (t & 1) * (2 * TILE) + wave * (LOADS * 1024);
 #pragma unroll
-            for (int r = 0; r < LOADS; ++r) {
-                const bool in = row_of[r] < valid;
-                copy_to_lds(kr, sm[t & 1][0] + (wave * LOADS + r) * 1024, in ? off_k[r] : 0x80000000u);
-                copy_to_lds(vr, sm[t & 1][1] + (wave * LOADS + r) * 1024, in ? off_v[r] : 0x80000000u);
-            }
+            for (int r = 0; r < LOADS; ++r) __builtin_amdgcn_raw_ptr_buffer_load_lds(kr, dst + r * 1024, 16, off_k[r], 0, 0, 0);
+#pragma unroll
+            for (int r = 0; r < LOADS; ++r) __builtin_amdgcn_raw_ptr_buffer_load_lds(vr, dst + TILE + r * 1024, 16, off_v[r], 0, 0, 0);
         };
+
+        // fragment addresses of an even tile: K row col, piece 2 c + h; V rows 4 h + (lane % 16) / 4 (+ 8), pieces 4 d + pp.
+        // The swizzle is an xor of disjoint bits, so that rows further on are constant offsets.
+        LdsPtr ka[KS], va[DB][2];
+#pragma unroll
+        for (int c = 0; c < KS; ++c) ka[c] = lds + col * ROW + (((2 * c + h) ^ k_swizzle<DP>(col)) << 4);
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int row = 4 * h + ((lane & 15) >> 2) + 8 * e, piece = 4 * d + 2 * (lane >> 4 & 1) + ((lane & 3) >> 1);
+                va[d][e]      = lds + TILE + row * ROW + ((piece ^ v_swizzle<DP>(row)) << 4) + (lane & 1) * 8;
+            }
 
         float16v acc[DB];
 #pragma unroll
         for (int d = 0; d < DB; ++d)
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[d][r] = 0.f;
+        // the reference of the exponents, at most 8 below the largest one seen: weights up to 2^8 cost no digits, and
+        // O is rescaled only where a maximum grows by more than that
         float m = -__builtin_inff(), l = 0.f;
 
-        const int tiles = (k_end + kAttnK - 1) / kAttnK;
-        if (tiles > 0) issue(0);
-        for (int t = 0; t < tiles; ++t) {
-            __builtin_amdgcn_s_waitcnt(7 << 4);         // vmcnt(0), lgkmcnt(0): its pieces of tile t have landed, its reads of t - 1 too
-            __asm__ volatile("s_barrier" ::: "memory");       // everybody's have, and nobody reads tile t - 1 any more
-            if (t + 1 < tiles) issue(t + 1);
-            const int key0 = t * kAttnK;
-            if (key0 >= high) continue;
-            const unsigned char *kt = sm[t & 1][0], *vt = sm[t & 1][1];
-
-            float16v s[2];
+        auto tile = [&](int t, auto odd_c, auto masked_c) __attribute__((always_inline)) {
+            constexpr int  BUF    = decltype(odd_c)::value * 2 * TILE;
+            constexpr bool MASKED = decltype(masked_c)::value;
+            const int      key0   = t * kAttnK;
+            const auto     seen   = [&](int k, int j) { return key0 + 16 * k + 8 * (j >> 2) + 4 * h + (j & 3) < limit; };
+            float16v       s[2];
 #pragma unroll
             for (int kk = 0; kk < 2; ++kk) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) s[kk][r] = 0.f;
-                const int row = kk * 32 + col;
 #pragma unroll
-                for (int c = 0; c < KS; ++c) {
-                    const typename A::V8 kf = *reinterpret_cast<const typename A::V8 *>(kt + row * DP * 2 + (((2 * c + h) ^ k_swizzle<DP>(row)) << 4));
-                    s[kk]                   = A::mfma(kf, qf[c], s[kk]);
-                }
+                for (int c = 0; c < KS; ++c) s[kk] = A::mfma(__builtin_bit_cast(V8, lds_read16(ka[c] + BUF + kk * 32 * ROW)), qf[c], s[kk]);
             }
-            const bool masked = key0 + kAttnK > low;
-            if (masked) {
+            if constexpr (MASKED) {
 #pragma unroll
                 for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
                     for (int r = 0; r < 16; ++r)
-                        if (key0 + kk * 32 + 8 * (r >> 2) + 4 * h + (r & 3) >= limit) s[kk][r] = -__builtin_inff();
+                        if (!seen(2 * kk + (r >> 3), r & 7)) s[kk][r] = -__builtin_inff();
             }
             float top = s[0][0];
 #pragma unroll
             for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) top = fmaxf(top, s[kk][r]);
-            top              = fmaxf(top, __shfl_xor(top, 32));
-            const float to   = fmaxf(m, top), base = to == -__builtin_inff() ? 0.f : to * a.c2;
-            if (__any(to > m)) {
-                const float alpha = exp2_hw(m * a.c2 - base);
+            top = max_halves(top) * a.c2;
+            if (__any(top > m + 8.f)) {
+                const float to    = fmaxf(m, top);
+                const float alpha = exp2_hw(m - (to == -__builtin_inff() ? 0.f : to));
                 l *= alpha;
 #pragma unroll
                 for (int d = 0; d < DB; ++d)
@@ -189,86 +202,83 @@ namespace vkhip {
                     for (int r = 0; r < 16; ++r) acc[d][r] *= alpha;
                 m = to;
             }
-            typename A::V8 pf[4];
+            const float base = m == -__builtin_inff() ? 0.f : m;
+            V8          pf[4];
 #pragma unroll
             for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const float p = exp2_hw(__builtin_fmaf(s[kk][r], a.c2, -base));
-                    l += p;
-                    pf[kk * 2 + (r >> 3)][r & 7] = (T) p;
+                for (int r = 0; r < 16; r += 2) {
+                    typedef float F2 __attribute__((ext_vector_type(2)));
+                    typedef T     T2 __attribute__((ext_vector_type(2)));
+                    const F2      p = {exp2_hw(__builtin_fmaf(s[kk][r], a.c2, -base)), exp2_hw(__builtin_fmaf(s[kk][r + 1], a.c2, -base))};
+                    l += p[0];
+                    l += p[1];
+                    const T2 x = __builtin_convertvector(p, T2);
+                    pf[kk * 2 + (r >> 3)][r & 7]       = x[0];
+                    pf[kk * 2 + (r >> 3)][(r & 7) + 1] = x[1];
                 }
-            // V: rows 16 k + 4 h + {0 .. 3} and 8 further, channels 32 d + lane % 32
             const auto v_frag = [&](int d, int k) __attribute__((always_inline)) {
-                const int   row = 16 * k + 4 * h + ((lane & 15) >> 2), piece = 4 * d + 2 * (lane >> 4 & 1) + ((lane & 3) >> 1);
-                const uint2 x = lds_read_tr(vt + row * DP * 2 + ((piece ^ v_swizzle<DP>(row)) << 4) + (lane & 1) * 8);
-                const uint2 y = lds_read_tr(vt + (row + 8) * DP * 2 + ((piece ^ v_swizzle<DP>(row + 8)) << 4) + (lane & 1) * 8);
-                return tk_u32x4 {x.x, x.y, y.x, y.y};
+                const tk_u32x2 x = lds_read_tr(va[d][0] + BUF + k * 16 * ROW), y = lds_read_tr(va[d][1] + BUF + k * 16 * ROW);
+                return tk_u32x4 {x[0], x[1], y[0], y[1]};
             };
-            if (masked) {
-                // a weight of zero does not keep a NaN or an infinity of V out of a product: look for them where
-                // something is masked
-                unsigned odd = 0;
-#pragma unroll
-                for (int d = 0; d < DB; ++d)
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const tk_u32x4 f = v_frag(d, k);
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) odd |= (f[j] & (A::kExp * 0x10001u)) + (0x8000u - A::kExp) * 0x10001u;
-                    }
-                if (__any((odd & 0x80008000u) != 0)) {
-                    // finite values as usual; then NaN, +inf and -inf each by a product that counts the seen ones
-                    for (int kind = 0; kind < 4; ++kind) {
-                        typename A::V8 wf[4];
-#pragma unroll
-                        for (int k = 0; k < 4; ++k)
-#pragma unroll
-                            for (int j = 0; j < 8; ++j) {
-                                const int key = key0 + 16 * k + 8 * (j >> 2) + 4 * h + (j & 3);
-                                wf[k][j]      = kind ? (T) (key < limit ? 1.f : 0.f) : pf[k][j];
-                            }
-                        for (int d = 0; d < DB; ++d) {
-                            float16v x;
-#pragma unroll
-                            for (int r = 0; r < 16; ++r) x[r] = 0.f;
-                            if (kind == 0) {
-#pragma unroll
-                                for (int dd = 0; dd < DB; ++dd)
-                                    if (dd == d) x = acc[dd];
-                            }
-#pragma unroll
-                            for (int k = 0; k < 4; ++k) {
-                                tk_u32x4 f = v_frag(d, k);
-#pragma unroll
-                                for (int j = 0; j < 4; ++j) {
-                                    unsigned out = 0;
-#pragma unroll
-                                    for (int e = 0; e < 2; ++e) {
-                                        const unsigned u = f[j] >> (16 * e) & 0xFFFFu, mag = u & 0x7FFFu;
-                                        const bool     hit = kind == 1 ? mag > A::kExp : mag == A::kExp && (u >> 15) == (unsigned) (kind - 2);
-                                        const unsigned one = __builtin_bit_cast(uint16_t, (T) 1.f);
-                                        out |= (kind == 0 ? (mag >= A::kExp ? 0u : u) : (hit ? one : 0u)) << (16 * e);
-                                    }
-                                    f[j] = out;
-                                }
-                                x = A::mfma(__builtin_bit_cast(typename A::V8, f), wf[k], x);
-                            }
-                            const float special = kind == 1 ? __builtin_nanf("") : (kind == 2 ? __builtin_inff() : -__builtin_inff());
-#pragma unroll
-                            for (int dd = 0; dd < DB; ++dd)
-                                if (dd == d)
-#pragma unroll
-                                    for (int r = 0; r < 16; ++r) acc[dd][r] = kind == 0 ? x[r] : (x[r] > 0.f ? acc[dd][r] + special : acc[dd][r]);
-                        }
-                    }
-                    continue;
-                }
-            }
+            // A weight of zero does not keep a NaN or an infinity of V out of a product. Where something is masked they
+            // are left out of it, and what the queries do see of them is added key by key.
+            unsigned odd = 0;
 #pragma unroll
             for (int k = 0; k < 4; ++k)
 #pragma unroll
-                for (int d = 0; d < DB; ++d) acc[d] = A::mfma(__builtin_bit_cast(typename A::V8, v_frag(d, k)), pf[k], acc[d]);
+                for (int d = 0; d < DB; ++d) {
+                    tk_u32x4 f = v_frag(d, k);
+                    if constexpr (MASKED)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) { // a carry into the sign bit marks an exponent of all ones
+                            const unsigned hit = ((f[j] & (A::kExp * 0x10001u)) + (0x8000u - A::kExp) * 0x10001u) & 0x80008000u;
+                            odd |= hit;
+                            f[j] &= ~((hit >> 15) * 0xFFFFu);
+                        }
+                    acc[d] = A::mfma(__builtin_bit_cast(V8, f), pf[k], acc[d]);
+                }
+            if constexpr (MASKED)
+                if (__any(odd != 0)) {
+                    __attribute__((address_space(3))) T *w = (__attribute__((address_space(3))) T *) (lds + 4 * TILE + wave * (kAttnK * 64));
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) w[(16 * k + 8 * (j >> 2) + 4 * h + (j & 3)) * 32 + col] = pf[k][j];
+                    __builtin_amdgcn_s_waitcnt(0xC07F); // lgkmcnt(0): the wave's own weights
+#pragma unroll 1
+                    for (int key = 0; key < kAttnK; ++key) {
+                        const float p = (float) w[key * 32 + col];
+                        LdsPtr      v = lds + BUF + TILE + key * ROW + 8 * h;
+#pragma unroll
+                        for (int d = 0; d < DB; ++d)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) {
+                                const auto x = *(__attribute__((address_space(3))) const typename A::V4 *) (v + (((4 * d + r) ^ v_swizzle<DP>(key)) << 4));
+#pragma unroll
+                                for (int j = 0; j < 4; ++j) {
+                                    const float y = (float) x[j];
+                                    if (key0 + key < limit && !(fabsf(y) < __builtin_inff())) acc[d][4 * r + j] += p * y;
+                                }
+                            }
+                    }
+                }
+        };
+
+        using std::false_type;
+        using std::true_type;
+        if (tiles > 0) issue(0);
+        for (int t = 0; t < tiles; ++t) {
+            __builtin_amdgcn_s_waitcnt(7 << 4);         // vmcnt(0), lgkmcnt(0): its pieces of tile t have landed, its reads of t - 1 too
+            __asm__ volatile("s_barrier" ::: "memory"); // everybody's have, and nobody reads tile t - 1 any more
+            if (t + 1 < tiles) issue(t + 1);
+            if (t < plain) {
+                if (t & 1) tile(t, std::integral_constant<int, 1>(), false_type());
+                else tile(t, std::integral_constant<int, 0>(), false_type());
+            } else if (t < used) {
+                if (t & 1) tile(t, std::integral_constant<int, 1>(), true_type());
+                else tile(t, std::integral_constant<int, 0>(), true_type());
+            }
         }
 
         l += __shfl_xor(l, 32);
@@ -286,6 +296,7 @@ namespace vkhip {
                 for (int j = 0; j < 4; ++j) x[j] = (T) (acc[d][4 * r + j] * inv);
                 *reinterpret_cast<typename A::V4 *>(dst + at) = x;
             }
+#endif
     }
 
     static const char *attn_refusal(const vkhip_attention_desc *d) {
@@ -297,7 +308,7 @@ namespace vkhip {
         const int64_t st[8] = {d->q_row, d->q_head, d->k_row, d->k_head, d->v_row, d->v_head, d->o_row, d->o_head};
         for (int64_t v: st)
             if (v < 0 || v % 8) return "strides are not multiples of 8";
-        if (d->k_row > (1 << 23) || d->v_row > (1 << 23)) return "k_row or v_row over 2^23";
+        if (d->k_row < d->head_dim || d->v_row < d->head_dim || d->k_row > (1 << 23) || d->v_row > (1 << 23)) return "k_row or v_row under head_dim or over 2^23";
         if ((ceil_div(d->total_q, kAttnQ) + d->batch) * (int64_t) d->q_heads > 0x7FFFFFFF) return "too many queries and heads";
         return nullptr;
     }
