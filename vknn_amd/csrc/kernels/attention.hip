@@ -80,7 +80,7 @@ namespace vkhip {
         __shared__ __attribute__((aligned(1024))) unsigned char sm[4 * TILE + 4 * kAttnK * 64]; // K, V of even tiles, K, V of odd ones, a wave's weights
         LdsPtr lds = (LdsPtr) sm;
 
-        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, col = lane & 31;
+        const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, col = lane & 31;
         // heads of one key/value head next to each other in the grid: workgroups go to the 8 XCDs in turn
         const int head_kv = blockIdx.x % a.kv_heads, group = a.q_heads / a.kv_heads;
         const int head_q = head_kv * group + blockIdx.x / a.kv_heads % group;
@@ -96,15 +96,16 @@ namespace vkhip {
         const int shift = nk - nq;
         const int D     = a.head_dim;
 
+        // keys below `limit` are seen; queries past the last one compute something that is not stored
         const int qi    = i0 + wave * 32 + col;
-        const int limit = qi < nq ? (a.causal ? qi + shift + 1 : nk) : 0; // keys below it are seen
+        const int limit = a.causal ? min(nk, qi + shift + 1) : nk;
         const int k_end = max(0, a.causal ? min(nk, min(i0 + kAttnQ, nq) + shift) : nk);
         const int tiles = (k_end + kAttnK - 1) / kAttnK;
-        // the wave's own tiles: `plain` of them seen whole by all its queries, none of use from `used` on
-        const int w_first = __builtin_amdgcn_readfirstlane(i0 + wave * 32), w_last = min(w_first + 32, nq) - 1;
-        const int low = w_first + 31 < nq ? (a.causal ? w_first + shift + 1 : nk) : 0;
-        const int high = w_first < nq ? (a.causal ? min(nk, w_last + shift + 1) : nk) : 0;
-        const int plain = max(0, low) / kAttnK, used = (max(0, high) + kAttnK - 1) / kAttnK;
+        // the first tiles, an even number, are seen whole by every query of the workgroup
+        const int plain = max(0, a.causal ? min(nk, i0 + shift + 1) : nk) / kAttnK & ~1;
+        // and this wave has no use for tiles from `used` on
+        const int w_first = i0 + wave * 32;
+        const int used    = w_first < nq ? (max(0, a.causal ? min(nk, min(w_first + 32, nq) + shift) : nk) + kAttnK - 1) / kAttnK : 0;
 
         V8 qf[KS];
         {
@@ -131,13 +132,12 @@ namespace vkhip {
             off_v[r]     = cv * 8 < D ? (unsigned) (row * v_bytes + cv * 16) : 0x80000000u;
         }
         // past the sequence's last row, where the resource ends, and past the head's channels the copy writes zeros
-        auto issue = [&](int t) __attribute__((always_inline)) {
+        auto issue = [&](int t, auto odd_c) __attribute__((always_inline)) {
             const int rows = min(kAttnK, nk - t * kAttnK) - 1;
-            const __amdgpu_buffer_rsrc_t kr =
-                __builtin_amdgcn_make_buffer_rsrc((void *) (kb + (int64_t) t * kAttnK * k_bytes), (short) 0, rows * k_bytes + D * 2, 0x00020000);
-            const __amdgpu_buffer_rsrc_t vr =
-                __builtin_amdgcn_make_buffer_rsrc((void *) (vb + (int64_t) t * kAttnK * v_bytes), (short) 0, rows * v_bytes + D * 2, 0x00020000);
-            LdsPtr dst = lds + (t & 1) * (2 * TILE) + wave * (LOADS * 1024);
+            const __amdgpu_buffer_rsrc_t kr = __builtin_amdgcn_make_buffer_rsrc((void *) kb, (short) 0, rows * k_bytes + D * 2, 0x00020000);
+            const __amdgpu_buffer_rsrc_t vr = __builtin_amdgcn_make_buffer_rsrc((void *) vb, (short) 0, rows * v_bytes + D * 2, 0x00020000);
+            kb += (int64_t) kAttnK * k_bytes, vb += (int64_t) kAttnK * v_bytes;
+            LdsPtr dst = lds + odd_c * (2 * TILE) + wave * (LOADS * 1024);
 #pragma unroll
             for (int r = 0; r < LOADS; ++r) __builtin_amdgcn_raw_ptr_buffer_load_lds(kr, dst + r * 1024, 16, off_k[r], 0, 0, 0);
 #pragma unroll
@@ -167,7 +167,7 @@ namespace vkhip {
         float m = -__builtin_inff(), l = 0.f;
 
         auto tile = [&](int t, auto odd_c, auto masked_c) __attribute__((always_inline)) {
-            constexpr int  BUF    = decltype(odd_c)::value * 2 * TILE;
+            const int      BUF    = odd_c * (2 * TILE);
             constexpr bool MASKED = decltype(masked_c)::value;
             const int      key0   = t * kAttnK;
             const auto     seen   = [&](int k, int j) { return key0 + 16 * k + 8 * (j >> 2) + 4 * h + (j & 3) < limit; };
@@ -265,20 +265,27 @@ namespace vkhip {
                 }
         };
 
-        using std::false_type;
-        using std::true_type;
-        if (tiles > 0) issue(0);
-        for (int t = 0; t < tiles; ++t) {
-            __builtin_amdgcn_s_waitcnt(7 << 4);         // vmcnt(0), lgkmcnt(0): its pieces of tile t have landed, its reads of t - 1 too
-            __asm__ volatile("s_barrier" ::: "memory"); // everybody's have, and nobody reads tile t - 1 any more
-            if (t + 1 < tiles) issue(t + 1);
-            if (t < plain) {
-                if (t & 1) tile(t, std::integral_constant<int, 1>(), false_type());
-                else tile(t, std::integral_constant<int, 0>(), false_type());
-            } else if (t < used) {
-                if (t & 1) tile(t, std::integral_constant<int, 1>(), true_type());
-                else tile(t, std::integral_constant<int, 0>(), true_type());
-            }
+        // tile t has landed (every wave's pieces), and nobody reads tile t - 1 any more
+        const auto landed = [] __attribute__((always_inline)) {
+            __builtin_amdgcn_s_waitcnt(7 << 4); // vmcnt(0), lgkmcnt(0)
+            __asm__ volatile("s_barrier" ::: "memory");
+        };
+        const std::integral_constant<int, 0> even;
+        const std::integral_constant<int, 1> odd;
+        if (tiles > 0) issue(0, even);
+        int t = 0;
+        for (; t < plain; t += 2) {
+            landed();
+            issue(t + 1, odd);
+            if (used) tile(t, even, std::false_type());
+            landed();
+            if (t + 2 < tiles) issue(t + 2, even);
+            if (used) tile(t + 1, odd, std::false_type());
+        }
+        for (; t < tiles; ++t) {
+            landed();
+            if (t + 1 < tiles) issue(t + 1, t + 1 & 1);
+            if (t < used) tile(t, t & 1, std::true_type());
         }
 
         l += __shfl_xor(l, 32);
