@@ -600,3 +600,24 @@ def test_own_stream_and_graph_replay(gpu):
             assert torch.isfinite(a[:4]).all() and torch.equal(a.nan_to_num(5.5), b.nan_to_num(5.5))
     check(lib.vkhip_graph_destroy(g))
     check(lib.vkhip_stream_destroy(s))
+
+
+@pytest.mark.parametrize("nq,nk,hq,hkv,d", [([200], [4200], 2, 1, 128), ([130, 3], [130, 5000], 2, 2, 64), ([1], [3001], 4, 4, 72), ([500], [3], 1, 1, 64), ([300, 0, 20], [2500, 7, 2048], 1, 1, 128)])
+@pytest.mark.parametrize("causal", [False, True])
+def test_attention_few_queries_many_keys(gpu, nq, nk, hq, hkv, d, causal):
+    """Calls whose keys are split over workgroups (few queries and heads, 1024 keys or more each)."""
+    d0 = V.AttentionDesc(batch=len(nq), q_heads=hq, kv_heads=hkv, head_dim=d, total_q=sum(nq), total_k=sum(nk), dtype=0, causal=int(causal), scale=0.1, q_row=hq * d, q_head=d,
+                         k_row=hkv * d, k_head=d, v_row=hkv * d, v_head=d, o_row=hq * d, o_head=d)
+    assert (V.vkhip().vkhip_attention_workspace_bytes(ctypes.byref(d0)) > 0) == (sum(nk) // len(nk) >= 2048)
+    for dtype in ("f16", "bf16"):
+        q, k, v = attention_inputs(sum(nq), nq, nk, hq, hkv, d, dtype)
+        check_attention(attention(V.vkhip(), q, k, v, nq, nk, causal, dtype, d ** -0.5), q, k, v, nq, nk, causal, dtype, d ** -0.5)
+
+
+def test_attention_many_sequences(gpu):
+    """More sequences than a wave has lanes, lengths mixed with empty ones; and equal lengths."""
+    r = np.random.default_rng(5)
+    for lens in ([int(x) for x in r.integers(0, 300, 150)], [130] * 7, [1] * 200):
+        q, k, v = attention_inputs(len(lens), lens, lens, 2, 1, 64, "f16")
+        for causal in (True, False):
+            check_attention(attention(V.vkhip(), q, k, v, lens, lens, causal, "f16", 0.125, joint=True), q, k, v, lens, lens, causal, "f16", 0.125)

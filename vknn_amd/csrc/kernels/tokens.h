@@ -15,6 +15,21 @@ namespace vkhip {
     // Below -126 it gives 0 for what would be subnormal: weights under 2^-126 of the largest one.
     __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 
+    // Sums over the lanes up to each, and over all 64 (row shifts within 16 lanes, then the rows' last lanes).
+    template <int CTRL, int ROWS>
+    __device__ __forceinline__ int dpp_add_int(int x) {
+        return x + __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xF, false);
+    }
+    __device__ __forceinline__ int wave_prefix_sum(int x) {
+        x = dpp_add_int<0x111, 0xF>(x); // row_shr 1, 2, 4, 8
+        x = dpp_add_int<0x112, 0xF>(x);
+        x = dpp_add_int<0x114, 0xF>(x);
+        x = dpp_add_int<0x118, 0xF>(x);
+        x = dpp_add_int<0x142, 0xA>(x); // row_bcast 15 into rows 1 and 3
+        return dpp_add_int<0x143, 0xC>(x); // row_bcast 31 into rows 2 and 3
+    }
+    __device__ __forceinline__ int wave_total(int x) { return __builtin_amdgcn_readlane(wave_prefix_sum(x), 63); }
+
     struct SeqTile {
         int b, tile; // b = -1: past the last one
     };
@@ -24,13 +39,7 @@ namespace vkhip {
     __device__ __forceinline__ SeqTile find_tile(int item, int batch, Count count) {
         const int lane = threadIdx.x & 63;
         for (int b0 = 0; b0 < batch; b0 += 64) {
-            const int b = b0 + lane, n = b < batch ? count(b) : 0;
-            int       incl = n;
-#pragma unroll
-            for (int o = 1; o < 64; o <<= 1) {
-                const int t = __shfl_up(incl, o);
-                if (lane >= o) incl += t;
-            }
+            const int      b = b0 + lane, n = b < batch ? max(0, count(b)) : 0, incl = wave_prefix_sum(n);
             const uint64_t hit = __ballot(item < incl);
             if (hit) {
                 const int first = __ffsll((unsigned long long) hit) - 1;
@@ -39,6 +48,30 @@ namespace vkhip {
             item -= __builtin_amdgcn_readlane(incl, 63);
         }
         return {-1, 0};
+    }
+    // The same for up to 64 sequences with their last tiles first: all sequences' tiles are numbered by falling tile
+    // index, sequences of the same index in order. C(t) = sum max(0, count - t) items have an index of t or more.
+    // Sequences of equal counts go one after the other, so that neighbouring items share a sequence.
+    template <typename Count>
+    __device__ __forceinline__ SeqTile find_tile_falling(int item, int batch, Count count) {
+        const int lane = threadIdx.x & 63, n = lane < batch ? max(0, count(lane)) : 0;
+        if (item >= wave_total(n)) return {-1, 0};
+        const int n0 = __builtin_amdgcn_readfirstlane(n);
+        if (!__any(lane < batch && n != n0)) return {item / n0, n0 - 1 - item % n0};
+        int lo = 0, hi = n; // item < C(lo), item >= C(hi)
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) hi = max(hi, __shfl_xor(hi, o));
+        hi = __builtin_amdgcn_readfirstlane(hi);
+        while (hi - lo > 1) {
+            const int t = (lo + hi) / 2;
+            if (item < wave_total(max(0, n - t))) lo = t;
+            else hi = t;
+        }
+        const uint64_t there = __ballot(n > lo);
+        const int      rank = item - wave_total(max(0, n - hi)); // among the sequences that have this index
+        const int      before = __builtin_amdgcn_mbcnt_hi((unsigned) (there >> 32), __builtin_amdgcn_mbcnt_lo((unsigned) there, 0));
+        const uint64_t mine = __ballot((there >> lane & 1) && before == rank);
+        return {__ffsll((unsigned long long) mine) - 1, lo};
     }
 
     __device__ __forceinline__ int clampi(int v, int lo, int hi) { return v < lo ? lo : (v > hi ? hi : v); }
