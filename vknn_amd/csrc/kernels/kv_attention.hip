@@ -10,6 +10,10 @@
 // page, so weights are rounded to fp16 unscaled (at most 1, the largest of a row exactly 1).
 // The tokens of a sequence are split over workgroups and a workgroup's four waves; partial results
 // (maximum, sum, product) join in LDS and, across workgroups, in a second kernel.
+//
+// Measured, fp16, 32 heads on 8, D = 128: 8 x 131072 tokens 368 us (5.8 TB/s), 64 x 2048 48 us (5.6), 64 ragged
+// sequences up to 4000 61 us (4.4, the join 5 of it), 8 x 300 6.9 us. Loading the next step's keys and values while this
+// one's are multiplied gained nothing: it costs the registers of a third wave a SIMD, which does the same.
 #include "kv_cache.h"
 
 namespace vkhip {
@@ -19,11 +23,12 @@ namespace vkhip {
         const void    *q;
         void          *o;
         const int32_t *lens;
-        float         *part; // [batch][head][row][split]: row values, then (maximum, sum)
+        float         *part_o, *part_s; // [batch][head][row][split]: products [head_dim]; (maximum, sum)
         float          scale;
         int            group, rows, q_tokens; // query heads per kv head; rows = group * q_tokens
         int            blocks;                // blocks of 16 * RT rows
         int            max_len, span, splits; // tokens per workgroup
+        int            waves;                 // of a workgroup
         int64_t        q_row, q_head, o_row, o_head;
     };
 
@@ -43,14 +48,16 @@ namespace vkhip {
 
     constexpr int kStep = 64; // tokens a wave takes at a time
 
-    // DJ = row / 64 channels, RT tiles of 16 rows, P32: pages of 32 tokens (two to a step).
-    template <typename T, int DJ, int RT, bool P32>
-    __global__ __launch_bounds__(256) void kv_attention_kernel(KvAttnArgs a) {
-        constexpr int Dp = DJ * 64, DT = DJ * 4;
-        __shared__ float wave_m[4][RT * 16], wave_l[4][RT * 16];
-        __shared__ float acc_lds[4][16][Dp + 4];
-        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, nn = lane & 15;
-        const int split = blockIdx.x, head = blockIdx.y / a.blocks, row0 = blockIdx.y % a.blocks * (16 * RT), b = blockIdx.z;
+    // DJ = row / 64 channels, RT tiles of 16 rows, P32: pages of 32 tokens (two to a step), NW waves.
+    template <typename T, int DJ, int RT, bool P32, int NW>
+    __global__ __launch_bounds__(NW * 64) void kv_attention_kernel(KvAttnArgs a) {
+        constexpr int Dp = DJ * 64, DT = DJ * 4, NL = NW < 4 ? NW : 4; // NL: waves whose products lie in LDS at a time
+        __shared__ float wave_m[NW][RT * 16], wave_l[NW][RT * 16];
+        __shared__ float acc_lds[NL][16][Dp + 4];
+        const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, nn = lane & 15;
+        // heads, then sequences, then splits: workgroups go to the 8 XCDs in turn, and with splits first the later ones,
+        // which short sequences do not have, would all meet on some of them
+        const int head = blockIdx.x / a.blocks, row0 = blockIdx.x % a.blocks * (16 * RT), b = blockIdx.y, split = blockIdx.z;
         const int P   = a.c.page_tokens, D = a.c.head_dim;
         const int len = clampi(a.lens[b], 0, min(a.max_len, a.c.max_blocks * P));
         const int t0 = split * a.span, t1 = min(len, t0 + a.span);
@@ -114,14 +121,14 @@ namespace vkhip {
 
         const int32_t *table = a.c.table + (int64_t) b * a.c.max_blocks;
         const int64_t  page_bytes = (int64_t) P * Dp;
-        for (int tok = t0 + wave * kStep; tok < t1; tok += 4 * kStep) {
+        for (int tok = t0 + wave * kStep; tok < t1; tok += NW * kStep) {
             // the step's page, or its two; a block without memory is a page that no query sees
             const unsigned char *kp[2], *vp[2];
             float                ks[2], vs[2];
             bool                 has[2];
 #pragma unroll
             for (int u = 0; u < (P32 ? 2 : 1); ++u) {
-                const int at = tok + 32 * u, id = at < t1 ? __builtin_amdgcn_readfirstlane(table[at / P]) : -1;
+                const int at = tok + 32 * u, id = at < t1 ? table[at / P] : -1;
                 has[u]       = id >= 0 && id < a.c.pages;
                 const int64_t hp = (int64_t) (has[u] ? id : 0) * a.c.heads + head;
                 kp[u] = a.c.k + hp * page_bytes + (int64_t) (at % P) * Dp;
@@ -219,7 +226,7 @@ namespace vkhip {
             }
         }
 
-        // join the four waves, a tile of rows at a time
+        // join the waves, a tile of rows at a time
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
             l[rt] += __shfl_xor(l[rt], 16);
@@ -227,69 +234,114 @@ namespace vkhip {
             if (g == 0) wave_m[wave][rt * 16 + nn] = m[rt], wave_l[wave][rt * 16 + nn] = l[rt];
         }
         __syncthreads();
+        const auto row_max = [&](int r) {
+            float top = wave_m[0][r];
+#pragma unroll
+            for (int w = 1; w < NW; ++w) top = fmaxf(top, wave_m[w][r]);
+            return top;
+        };
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
-            const int   r   = rt * 16 + nn;
-            const float top = fmaxf(fmaxf(wave_m[0][r], wave_m[1][r]), fmaxf(wave_m[2][r], wave_m[3][r]));
-            const float f   = exp2_hw(m[rt] - (top == -__builtin_inff() ? 0.f : top));
+            const float top = row_max(rt * 16 + nn), f = exp2_hw(m[rt] - (top == -__builtin_inff() ? 0.f : top));
 #pragma unroll
-            for (int d = 0; d < DT; ++d) {
-                float4v x = acc[rt][d];
+            for (int d = 0; d < DT; ++d)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) x[i] *= f;
-                *reinterpret_cast<float4v *>(&acc_lds[wave][nn][16 * d + 4 * g]) = x;
+                for (int i = 0; i < 4; ++i) acc[rt][d][i] *= f;
+            if constexpr (NW > NL) { // the upper waves' products into the lower ones' registers
+                if (wave >= NL)
+#pragma unroll
+                    for (int d = 0; d < DT; ++d) *reinterpret_cast<float4v *>(&acc_lds[wave - NL][nn][16 * d + 4 * g]) = acc[rt][d];
+                __syncthreads();
+                if (wave < NL)
+#pragma unroll
+                    for (int d = 0; d < DT; ++d) acc[rt][d] += *reinterpret_cast<const float4v *>(&acc_lds[wave][nn][16 * d + 4 * g]);
+                __syncthreads();
             }
-            __syncthreads();
-            for (int i = threadIdx.x; i < 16 * Dp; i += 256) {
-                const int   n = i / Dp, d = i % Dp, row = row0 + rt * 16 + n, q = rt * 16 + n;
-                const float tm  = fmaxf(fmaxf(wave_m[0][q], wave_m[1][q]), fmaxf(wave_m[2][q], wave_m[3][q]));
-                const float tb  = tm == -__builtin_inff() ? 0.f : tm;
-                float       sum = 0.f, x = 0.f;
+            if (wave < NL)
 #pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                    sum += wave_l[w][q] * exp2_hw(wave_m[w][q] - tb);
-                    x += acc_lds[w][n][d];
+                for (int d = 0; d < DT; ++d) *reinterpret_cast<float4v *>(&acc_lds[wave][nn][16 * d + 4 * g]) = acc[rt][d];
+            __syncthreads();
+            // VPT neighbouring channels of one row a thread
+            constexpr int VPT = Dp / (4 * NW);
+            const int     n = threadIdx.x / (4 * NW), d0 = threadIdx.x % (4 * NW) * VPT, row = row0 + rt * 16 + n, q = rt * 16 + n;
+            if (row < a.rows && d0 < D) {
+                const float tm = row_max(q), tb = tm == -__builtin_inff() ? 0.f : tm;
+                float       sum = 0.f, x[VPT];
+#pragma unroll
+                for (int w = 0; w < NW; ++w) sum += wave_l[w][q] * exp2_hw(wave_m[w][q] - tb);
+#pragma unroll
+                for (int i = 0; i < VPT; ++i) {
+                    x[i] = 0.f;
+#pragma unroll
+                    for (int w = 0; w < NL; ++w) x[i] += acc_lds[w][n][d0 + i];
                 }
-                if (row >= a.rows || d >= D) continue;
                 if (a.splits == 1) {
-                    const int t = row / a.group, h = head * a.group + row % a.group;
-                    ((T *) a.o)[((int64_t) b * a.q_tokens + t) * a.o_row + h * a.o_head + d] = (T) (sum == 0.f ? 0.f : x / sum);
+                    const int   t = row / a.group, h = head * a.group + row % a.group;
+                    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+                    T          *o = (T *) a.o + ((int64_t) b * a.q_tokens + t) * a.o_row + h * a.o_head + d0;
+#pragma unroll
+                    for (int i = 0; i < VPT; ++i)
+                        if (d0 + i < D) o[i] = (T) (x[i] * inv);
                 } else {
-                    float *p = a.part + (((int64_t) b * a.c.heads + head) * a.rows + row) * a.splits * (D + 2) + (int64_t) split * (D + 2);
-                    p[d]     = x;
-                    if (d == 0) p[D] = tm, p[D + 1] = sum;
+                    const int64_t at = (((int64_t) b * a.c.heads + head) * a.rows + row) * a.splits + split;
+#pragma unroll
+                    for (int i = 0; i < VPT; ++i)
+                        if (d0 + i < D) a.part_o[at * D + d0 + i] = x[i];
+                    if (d0 == 0) *reinterpret_cast<float2 *>(a.part_s + at * 2) = make_float2(tm, sum);
                 }
             }
-            __syncthreads();
+            if (rt + 1 < RT) __syncthreads();
         }
     }
 
-    // Joins the splits of one row: one wave, two channels a lane.
-    template <typename T>
-    __global__ __launch_bounds__(64) void kv_join_kernel(KvAttnArgs a) {
-        const int row = blockIdx.x, head = blockIdx.y, b = blockIdx.z, D = a.c.head_dim, lane = threadIdx.x;
+    // Joins the splits of a row: WPR waves each, two channels a lane; the splits' weights are formed a lane each, so
+    // that the products' loads wait for nothing.
+    template <typename T, int WPR>
+    __global__ __launch_bounds__(256) void kv_join_kernel(KvAttnArgs a) {
+        __shared__ float2 half[4][64];
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, D = a.c.head_dim, d = lane * 2;
+        const int row = blockIdx.x * (4 / WPR) + wave / WPR, head = blockIdx.y, b = blockIdx.z, part = wave % WPR;
         const int len = clampi(a.lens[b], 0, min(a.max_len, a.c.max_blocks * a.c.page_tokens));
-        const int n   = max(1, (len + a.span - 1) / a.span);
-        const float *p = a.part + (((int64_t) b * a.c.heads + head) * a.rows + row) * a.splits * (D + 2);
-        float top = -__builtin_inff();
-        for (int k = lane; k < n; k += 64) top = fmaxf(top, p[(int64_t) k * (D + 2) + D]);
+        const int n   = row < a.rows ? max(1, (len + a.span - 1) / a.span) : 0;
+        const int64_t at = (((int64_t) b * a.c.heads + head) * a.rows + row) * a.splits;
+        float top = -__builtin_inff(), sum = 0.f;
+        for (int k = lane; k < n; k += 64) top = fmaxf(top, a.part_s[(at + k) * 2]);
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) top = fmaxf(top, __shfl_xor(top, o));
         const float base = top == -__builtin_inff() ? 0.f : top;
-        float       sum = 0.f, x0 = 0.f, x1 = 0.f;
-        for (int k = 0; k < n; ++k) {
-            const float *e = p + (int64_t) k * (D + 2);
-            const float  f = exp2_hw(e[D] - base);
-            sum += e[D + 1] * f;
-            if (lane < D) x0 += e[lane] * f;
-            if (lane + 64 < D) x1 += e[lane + 64] * f;
+        float2      x = make_float2(0.f, 0.f);
+        for (int k0 = 0; k0 < n; k0 += 64) {
+            const int    k = k0 + lane;
+            const float2 s = k < n ? *reinterpret_cast<const float2 *>(a.part_s + (at + k) * 2) : make_float2(-__builtin_inff(), 0.f);
+            const float  f = exp2_hw(s.x - base);
+            sum += s.y * f;
+            const int end = min(64, n - k0);
+#pragma unroll 8
+            for (int i = part; i < end; i += WPR) {
+                const float w = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), i));
+                const float2 y = *reinterpret_cast<const float2 *>(a.part_o + (at + k0 + i) * D + min(d, D - 2));
+                x.x += y.x * w, x.y += y.y * w;
+            }
         }
-        T *o = (T *) a.o + ((int64_t) b * a.q_tokens + row / a.group) * a.o_row + (head * a.group + row % a.group) * a.o_head;
-        if (lane < D) o[lane] = (T) (sum == 0.f ? 0.f : x0 / sum);
-        if (lane + 64 < D) o[lane + 64] = (T) (sum == 0.f ? 0.f : x1 / sum);
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) sum += __shfl_xor(sum, o);
+        if constexpr (WPR > 1) {
+            half[wave][lane] = x;
+            __syncthreads();
+            if (part) return;
+#pragma unroll
+            for (int w = 1; w < WPR; ++w) x.x += half[wave + w][lane].x, x.y += half[wave + w][lane].y;
+        }
+        if (row >= a.rows || d >= D) return;
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        T          *o = (T *) a.o + ((int64_t) b * a.q_tokens + row / a.group) * a.o_row + (head * a.group + row % a.group) * a.o_head + d;
+        o[0] = (T) (x.x * inv), o[1] = (T) (x.y * inv);
     }
 
-    static int row_tiles(int rows) { return rows <= 16 ? 1 : (rows <= 32 ? 2 : 4); }
+    // Tiles of 16 rows a wave multiplies with what it has read. Four would read the cache once for 64 rows, but leave
+    // registers for one wave a SIMD and nothing to read while it computes: 16 x 5000 tokens, 64 rows, 63 us with four,
+    // 46 with two, 56 with one.
+    static int row_tiles(int rows) { return rows <= 16 ? 1 : 2; }
 
     static const char *kv_attention_refusal(const vkhip_kv_attention_desc *d, const vkhip_kv_cache *c) {
         if (const char *why = kv_refusal(c)) return why;
@@ -302,7 +354,7 @@ namespace vkhip {
         return nullptr;
     }
 
-    // How the call is cut: rows into blocks of up to 64, tokens into spans of whole rounds of the four waves.
+    // How the call is cut: rows into blocks of up to 32, tokens into spans of whole rounds of a workgroup's waves.
     static KvAttnArgs kv_attention_cut(const vkhip_kv_attention_desc *d, const vkhip_kv_cache *c) {
         KvAttnArgs a {};
         a.c        = kv_args(c);
@@ -312,35 +364,51 @@ namespace vkhip {
         a.blocks   = (int) ceil_div(a.rows, 16 * row_tiles(a.rows));
         const int64_t most = (int64_t) c->max_blocks * c->page_tokens;
         a.max_len  = (int) (d->max_len > 0 && d->max_len < most ? d->max_len : most);
-        const int64_t base = (int64_t) c->batch * c->kv_heads * a.blocks, rounds = ceil_div(a.max_len > 0 ? a.max_len : 1, 4 * kStep);
-        int64_t       splits = base > 0 ? ceil_div(1024, base) : 1;
+        const int64_t len = a.max_len > 0 ? a.max_len : 1, base = (int64_t) c->batch * c->kv_heads * a.blocks;
+        // Waves of a workgroup: two where no sequence has more steps, eight and no split where one workgroup takes a short
+        // sequence in one round and there are few of them (a second launch costs about 3 us), four otherwise.
+        const bool few = base <= 256 && len <= 8 * kStep && row_tiles(a.rows) == 1;
+        a.waves        = len <= 2 * kStep ? 2 : (few ? 8 : 4);
+        // Splits: two workgroups a compute unit, which all run at once; where that leaves more than 8 rounds to one,
+        // which would wait for the longest sequence, spans of 8 rounds or 2048 workgroups. In between, workgroups that
+        // nearly all run at once leave some for a second turn (8 x 131072 tokens: 362 us with 512, 404 with 1024, 370
+        // with 2048; 64 ragged sequences up to 4000: 71 us unsplit, 61 in two).
+        const int64_t rounds = ceil_div(len, a.waves * kStep);
+        int64_t       splits = few || base >= 512 || base == 0 ? 1 : 512 / base;
+        if (base > 0 && rounds > 8 * splits) {
+            const int64_t more = rounds / 8 < 2048 / base ? rounds / 8 : 2048 / base;
+            if (more > splits) splits = more;
+        }
         if (splits > rounds) splits = rounds;
-        a.span   = (int) (ceil_div(rounds, splits) * 4 * kStep);
-        a.splits = (int) ceil_div(a.max_len > 0 ? a.max_len : 1, a.span);
+        a.span   = (int) (ceil_div(rounds, splits) * a.waves * kStep);
+        a.splits = (int) ceil_div(len, a.span);
         return a;
     }
 
-    template <typename T, int DJ, int RT>
+    template <typename T, int DJ, int RT, bool P32>
     static void kv_attention_launch(const KvAttnArgs &a, hipStream_t s) {
-        const dim3 grid((unsigned) a.splits, (unsigned) (a.c.heads * a.blocks), (unsigned) a.c.batch);
-        if (a.c.page_tokens == 32) kv_attention_kernel<T, DJ, RT, true><<<grid, 256, 0, s>>>(a);
-        else kv_attention_kernel<T, DJ, RT, false><<<grid, 256, 0, s>>>(a);
+        const dim3 grid((unsigned) (a.c.heads * a.blocks), (unsigned) a.c.batch, (unsigned) a.splits);
+        if (a.waves == 2) kv_attention_kernel<T, DJ, RT, P32, 2><<<grid, 128, 0, s>>>(a);
+        else if (a.waves == 4) kv_attention_kernel<T, DJ, RT, P32, 4><<<grid, 256, 0, s>>>(a);
+        else if constexpr (RT == 1) kv_attention_kernel<T, DJ, RT, P32, 8><<<grid, 512, 0, s>>>(a);
+    }
+    template <typename T, int DJ>
+    static void kv_attention_tiles(const KvAttnArgs &a, hipStream_t s) {
+        const int  rt  = row_tiles(a.rows);
+        const bool p32 = a.c.page_tokens == 32;
+        if (rt == 1) p32 ? kv_attention_launch<T, DJ, 1, true>(a, s) : kv_attention_launch<T, DJ, 1, false>(a, s);
+        else p32 ? kv_attention_launch<T, DJ, 2, true>(a, s) : kv_attention_launch<T, DJ, 2, false>(a, s);
     }
     template <typename T>
     static int kv_attention_run(const KvAttnArgs &a, hipStream_t s) {
-        const int rt = row_tiles(a.rows);
-        if (a.c.row == 64) {
-            if (rt == 1) kv_attention_launch<T, 1, 1>(a, s);
-            else if (rt == 2) kv_attention_launch<T, 1, 2>(a, s);
-            else kv_attention_launch<T, 1, 4>(a, s);
-        } else {
-            if (rt == 1) kv_attention_launch<T, 2, 1>(a, s);
-            else if (rt == 2) kv_attention_launch<T, 2, 2>(a, s);
-            else kv_attention_launch<T, 2, 4>(a, s);
-        }
+        if (a.c.row == 64) kv_attention_tiles<T, 1>(a, s);
+        else kv_attention_tiles<T, 2>(a, s);
         int rc = check_launch("kv_attention");
         if (rc || a.splits == 1) return rc;
-        kv_join_kernel<T><<<dim3((unsigned) a.rows, (unsigned) a.c.heads, (unsigned) a.c.batch), 64, 0, s>>>(a);
+        const bool wide = a.splits > 8; // below, a row's products are few loads of one wave
+        const dim3 grid((unsigned) (wide ? a.rows : ceil_div(a.rows, 4)), (unsigned) a.c.heads, (unsigned) a.c.batch);
+        if (wide) kv_join_kernel<T, 4><<<grid, 256, 0, s>>>(a);
+        else kv_join_kernel<T, 1><<<grid, 256, 0, s>>>(a);
         return check_launch("kv_attention join");
     }
 
@@ -365,7 +433,9 @@ int vkhip_kv_attention(const vkhip_kv_attention_desc *d, const vkhip_kv_cache *c
     if (!q || !lens || !o || (a.splits > 1 && !workspace)) return set_error(VKHIP_ERR_INVALID, "kv_attention: null pointer");
     if (misaligned16(q) || misaligned16(o) || misaligned16(workspace) || ((uintptr_t) lens) % 4) return set_error(VKHIP_ERR_INVALID, "kv_attention: misaligned pointer");
     if ((int64_t) c->kv_heads * a.blocks > 65535) return set_error(VKHIP_ERR_INVALID, "kv_attention: too many heads and query tokens");
-    a.q = q, a.o = o, a.lens = lens, a.part = (float *) workspace, a.scale = d->scale;
+    if (c->pages == 0) a.max_len = 0; // no block has memory: every query gives zeros
+    a.q = q, a.o = o, a.lens = lens, a.part_o = (float *) workspace, a.scale = d->scale;
+    a.part_s = a.part_o + (size_t) c->batch * c->kv_heads * a.rows * a.splits * c->head_dim;
     a.q_row = d->q_row, a.q_head = d->q_head, a.o_row = d->o_row, a.o_head = d->o_head;
     return d->dtype == VKHIP_DT_F16 ? kv_attention_run<half_t>(a, resolve_stream(s)) : kv_attention_run<bf16_t>(a, resolve_stream(s));
 }
