@@ -128,11 +128,11 @@ namespace vkhip {
             bool                 has[2];
 #pragma unroll
             for (int u = 0; u < (P32 ? 2 : 1); ++u) {
-                const int at = tok + 32 * u, id = at < t1 ? table[at / P] : -1;
+                const int at = tok + 32 * u, id = at < t1 ? table[at >> a.c.page_shift] : -1;
                 has[u]       = id >= 0 && id < a.c.pages;
                 const int64_t hp = (int64_t) (has[u] ? id : 0) * a.c.heads + head;
-                kp[u] = a.c.k + hp * page_bytes + (int64_t) (at % P) * Dp;
-                vp[u] = a.c.v + hp * page_bytes + at % P;
+                kp[u] = a.c.k + hp * page_bytes + (int64_t) (at & (P - 1)) * Dp;
+                vp[u] = a.c.v + hp * page_bytes + (at & (P - 1));
                 ks[u] = has[u] ? a.c.k_scale[hp] : 0.f;
                 vs[u] = has[u] ? a.c.v_scale[hp] : 0.f;
             }

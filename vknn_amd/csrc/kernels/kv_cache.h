@@ -8,7 +8,7 @@ namespace vkhip {
         unsigned char *k, *v; // [page][head][token][row], [page][head][row][token]
         float         *k_scale, *v_scale;
         const int32_t *table;
-        int            pages, page_tokens, heads, head_dim, row, batch, max_blocks;
+        int            pages, page_tokens, page_shift, heads, head_dim, row, batch, max_blocks; // page_tokens = 1 << page_shift
     };
 
     const char *kv_refusal(const vkhip_kv_cache *c);

@@ -33,17 +33,39 @@ namespace vkhip {
     struct SeqTile {
         int b, tile; // b = -1: past the last one
     };
-    // Work items are numbered sequence by sequence, count(b) of them for sequence b. Every wave finds its
-    // own by a prefix sum over 64 sequences at a time; the result is the same in every lane.
+    // Work items are numbered sequence by sequence, count(b) of them for sequence b. Every wave finds its own by a
+    // prefix sum over its lanes, a sequence each or, past 64, four neighbouring ones; the result is the same in
+    // every lane.
     template <typename Count>
     __device__ __forceinline__ SeqTile find_tile(int item, int batch, Count count) {
         const int lane = threadIdx.x & 63;
-        for (int b0 = 0; b0 < batch; b0 += 64) {
-            const int      b = b0 + lane, n = b < batch ? max(0, count(b)) : 0, incl = wave_prefix_sum(n);
+        if (batch <= 64) {
+            const int      n = lane < batch ? max(0, count(lane)) : 0, incl = wave_prefix_sum(n);
+            const uint64_t hit = __ballot(item < incl);
+            if (!hit) return {-1, 0};
+            const int first = __ffsll((unsigned long long) hit) - 1;
+            return {first, item - __builtin_amdgcn_readlane(incl - n, first)};
+        }
+        for (int b0 = 0; b0 < batch; b0 += 256) {
+            int n[4], all = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int b = b0 + lane * 4 + i;
+                n[i]        = b < batch ? max(0, count(b)) : 0;
+                all += n[i];
+            }
+            const int      incl = wave_prefix_sum(all);
             const uint64_t hit = __ballot(item < incl);
             if (hit) {
                 const int first = __ffsll((unsigned long long) hit) - 1;
-                return {b0 + first, item - __builtin_amdgcn_readlane(incl - n, first)};
+                item -= __builtin_amdgcn_readlane(incl - all, first);
+                int i = 0;
+#pragma unroll
+                for (int k = 0; k < 3; ++k) {
+                    const int c = __builtin_amdgcn_readlane(n[k], first);
+                    if (i == k && item >= c) item -= c, ++i;
+                }
+                return {b0 + first * 4 + i, item};
             }
             item -= __builtin_amdgcn_readlane(incl, 63);
         }
