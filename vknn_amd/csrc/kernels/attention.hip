@@ -79,7 +79,7 @@ namespace vkhip {
         constexpr int TILE   = kAttnK * ROW;      // bytes of a K or V tile
         constexpr int LOADS  = TILE / 1024 / 4;   // wave loads of 1 KB per wave and tile
         constexpr int KS = DP / 16, DB = DP / 32; // contraction steps of a score, 32-channel blocks of the output
-        __shared__ __attribute__((aligned(1024))) unsigned char sm[4 * TILE + 4 * kAttnK * 64]; // K, V of even tiles, K, V of odd ones, a wave's weights
+        __shared__ __attribute__((aligned(1024))) unsigned char sm[4 * TILE + 4 * kAttnK * 32 + 32]; // K, V of even tiles, of odd ones, the waves' weights and findings
         LdsPtr lds = (LdsPtr) sm;
 
         const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, col = lane & 31;
@@ -166,11 +166,16 @@ namespace vkhip {
         for (int d = 0; d < DB; ++d)
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[d][r] = 0.f;
+        // sign bits of the two values whose exponent is all ones: a carry goes there
+        const auto not_finite = [](unsigned two) { return ((two & (A::kExp * 0x10001u)) + (0x8000u - A::kExp) * 0x10001u) & 0x80008000u; };
         // the reference of the exponents, at most 8 below the largest one seen: weights up to 2^8 cost no digits, and
         // O is rescaled only where a maximum grows by more than that
         float m = -__builtin_inff(), l = 0.f;
 
-        auto tile = [&](int t, auto odd_c, auto masked_c) __attribute__((always_inline)) {
+        // A weight of zero does not keep a NaN or an infinity of V out of a product. Where something is masked, each wave
+        // looks through the piece of V that it copied and clears what it finds (`spoiled`: something was); what the
+        // queries do see of it is then added key by key, read from memory again.
+        auto tile = [&](int t, auto odd_c, auto masked_c, bool spoiled) __attribute__((always_inline)) {
             const int      BUF    = odd_c * (2 * TILE);
             constexpr bool MASKED = decltype(masked_c)::value;
             const int      key0   = t * kAttnK;
@@ -225,40 +230,34 @@ namespace vkhip {
                 const tk_u32x2 x = lds_read_tr(va[d][0] + BUF + k * 16 * ROW), y = lds_read_tr(va[d][1] + BUF + k * 16 * ROW);
                 return tk_u32x4 {x[0], x[1], y[0], y[1]};
             };
-            // A weight of zero does not keep a NaN or an infinity of V out of a product. Where something is masked they
-            // are left out of it, and what the queries do see of them is added key by key.
-            unsigned odd = 0;
 #pragma unroll
             for (int k = 0; k < 4; ++k)
 #pragma unroll
                 for (int d = 0; d < DB; ++d) {
-                    tk_u32x4 f = v_frag(d, k);
-                    if constexpr (MASKED)
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) { // a carry into the sign bit marks an exponent of all ones
-                            const unsigned hit = ((f[j] & (A::kExp * 0x10001u)) + (0x8000u - A::kExp) * 0x10001u) & 0x80008000u;
-                            odd |= hit;
-                            f[j] &= ~((hit >> 15) * 0xFFFFu);
-                        }
-                    acc[d] = A::mfma(__builtin_bit_cast(V8, f), pf[k], acc[d]);
+                    acc[d] = A::mfma(__builtin_bit_cast(V8, v_frag(d, k)), pf[k], acc[d]);
                 }
-            if constexpr (MASKED)
-                if (__any(odd != 0)) {
-                    __attribute__((address_space(3))) T *w = (__attribute__((address_space(3))) T *) (lds + 4 * TILE + wave * (kAttnK * 64));
+            if (MASKED && spoiled) {
+                __attribute__((address_space(3))) T *w = (__attribute__((address_space(3))) T *) (lds + 4 * TILE + wave * (kAttnK * 32));
+                const T *rows = (const T *) a.v + (int64_t) (k0 + key0) * a.v_row + (int64_t) head_kv * a.v_head;
+#pragma unroll 1
+                for (int half = 0; half < 2; ++half) { // 32 keys at a time, their weights in LDS
 #pragma unroll
-                    for (int k = 0; k < 4; ++k)
+                    for (int k = 0; k < 2; ++k) {
+                        const V8 p = half ? pf[2 + k] : pf[k];
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) w[(16 * k + 8 * (j >> 2) + 4 * h + (j & 3)) * 32 + col] = pf[k][j];
+                        for (int j = 0; j < 8; ++j) w[(16 * k + 8 * (j >> 2) + 4 * h + (j & 3)) * 32 + col] = p[j];
+                    }
                     __builtin_amdgcn_s_waitcnt(0xC07F); // lgkmcnt(0): the wave's own weights
 #pragma unroll 1
-                    for (int key = 0; key < kAttnK; ++key) {
-                        const float p = (float) w[key * 32 + col];
-                        LdsPtr      v = lds + BUF + TILE + key * ROW + 8 * h;
+                    for (int key = half * 32; key < min(half * 32 + 32, nk - key0); ++key) {
+                        const float p = (float) w[(key & 31) * 32 + col];
+                        const T    *v = rows + (int64_t) key * a.v_row + 4 * h;
 #pragma unroll
                         for (int d = 0; d < DB; ++d)
 #pragma unroll
                             for (int r = 0; r < 4; ++r) {
-                                const auto x = *(__attribute__((address_space(3))) const typename A::V4 *) (v + (((4 * d + r) ^ v_swizzle<DP>(key)) << 4));
+                                if (32 * d + 8 * r + 4 * h >= D) continue;
+                                const typename A::V4 x = *reinterpret_cast<const typename A::V4 *>(v + 32 * d + 8 * r);
 #pragma unroll
                                 for (int j = 0; j < 4; ++j) {
                                     const float y = (float) x[j];
@@ -266,7 +265,9 @@ namespace vkhip {
                                 }
                             }
                     }
+                    __builtin_amdgcn_s_waitcnt(0xC07F); // read before the next half is written
                 }
+            }
         };
 
         // tile t has landed (every wave's pieces), and nobody reads tile t - 1 any more
@@ -281,15 +282,36 @@ namespace vkhip {
         for (; t < plain; t += 2) {
             landed();
             issue(t + 1, odd);
-            if (used) tile(t, even, std::false_type());
+            if (used) tile(t, even, std::false_type(), false);
             landed();
             if (t + 2 < tiles) issue(t + 2, even);
-            if (used) tile(t + 1, odd, std::false_type());
+            if (used) tile(t + 1, odd, std::false_type(), false);
         }
+        __attribute__((address_space(3))) unsigned *found = (__attribute__((address_space(3))) unsigned *) (lds + 4 * TILE + 4 * kAttnK * 32);
         for (; t < tiles; ++t) {
-            landed();
+            const int parity = t & 1;
+            __builtin_amdgcn_s_waitcnt(7 << 4); // vmcnt(0), lgkmcnt(0)
+            unsigned any = 0;
+#pragma unroll
+            for (int r = 0; r < LOADS; ++r) {
+                LdsPtr   at = lds + parity * (2 * TILE) + TILE + (wave * LOADS + r) * 1024 + lane * 16;
+                tk_u32x4 v  = lds_read16(at);
+                unsigned hit = 0;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const unsigned bad = not_finite(v[j]);
+                    hit |= bad;
+                    v[j] &= ~((bad >> 15) * 0xFFFFu);
+                }
+                if (hit) *(__attribute__((address_space(3))) tk_u32x4 *) at = v;
+                any |= hit;
+            }
+            const bool mine = __any(any != 0);
+            if (lane == 0) found[parity * 4 + wave] = mine;
+            __builtin_amdgcn_s_waitcnt(0xC07F); // lgkmcnt(0)
+            __asm__ volatile("s_barrier" ::: "memory");
             if (t + 1 < tiles) issue(t + 1, t + 1 & 1);
-            if (t < used) tile(t, t & 1, std::true_type());
+            if (t < used) tile(t, parity, std::true_type(), __builtin_amdgcn_readfirstlane(found[parity * 4] | found[parity * 4 + 1] | found[parity * 4 + 2] | found[parity * 4 + 3]) != 0);
         }
 
         l += __shfl_xor(l, 32);
