@@ -454,8 +454,8 @@ int vkhip_resize_nearest_view(const void *x, int64_t x_pstride, void *y, int64_t
 
 /* Group norm with an activation: y = act((x - mean) * rstd * gamma[c] + beta[c]), mean and biased
  * variance over the H*W pixels and C/groups channels of a group of one image, rstd = 1/sqrt(var + eps).
- *   x_fmt / y_fmt: 1 NHWC (rows of C channels, one per pixel) or 2 NC4HW4 (F16 only; channels past C
- *           are not read and written +0), independently.
+ *   x_fmt / y_fmt: 1 NHWC (rows of C channels, one per pixel) or 2 NC4HW4 (F16 only; the lanes of
+ *           channels past C are not used, and written +0), independently.
  *   x_row / y_row: elements from one NHWC row to the next (0 = C), for rows that are slices of wider ones.
  *   gamma, beta: fp32 [C] on the device; NULL = 1 and 0.
  * y may be x where format and rows agree. workspace: vkhip_group_norm_workspace_bytes (0 for a
@@ -477,9 +477,10 @@ int    vkhip_group_norm(const vkhip_group_norm_desc *d, const void *x, const flo
  *   o = sum_j softmax_j(scale * q . k_j) v_j over every key of the sequence or, with causal, over the keys
  *   j <= i + nk - nq for query i of nq (the last query sees the last key).
  * A query that sees no key gives zeros. What a query does not see never reaches it, NaN and
- * infinities included. F16 or BF16; head_dim a multiple of 8 up to 128; scale > 0; every row of every
- * head starts on a 16-byte boundary. o must not overlap q, k or v. workspace:
- * vkhip_attention_workspace_bytes (may be 0: then NULL is taken). */
+ * infinities included. Weights are rounded to the 16-bit type before they multiply v, their sum is not.
+ * F16 or BF16; head_dim a multiple of 8 up to 128; scale > 0; every row of every head starts on a
+ * 16-byte boundary; k_row and v_row head_dim .. 2^23. o must not overlap q, k or v. workspace:
+ * vkhip_attention_workspace_bytes (0: NULL is taken), 16-byte aligned, contents undefined. */
 typedef struct vkhip_attention_desc {
     int32_t batch, q_heads, kv_heads, head_dim;
     int32_t total_q, total_k; /* rows of q and o, and of k and v */
@@ -518,16 +519,18 @@ typedef struct vkhip_kv_rows {
  * Per page and head: s = max(s0, max|x| / 127) over the rows x that join it, s0 the scale of the tokens
  * already there (0 for none); if the scale grew those become rint(q * (s0 / s)), the new ones
  * rint(x / s). A NaN or infinity among the rows makes the scale NaN: all that the page holds reads as NaN
- * until it begins anew. A page that two sequences share must not be appended to. */
+ * until it begins anew. Rows past max_blocks * page_tokens are dropped. A page that two sequences share must
+ * not be appended to. */
 int vkhip_kv_append(const vkhip_kv_cache *c, const vkhip_kv_rows *r, const void *k, const void *v, const int32_t *cu, const int32_t *lens,
                     vkhip_stream_t s);
 /* The tokens start[b] .. start[b] + cu[b+1] - cu[b] of sequence b as the rows cu[b] .. cu[b+1]: what prompt
- * attention behind a cached prefix takes. */
+ * attention behind a cached prefix takes. Rows of tokens past max_blocks * page_tokens are not written. */
 int vkhip_kv_read(const vkhip_kv_cache *c, const vkhip_kv_rows *r, const int32_t *start, const int32_t *cu, void *k, void *v, vkhip_stream_t s);
 /* Attention over the cache: the last q_tokens (1 .. 64) tokens of each sequence of lens[b] tokens, query t at
  * position lens[b] - q_tokens + t, over the tokens up to its own position. q and o: row b * q_tokens + t,
  * F16 or BF16, 16-byte aligned rows per head. max_len: no length is larger (0: max_blocks * page_tokens);
- * it sizes the launch, longer sequences are cut to it. A query that sees no token gives zeros. */
+ * it sizes the launch, longer sequences are cut to it. A query that sees no token gives zeros. workspace:
+ * vkhip_kv_attention_workspace_bytes (0: NULL is taken), 16-byte aligned, contents undefined. */
 typedef struct vkhip_kv_attention_desc {
     int32_t q_heads, q_tokens, dtype, max_len;
     float   scale;

@@ -54,6 +54,11 @@ def test_attention_refuses_pointers(at):
         refused(V.vkhip().vkhip_attention_packed(R(V.AttentionDesc(**AT)), *p, A, None), "attention_packed")
 
 
+@pytest.mark.parametrize("change", [dict(k_row=56), dict(v_row=0)])
+def test_attention_refuses_overlapping_rows(change):
+    refused(V.vkhip().vkhip_attention_packed(R(V.AttentionDesc(**{**AT, **change})), A, A, A, A, A, A, A, None), "attention_packed")
+
+
 def cache(**change):
     return V.KvCache(**{**dict(k=A, v=A, k_scale=A, v_scale=A, table=A, pages=8, page_tokens=64, kv_heads=2, head_dim=64, batch=2, max_blocks=4), **change})
 
