@@ -19,13 +19,12 @@ import numpy as np
 import pytest
 
 import vknn_amd as V
-from vknn_amd import check
+from vknn_amd import DeviceBuffer, check
 
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
 
 DT = {"f16": (torch.float16, V.DT_F16, 2.0 ** -11), "bf16": (torch.bfloat16, V.DT_BF16, 2.0 ** -8), "f32": (torch.float32, V.DT_F32, 2.0 ** -24)}
-TORCH_STREAM = 1  # the runtime's handle of the default stream, where torch works; NULL is the library's own
 TINY = {"f16": 2.0 ** -25, "bf16": 1e-38, "f32": 1e-38}
 
 
@@ -33,13 +32,58 @@ def rand(seed, *shape):
     return torch.randn(shape, generator=torch.Generator().manual_seed(seed))
 
 
+class Dev:
+    """A CPU tensor's copy in device memory (torch computes on the CPU here: its own GPU runtime is not needed)."""
+
+    def __init__(self, t):
+        self.shape, self.dtype = t.shape, t.dtype
+        self.nbytes = t.numel() * t.element_size()
+        self.buf = DeviceBuffer(max(self.nbytes, 16))
+        self.put(t)
+
+    @classmethod
+    def zeros(cls, shape, dtype):
+        self = cls.__new__(cls)
+        self.shape, self.dtype, self.nbytes = torch.Size(shape), dtype, math.prod(shape) * torch.empty(0, dtype=dtype).element_size()
+        self.buf = DeviceBuffer(self.nbytes)
+        self.buf.zero()
+        return self
+
+    def data_ptr(self):
+        return self.buf.ptr
+
+    def put(self, t):
+        assert t.shape == self.shape and t.dtype == self.dtype
+        if self.nbytes:
+            self.buf.upload(t.contiguous().flatten().view(torch.uint8).numpy())
+
+    def get(self):
+        return torch.from_numpy(self.buf.download(np.uint8, self.nbytes)).view(self.dtype).view(self.shape)
+
+    def rows(self, ids):
+        """Some entries of the first axis, without the others."""
+        each = self.nbytes // self.shape[0]
+        out = np.empty((len(ids), each), np.uint8)
+        for i, k in enumerate(ids):
+            check(V.vkhip().vkhip_memcpy_d2h(out[i].ctypes.data, self.buf.ptr + int(k) * each, each, None), "d2h")
+        return torch.from_numpy(out.reshape(-1)).view(self.dtype).view(len(ids), *self.shape[1:])
+
+
+def full(shape, value, dtype):
+    return Dev(torch.full(shape, value, dtype=dtype))
+
+
 def ints(a):
-    return torch.tensor(a, dtype=torch.int32, device="cuda")
+    return Dev(torch.tensor(a, dtype=torch.int32))
 
 
 def workspace(n):
     """Scratch with NaN bit patterns: what is read without being written shows."""
-    return torch.full((max(n, 16),), 255, dtype=torch.uint8, device="cuda")
+    return full((max(n, 16),), 255, torch.uint8)
+
+
+def sync():
+    check(V.vkhip().vkhip_device_sync(), "sync")
 
 
 # ------------------------------------------------------------------------------------ group norm
@@ -60,32 +104,34 @@ def from_nc4(y, c):
     return y.permute(0, 2, 1, 3).reshape(y.shape[0], y.shape[2], -1)[:, :, :c]
 
 
-def group_norm(lib, x, groups, gamma, beta, dtype="f16", xf=1, yf=1, act=0, lo=0.0, hi=0.0, eps=1e-5, h=None, x_pad=0, y_pad=0, stream=TORCH_STREAM, inplace=False):
+def group_norm(lib, x, groups, gamma, beta, dtype="f16", xf=1, yf=1, act=0, lo=0.0, hi=0.0, eps=1e-5, h=None, x_pad=0, y_pad=0, stream=None, inplace=False):
     """x: [n, p, c] CPU values of the type; the output [n, p, c], and what lay beside its rows."""
     n, p, c = x.shape
     dt, code, _ = DT[dtype]
     h = h or p
     if xf == 2:
-        dx = to_nc4(x).to(dt).cuda()
+        dx = Dev(to_nc4(x).to(dt))
     else:
-        dx = torch.full((n, p, c + x_pad), float("nan"), dtype=dt, device="cuda")
-        dx[:, :, :c] = x.to(dt).cuda()
-    dy = dx if inplace else (torch.full((n, (c + 3) // 4, p, 4), 7.0, dtype=dt, device="cuda") if yf == 2 else torch.full((n, p, c + y_pad), 7.0, dtype=dt, device="cuda"))
+        rows = torch.full((n, p, c + x_pad), float("nan"), dtype=dt)
+        rows[:, :, :c] = x.to(dt)
+        dx = Dev(rows)
+    dy = dx if inplace else full((n, (c + 3) // 4, p, 4) if yf == 2 else (n, p, c + y_pad), 7.0, dt)
     d = V.GroupNormDesc(N=n, C=c, H=h, W=p // h, groups=groups, x_fmt=xf, y_fmt=yf, dtype=code, act=act, act_lo=lo, act_hi=hi, eps=eps,
                         x_row=c + x_pad if x_pad else 0, y_row=c + y_pad if y_pad else 0)
     ws = workspace(lib.vkhip_group_norm_workspace_bytes(ctypes.byref(d)))
-    g, b = (None if t is None else t.float().cuda() for t in (gamma, beta))
-    torch.cuda.synchronize()
+    g, b = (None if t is None else Dev(t.float()) for t in (gamma, beta))
+    sync()
     check(lib.vkhip_group_norm(ctypes.byref(d), dx.data_ptr(), None if g is None else g.data_ptr(), None if b is None else b.data_ptr(), dy.data_ptr(), ws.data_ptr(),
                                stream), "group_norm")
-    torch.cuda.synchronize()
+    sync()
     if yf == 2:
-        full = dy.cpu().permute(0, 2, 1, 3).reshape(n, p, -1)
-        assert (full[:, :, c:] == 0).all(), "channels past C are zero"
-        return full[:, :, :c].double()
+        y = dy.get().permute(0, 2, 1, 3).reshape(n, p, -1)
+        assert (y[:, :, c:] == 0).all(), "channels past C are zero"
+        return y[:, :, :c].double()
+    y = dy.get()
     if not inplace:
-        assert (dy[:, :, c:] == 7.0).all(), "nothing beside the rows is written"
-    return dy.cpu()[:, :, :c].double()
+        assert (y[:, :, c:] == 7.0).all(), "nothing beside the rows is written"
+    return y[:, :, :c].double()
 
 
 def check_gn(y, x, groups, gamma, beta, dtype, act, lo=0.0, hi=0.0, eps=1e-5):
@@ -157,27 +203,32 @@ def test_group_norm_in_place_and_empty(gpu):
 
 
 # ------------------------------------------------------------------------------------ packed attention
-def attention(lib, q, k, v, nq, nk, causal, dtype, scale, stream=TORCH_STREAM, joint=False, o_pad=0):
+def attention(lib, q, k, v, nq, nk, causal, dtype, scale, stream=None, joint=False, o_pad=0):
     """q [sum nq, hq, d], k, v [sum nk, hkv, d]; joint: the three are slices of one row matrix."""
     dt, code, _ = DT[dtype]
     hq, hkv, d = q.shape[1], k.shape[1], q.shape[2]
     if joint:
-        rows = torch.cat([q.flatten(1), k.flatten(1), v.flatten(1)], 1).to(dt).cuda()
-        dq, dk, dv = (t.unflatten(1, (-1, d)) for t in rows.split([hq * d, hkv * d, hkv * d], 1))
+        rows = Dev(torch.cat([q.flatten(1), k.flatten(1), v.flatten(1)], 1).to(dt))
+        width = (hq + 2 * hkv) * d
+        ptr = [rows.data_ptr(), rows.data_ptr() + hq * d * 2, rows.data_ptr() + (hq + hkv) * d * 2]
+        strides = [(width, d)] * 3
     else:  # heads outside rows
-        dq, dk, dv = (t.transpose(0, 1).contiguous().to(dt).cuda().transpose(0, 1) for t in (q, k, v))
-    out = torch.full((q.shape[0], hq, d + o_pad), 7.0, dtype=dt, device="cuda")
+        held = [Dev(t.transpose(0, 1).contiguous().to(dt)) for t in (q, k, v)]
+        ptr = [t.data_ptr() for t in held]
+        strides = [(d, t.shape[0] * d) for t in (q, k, v)]
+    out = full((q.shape[0], hq, d + o_pad), 7.0, dt)
     desc = V.AttentionDesc(batch=len(nq), q_heads=hq, kv_heads=hkv, head_dim=d, total_q=q.shape[0], total_k=k.shape[0], dtype=code, causal=int(causal), scale=scale,
-                           q_row=dq.stride(0), q_head=dq.stride(1), k_row=dk.stride(0), k_head=dk.stride(1), v_row=dv.stride(0), v_head=dv.stride(1),
-                           o_row=out.stride(0), o_head=out.stride(1))
+                           q_row=strides[0][0], q_head=strides[0][1], k_row=strides[1][0], k_head=strides[1][1], v_row=strides[2][0], v_head=strides[2][1],
+                           o_row=hq * (d + o_pad), o_head=d + o_pad)
     cq, ck = ints(np.cumsum([0] + list(nq)).tolist()), ints(np.cumsum([0] + list(nk)).tolist())
     ws = workspace(lib.vkhip_attention_workspace_bytes(ctypes.byref(desc)))
-    torch.cuda.synchronize()
-    check(lib.vkhip_attention_packed(ctypes.byref(desc), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), cq.data_ptr(), ck.data_ptr(), out.data_ptr(), ws.data_ptr(), stream),
+    sync()
+    check(lib.vkhip_attention_packed(ctypes.byref(desc), *ptr, cq.data_ptr(), ck.data_ptr(), out.data_ptr(), ws.data_ptr(), stream),
           "attention_packed")
-    torch.cuda.synchronize()
+    sync()
+    out = out.get()
     assert (out[:, :, d:] == 7.0).all()
-    return out[:, :, :d].cpu().double()
+    return out[:, :, :d].double()
 
 
 def attention64(q, k, v, see, scale):
@@ -279,43 +330,45 @@ class Cache:
         g = torch.Generator().manual_seed(seed)
         self.table = torch.randperm(self.pages, generator=g)[:batch * blocks].view(batch, blocks).int()
         # what a recycled page holds: anything, scales not finite
-        self.k = torch.randint(-128, 128, (self.pages, heads, page, self.dp), generator=g, dtype=torch.int8).cuda()
-        self.v = torch.randint(-128, 128, (self.pages, heads, self.dp, page), generator=g, dtype=torch.int8).cuda()
-        self.ks = torch.full((self.pages, heads), float("nan"), device="cuda")
-        self.vs = torch.full((self.pages, heads), float("nan"), device="cuda")
-        self.gpu_table = self.table.cuda()
+        self.k = Dev(torch.randint(-128, 128, (self.pages, heads, page, self.dp), generator=g, dtype=torch.int8))
+        self.v = Dev(torch.randint(-128, 128, (self.pages, heads, self.dp, page), generator=g, dtype=torch.int8))
+        self.ks = full((self.pages, heads), float("nan"), torch.float32)
+        self.vs = full((self.pages, heads), float("nan"), torch.float32)
+        self.gpu_table = Dev(self.table)
 
     def desc(self):
         return V.KvCache(k=self.k.data_ptr(), v=self.v.data_ptr(), k_scale=self.ks.data_ptr(), v_scale=self.vs.data_ptr(), table=self.gpu_table.data_ptr(), pages=self.pages,
                          page_tokens=self.page, kv_heads=self.heads, head_dim=self.d, batch=self.batch, max_blocks=self.blocks)
 
-    def rows(self, k, v, code):
-        return V.KvRows(dtype=code, total=k.shape[0], k_row=k.stride(0), k_head=k.stride(1), v_row=v.stride(0), v_head=v.stride(1))
+    def rows(self, k, code):
+        row, head = self.heads * k.shape[2], k.shape[2]
+        return V.KvRows(dtype=code, total=k.shape[0], k_row=row, k_head=head, v_row=row, v_head=head)
 
-    def append(self, k, v, new, lens, dtype, stream=TORCH_STREAM):
+    def append(self, k, v, new, lens, dtype, stream=None):
         dt, code, _ = DT[dtype]
-        k, v = k.to(dt).cuda(), v.to(dt).cuda()
+        k, v = Dev(k.to(dt)), Dev(v.to(dt))
         cu, at = ints(np.cumsum([0] + list(new)).tolist()), ints(lens)
-        torch.cuda.synchronize()
-        check(V.vkhip().vkhip_kv_append(ctypes.byref(self.desc()), ctypes.byref(self.rows(k, v, code)), k.data_ptr(), v.data_ptr(), cu.data_ptr(), at.data_ptr(), stream))
-        torch.cuda.synchronize()
+        sync()
+        check(V.vkhip().vkhip_kv_append(ctypes.byref(self.desc()), ctypes.byref(self.rows(k, code)), k.data_ptr(), v.data_ptr(), cu.data_ptr(), at.data_ptr(), stream))
+        sync()
 
     def read(self, start, count, dtype, pad=0):
         dt, code, _ = DT[dtype]
-        k, v = (torch.full((sum(count), self.heads, self.d + pad), 7.0, dtype=dt, device="cuda") for _ in range(2))
+        k, v = (full((sum(count), self.heads, self.d + pad), 7.0, dt) for _ in range(2))
         cu, at = ints(np.cumsum([0] + list(count)).tolist()), ints(start)
-        torch.cuda.synchronize()
-        check(V.vkhip().vkhip_kv_read(ctypes.byref(self.desc()), ctypes.byref(self.rows(k, v, code)), at.data_ptr(), cu.data_ptr(), k.data_ptr(), v.data_ptr(), TORCH_STREAM))
-        torch.cuda.synchronize()
+        sync()
+        check(V.vkhip().vkhip_kv_read(ctypes.byref(self.desc()), ctypes.byref(self.rows(k, code)), at.data_ptr(), cu.data_ptr(), k.data_ptr(), v.data_ptr(), None))
+        sync()
+        k, v = k.get(), v.get()
         assert (k[:, :, self.d:] == 7.0).all() and (v[:, :, self.d:] == 7.0).all()
-        return k[:, :, :self.d].cpu(), v[:, :, :self.d].cpu()
+        return k[:, :, :self.d], v[:, :, :self.d]
 
     def bytes_of(self, b, n):
         """The stored bytes [n, heads, d] of sequence b and each token's scale [n, heads], keys and values."""
         ids = self.table[b, :-(-n // self.page)].long()
-        k = self.k.cpu()[ids].permute(0, 2, 1, 3).reshape(-1, self.heads, self.dp)[:n, :, :self.d]
-        v = self.v.cpu()[ids].permute(0, 3, 1, 2).reshape(-1, self.heads, self.dp)[:n, :, :self.d]
-        return [(x, s.cpu()[ids].repeat_interleave(self.page, 0)[:n]) for x, s in ((k, self.ks), (v, self.vs))]
+        k = self.k.rows(ids).permute(0, 2, 1, 3).reshape(-1, self.heads, self.dp)[:n, :, :self.d]
+        v = self.v.rows(ids).permute(0, 3, 1, 2).reshape(-1, self.heads, self.dp)[:n, :, :self.d]
+        return [(x, s.rows(ids).repeat_interleave(self.page, 0)[:n]) for x, s in ((k, self.ks), (v, self.vs))]
 
 
 def append64(q, s, x, n0, page):
@@ -405,12 +458,14 @@ def test_append_not_finite(gpu, bad):
 
 def test_cache_blocks_without_memory(gpu):
     c = Cache(2, 3, 32, 1, 64)
-    c.gpu_table[0, 1], c.gpu_table[1, 0], c.gpu_table[1, 2] = -1, c.pages, 1 << 30
-    before = [t.clone() for t in (c.k, c.v, c.ks, c.vs)]
+    names = c.table.clone()
+    names[0, 1], names[1, 0], names[1, 2] = -1, c.pages, 1 << 30
+    c.gpu_table.put(names)
+    before = [t.get() for t in (c.k, c.v, c.ks, c.vs)]
     k, v = rand(3, 160, 1, 64), rand(4, 160, 1, 64)
     c.append(k, v, [80, 80], [0, 0], "f16")
     used = {int(c.table[0, 0]), int(c.table[0, 2]), int(c.table[1, 1])}
-    for was, now in zip(before, (c.k, c.v, c.ks, c.vs)):
+    for was, now in zip(before, [t.get() for t in (c.k, c.v, c.ks, c.vs)]):
         for p in set(range(c.pages)) - used:
             assert torch.equal(was[p].nan_to_num(1.5), now[p].nan_to_num(1.5)) if was.is_floating_point() else torch.equal(was[p], now[p])
     rk, _ = c.read([0, 0], [80, 80], "f16")
@@ -420,20 +475,21 @@ def test_cache_blocks_without_memory(gpu):
 
 
 # ------------------------------------------------------------------------------------ attention over the cache
-def kv_attention(lib, c, q, lens, dtype, scale, max_len=0, stream=TORCH_STREAM, o_pad=0):
+def kv_attention(lib, c, q, lens, dtype, scale, max_len=0, stream=None, o_pad=0):
     """q [batch, t, heads, d]"""
     dt, code, _ = DT[dtype]
-    dq = q.to(dt).cuda()
+    dq = Dev(q.to(dt))
     b, t, hq, d = q.shape
-    out = torch.full((b, t, hq, d + o_pad), 7.0, dtype=dt, device="cuda")
-    desc = V.KvAttentionDesc(q_heads=hq, q_tokens=t, dtype=code, max_len=max_len, scale=scale, q_row=dq.stride(1), q_head=dq.stride(2), o_row=out.stride(1), o_head=out.stride(2))
+    out = full((b, t, hq, d + o_pad), 7.0, dt)
+    desc = V.KvAttentionDesc(q_heads=hq, q_tokens=t, dtype=code, max_len=max_len, scale=scale, q_row=hq * d, q_head=d, o_row=hq * (d + o_pad), o_head=d + o_pad)
     cd, n = c.desc(), ints(lens)
     ws = workspace(lib.vkhip_kv_attention_workspace_bytes(ctypes.byref(desc), ctypes.byref(cd)))
-    torch.cuda.synchronize()
+    sync()
     check(lib.vkhip_kv_attention(ctypes.byref(desc), ctypes.byref(cd), dq.data_ptr(), n.data_ptr(), out.data_ptr(), ws.data_ptr(), stream), "kv_attention")
-    torch.cuda.synchronize()
+    sync()
+    out = out.get()
     assert (out[..., d:] == 7.0).all()
-    return out[..., :d].cpu().double()
+    return out[..., :d].double()
 
 
 def filled(batch, lens, page, heads, d, seed=0, blocks=None):
@@ -497,11 +553,15 @@ def test_kv_attention_spoiled_pages(gpu):
     c = filled(2, lens, 32, 1, 64, seed=5)
     q = rand(12, 2, 8, 2, 64)
     clean = kv_attention(V.vkhip(), c, q.half().float(), lens, "f16", 0.125)
-    c.ks[int(c.table[0, 3])] = float("nan")  # holds tokens 96 .. 99
-    c.vs[int(c.table[0, 3])] = float("nan")
+    for scales in (c.ks, c.vs):
+        spoiled = scales.get()
+        spoiled[int(c.table[0, 3])] = float("nan")  # holds tokens 96 .. 99
+        scales.put(spoiled)
     out = kv_attention(V.vkhip(), c, q.half().float(), lens, "f16", 0.125)
     assert torch.equal(out[0, :4], clean[0, :4]) and torch.isnan(out[0, 4:]).all() and torch.equal(out[1], clean[1])
-    c.gpu_table[0, 3], c.gpu_table[1, 1] = -1, c.pages + 5
+    names = c.table.clone()
+    names[0, 3], names[1, 1] = -1, c.pages + 5
+    c.gpu_table.put(names)
     out = kv_attention(V.vkhip(), c, q.half().float(), lens, "f16", 0.125)
     assert torch.isfinite(out).all() and torch.equal(out[0, :4], clean[0, :4])
     (kq, ks), (vq, vs) = c.bytes_of(1, 100)
@@ -509,7 +569,7 @@ def test_kv_attention_spoiled_pages(gpu):
     keep[32:64] = False
     k, v = (kq.double() * ks.double()[:, :, None])[keep], (vq.double() * vs.double()[:, :, None])[keep]
     check_attention(out[1], q[1].half().double(), k, v, [8], [68], True, "f16", 0.125)
-    c.gpu_table[:] = -1
+    c.gpu_table.put(torch.full_like(c.table, -1))
     assert (kv_attention(V.vkhip(), c, q.half().float(), lens, "f16", 0.125) == 0).all()
 
 
@@ -532,23 +592,20 @@ def test_kv_long_cache(gpu):
     c = Cache.__new__(Cache)
     c.page, c.heads, c.d, c.dp, c.batch, c.blocks, c.pages = page, heads, d, 128, 1, blocks, pages
     c.table = (pages - 1 - torch.arange(blocks)).view(1, blocks).int()
-    c.gpu_table = c.table.cuda()
-    c.k = torch.zeros((pages, heads, page, d), dtype=torch.int8, device="cuda")
-    c.v = torch.zeros((pages, heads, d, page), dtype=torch.int8, device="cuda")
-    c.ks, c.vs = torch.zeros((pages, heads), device="cuda"), torch.zeros((pages, heads), device="cuda")
+    c.gpu_table = Dev(c.table)
+    c.k, c.v = Dev.zeros((pages, heads, page, d), torch.int8), Dev.zeros((pages, heads, d, page), torch.int8)
+    c.ks, c.vs = Dev.zeros((pages, heads), torch.float32), Dev.zeros((pages, heads), torch.float32)
     k, v = rand(1, 70001, heads, d), rand(2, 70001, heads, d)
     c.append(k, v, lens, [0], "f16")
     rk, rv = c.read([69990], [11], "f16")
-    ids = c.table[0].long().cuda()
-    low = torch.ones(pages, dtype=torch.bool, device="cuda")
+    ids, ks, vs = c.table[0].long(), c.ks.get(), c.vs.get()
+    low = torch.ones(pages, dtype=torch.bool)
     low[ids] = False
-    assert (c.ks[low] == 0).all() and (c.ks[ids] > 0).all()
-    assert (rk.float() - k[69990:].half().float()).abs().max() <= 0.51 * c.ks[ids].max().item() + 1e-3
-    small = Cache.__new__(Cache)
-    small.__dict__.update(c.__dict__, k=c.k[ids].cpu(), v=c.v[ids].cpu(), ks=c.ks[ids].cpu(), vs=c.vs[ids].cpu(), table=torch.arange(blocks).view(1, blocks))
+    assert (ks[low] == 0).all() and (ks[ids] > 0).all()
+    assert (rk.float() - k[69990:].half().float()).abs().max() <= 0.51 * ks[ids].max().item() + 1e-3
+    assert (rv.float() - v[69990:].half().float()).abs().max() <= 0.51 * vs[ids].max().item() + 1e-3
     q = rand(3, 1, 1, 8, d).half().float()
-    check_kv_attention(kv_attention(V.vkhip(), c, q, lens, "f16", 0.09), small, q, lens, "f16", 0.09)
-    assert (rv.float() - v[69990:].half().float()).abs().max() <= 0.51 * c.vs[ids].max().item() + 1e-3
+    check_kv_attention(kv_attention(V.vkhip(), c, q, lens, "f16", 0.09), c, q, lens, "f16", 0.09)
 
 
 # ------------------------------------------------------------------------------------ streams and graphs
@@ -558,9 +615,9 @@ def test_own_stream_and_graph_replay(gpu):
     s, g = ctypes.c_void_p(), ctypes.c_void_p()
     check(lib.vkhip_stream_create(ctypes.byref(s)))
     n, p, c, heads, d = 2, 96, 64, 2, 32
-    x = torch.zeros((n, c // 4, p, 4), dtype=torch.float16, device="cuda")
-    tok, att = (torch.zeros((n * p, c), dtype=torch.float16, device="cuda") for _ in range(2))
-    step = torch.zeros((n, 1, heads, d), dtype=torch.float16, device="cuda")
+    x = full((n, c // 4, p, 4), 0.0, torch.float16)
+    tok, att = (full((n * p, c), 0.0, torch.float16) for _ in range(2))
+    step = full((n, 1, heads, d), 0.0, torch.float16)
     cache = Cache(n, 3, 32, heads, d)
     cu, zero, lens = ints([0, p, 2 * p]), ints([0, 0]), ints([p, p])
     gn = V.GroupNormDesc(N=n, C=c, H=8, W=12, groups=8, x_fmt=2, y_fmt=1, dtype=0, act=5, eps=1e-5)
@@ -579,23 +636,23 @@ def test_own_stream_and_graph_replay(gpu):
         check(lib.vkhip_kv_append(r(cd), r(rows), tok.data_ptr(), tok.data_ptr(), cu.data_ptr(), zero.data_ptr(), s))
         check(lib.vkhip_kv_attention(r(kd), r(cd), att.data_ptr(), lens.data_ptr(), step.data_ptr(), w3.data_ptr(), s))
 
-    torch.cuda.synchronize()
+    sync()
     check(lib.vkhip_graph_begin(s))
     chain()
     check(lib.vkhip_graph_end(s, ctypes.byref(g)))
     for i in range(4):
-        x.copy_(torch.randn(x.shape, generator=torch.Generator().manual_seed(i)).half())
+        x.put(rand(i, *x.shape).half())
         got = []
         for how in ("eager", "graph"):
             for t in (tok, att, step):
-                t.fill_(9.0)
-            torch.cuda.synchronize()
+                t.put(torch.full(t.shape, 9.0, dtype=t.dtype))
+            sync()
             if how == "eager":
                 chain()
             else:
                 check(lib.vkhip_graph_launch(g, s))
             check(lib.vkhip_stream_sync(s))
-            got.append([t.cpu().clone() for t in (tok, att, step, cache.ks, cache.vs)])
+            got.append([t.get() for t in (tok, att, step, cache.ks, cache.vs)])
         for a, b in zip(*got):
             assert torch.isfinite(a[:4]).all() and torch.equal(a.nan_to_num(5.5), b.nan_to_num(5.5))
     check(lib.vkhip_graph_destroy(g))
