@@ -88,8 +88,13 @@ namespace vkhip {
         constexpr int TILE   = kAttnK * ROW;      // bytes of a K or V tile
         constexpr int LOADS  = TILE / 1024 / 4;   // wave loads of 1 KB per wave and tile
         constexpr int KS = DP / 16, DB = DP / 32; // contraction steps of a score, 32-channel blocks of the output
-        __shared__ __attribute__((aligned(1024))) unsigned char sm[4 * TILE + 4 * kAttnK * 32 + 32]; // K, V of even tiles, of odd ones, the waves' weights and findings
-        LdsPtr lds = (LdsPtr) sm;
+        // arrays of their own for K and V of even and odd tiles: the compiler then knows that a read of one does not
+        // have to wait for the copies into the others
+        __shared__ __attribute__((aligned(1024))) unsigned char sm_k0[TILE], sm_v0[TILE], sm_k1[TILE], sm_v1[TILE];
+        __shared__ __attribute__((aligned(16))) unsigned char   sm_w[4 * kAttnK * 32]; // the waves' weights of 32 keys
+        __shared__ unsigned                                     found[8];
+        const auto k_tile = [&](auto odd_c) { return odd_c ? (LdsPtr) sm_k1 : (LdsPtr) sm_k0; };
+        const auto v_tile = [&](auto odd_c) { return odd_c ? (LdsPtr) sm_v1 : (LdsPtr) sm_v0; };
 
         const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, col = lane & 31;
         // heads of one key/value head next to each other in the grid: workgroups go to the 8 XCDs in turn
@@ -150,24 +155,24 @@ namespace vkhip {
             const __amdgpu_buffer_rsrc_t kr = __builtin_amdgcn_make_buffer_rsrc((void *) kb, (short) 0, rows * k_bytes + D * 2, 0x00020000);
             const __amdgpu_buffer_rsrc_t vr = __builtin_amdgcn_make_buffer_rsrc((void *) vb, (short) 0, rows * v_bytes + D * 2, 0x00020000);
             kb += (int64_t) kAttnK * k_bytes, vb += (int64_t) kAttnK * v_bytes;
-            LdsPtr dst = lds + odd_c * (2 * TILE) + wave * (LOADS * 1024);
+            const LdsPtr kd = k_tile(odd_c) + wave * (LOADS * 1024), vd = v_tile(odd_c) + wave * (LOADS * 1024);
 #pragma unroll
-            for (int r = 0; r < LOADS; ++r) __builtin_amdgcn_raw_ptr_buffer_load_lds(kr, dst + r * 1024, 16, off_k[r], 0, 0, 0);
+            for (int r = 0; r < LOADS; ++r) __builtin_amdgcn_raw_ptr_buffer_load_lds(kr, kd + r * 1024, 16, off_k[r], 0, 0, 0);
 #pragma unroll
-            for (int r = 0; r < LOADS; ++r) __builtin_amdgcn_raw_ptr_buffer_load_lds(vr, dst + TILE + r * 1024, 16, off_v[r], 0, 0, 0);
+            for (int r = 0; r < LOADS; ++r) __builtin_amdgcn_raw_ptr_buffer_load_lds(vr, vd + r * 1024, 16, off_v[r], 0, 0, 0);
         };
 
-        // fragment addresses of an even tile: K row col, piece 2 c + h; V rows 4 h + (lane % 16) / 4 (+ 8), pieces 4 d + pp.
+        // fragment offsets in a tile: K row col, piece 2 c + h; V rows 4 h + (lane % 16) / 4 (+ 8), pieces 4 d + pp.
         // The swizzle is an xor of disjoint bits, so that rows further on are constant offsets.
-        LdsPtr ka[KS], va[DB][2];
+        unsigned ka[KS], va[DB][2];
 #pragma unroll
-        for (int c = 0; c < KS; ++c) ka[c] = lds + col * ROW + (((2 * c + h) ^ k_swizzle<DP>(col)) << 4);
+        for (int c = 0; c < KS; ++c) ka[c] = col * ROW + (((2 * c + h) ^ k_swizzle<DP>(col)) << 4);
 #pragma unroll
         for (int d = 0; d < DB; ++d)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const int row = 4 * h + ((lane & 15) >> 2) + 8 * e, piece = 4 * d + 2 * (lane >> 4 & 1) + ((lane & 3) >> 1);
-                va[d][e]      = lds + TILE + row * ROW + ((piece ^ v_swizzle<DP>(row)) << 4) + (lane & 1) * 8;
+                va[d][e]      = row * ROW + ((piece ^ v_swizzle<DP>(row)) << 4) + (lane & 1) * 8;
             }
 
         float16v acc[DB];
@@ -185,7 +190,7 @@ namespace vkhip {
         // looks through the piece of V that it copied and clears what it finds (`spoiled`: something was); what the
         // queries do see of it is then added key by key, read from memory again.
         auto tile = [&](int t, auto odd_c, auto masked_c, bool spoiled) __attribute__((always_inline)) {
-            const int      BUF    = odd_c * (2 * TILE);
+            const LdsPtr   kt = k_tile(odd_c), vt = v_tile(odd_c);
             constexpr bool MASKED = decltype(masked_c)::value;
             const int      key0   = t * kAttnK;
             const auto     seen   = [&](int k, int j) { return key0 + 16 * k + 8 * (j >> 2) + 4 * h + (j & 3) < limit; };
@@ -195,7 +200,7 @@ namespace vkhip {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) s[kk][r] = 0.f;
 #pragma unroll
-                for (int c = 0; c < KS; ++c) s[kk] = A::mfma(__builtin_bit_cast(V8, lds_read16(ka[c] + BUF + kk * 32 * ROW)), qf[c], s[kk]);
+                for (int c = 0; c < KS; ++c) s[kk] = A::mfma(__builtin_bit_cast(V8, lds_read16(kt + ka[c] + kk * 32 * ROW)), qf[c], s[kk]);
             }
             if constexpr (MASKED) {
 #pragma unroll
@@ -236,7 +241,7 @@ namespace vkhip {
                     pf[kk * 2 + (r >> 3)][(r & 7) + 1] = x[1];
                 }
             const auto v_frag = [&](int d, int k) __attribute__((always_inline)) {
-                const tk_u32x2 x = lds_read_tr(va[d][0] + BUF + k * 16 * ROW), y = lds_read_tr(va[d][1] + BUF + k * 16 * ROW);
+                const tk_u32x2 x = lds_read_tr(vt + va[d][0] + k * 16 * ROW), y = lds_read_tr(vt + va[d][1] + k * 16 * ROW);
                 return tk_u32x4 {x[0], x[1], y[0], y[1]};
             };
 #pragma unroll
@@ -246,7 +251,7 @@ namespace vkhip {
                     acc[d] = A::mfma(__builtin_bit_cast(V8, v_frag(d, k)), pf[k], acc[d]);
                 }
             if (MASKED && spoiled) {
-                __attribute__((address_space(3))) T *w = (__attribute__((address_space(3))) T *) (lds + 4 * TILE + wave * (kAttnK * 32));
+                __attribute__((address_space(3))) T *w = (__attribute__((address_space(3))) T *) ((LdsPtr) sm_w + wave * (kAttnK * 32));
                 const T *rows = (const T *) a.v + (int64_t) (k0 + key0) * a.v_row + (int64_t) head_kv * a.v_head;
 #pragma unroll 1
                 for (int half = 0; half < 2; ++half) { // 32 keys at a time, their weights in LDS
@@ -296,14 +301,13 @@ namespace vkhip {
             if (t + 2 < tiles) issue(t + 2, even);
             if (used) tile(t + 1, odd, std::false_type(), false);
         }
-        __attribute__((address_space(3))) unsigned *found = (__attribute__((address_space(3))) unsigned *) (lds + 4 * TILE + 4 * kAttnK * 32);
         for (; t < tiles; ++t) {
             const int parity = t & 1;
             __builtin_amdgcn_s_waitcnt(7 << 4); // vmcnt(0), lgkmcnt(0)
             unsigned any = 0;
 #pragma unroll
             for (int r = 0; r < LOADS; ++r) {
-                LdsPtr   at = lds + parity * (2 * TILE) + TILE + (wave * LOADS + r) * 1024 + lane * 16;
+                LdsPtr   at = v_tile(parity) + (wave * LOADS + r) * 1024 + lane * 16;
                 tk_u32x4 v  = lds_read16(at);
                 unsigned hit = 0;
 #pragma unroll
