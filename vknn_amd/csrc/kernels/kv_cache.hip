@@ -15,10 +15,11 @@ namespace vkhip {
         int            total;
     };
 
-    // x / s to the nearest whole number. r = 1 / s: one remainder step makes x * r the correctly rounded
-    // quotient (but for rare last places). A scale so small that r or the remainder could leave the normal
+    // x / s to the nearest whole number, as the low byte of the result's bits (1.5 * 2^23 added: the sum's last place
+    // is 1). |x| is at most 127 s but for roundings. r = 1 / s: one remainder step makes x * r the correctly
+    // rounded quotient (but for rare last places). A scale so small that r or the remainder could leave the normal
     // range (bf16 rows near its smallest numbers) takes the division itself.
-    __device__ __forceinline__ int quantise(float x, float s, float r) {
+    __device__ __forceinline__ unsigned quantise(float x, float s, float r) {
         float q;
         if (s < 1e-30f) {
             q = s > 0.f ? x / s : 0.f;
@@ -26,7 +27,26 @@ namespace vkhip {
             q = x * r;
             q = __builtin_fmaf(__builtin_fmaf(-q, s, x), r, q);
         }
-        return clampi((int) rintf(q), -127, 127);
+        return __float_as_uint(q + 12582912.f);
+    }
+    __device__ __forceinline__ unsigned low_bytes(unsigned a, unsigned b, unsigned c, unsigned d) {
+        const unsigned ab = __builtin_amdgcn_perm(b, a, 0x0C0C0400u), cd = __builtin_amdgcn_perm(d, c, 0x0C0C0400u);
+        return ab | cd << 16;
+    }
+
+    // The largest magnitude of 8 values of 16 bits and a pair so far: without the sign their bits are ordered as they
+    // are, a NaN above infinity.
+    typedef unsigned short KvPair __attribute__((ext_vector_type(2)));
+    template <typename V>
+    __device__ __forceinline__ KvPair magnitude(KvPair m, V x) {
+        const tk_u32x4 b = __builtin_bit_cast(tk_u32x4, x);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) m = __builtin_elementwise_max(m, __builtin_bit_cast(KvPair, b[j] & 0x7FFF7FFFu));
+        return m;
+    }
+    template <typename T>
+    __device__ __forceinline__ float as_float(unsigned bits) {
+        return (float) __builtin_bit_cast(T, (unsigned short) bits);
     }
 
     // Sequence, block of page_tokens tokens, and the rows of the call that lie in it.
@@ -78,8 +98,8 @@ namespace vkhip {
         float         *scale  = (VALUES ? a.c.v_scale : a.c.k_scale) + at;
         unsigned char *page   = (VALUES ? a.c.v : a.c.k) + at * P * Dp;
 
-        V        x[R][4];
-        unsigned big = 0;
+        V      x[R][4];
+        KvPair most = {0, 0};
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             const Patch p = patch_of<THREADS>(r, quad0, dv);
@@ -96,22 +116,25 @@ namespace vkhip {
         for (int r = 0; r < R; ++r)
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-#pragma unroll
-                for (int j = 0; j < 8; ++j) big = max(big, __float_as_uint((float) x[r][k][j]) & 0x7FFFFFFFu);
+                most = magnitude(most, x[r][k]);
+        unsigned big = max((unsigned) most[0], (unsigned) most[1]);
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) big = max(big, (unsigned) __shfl_xor((int) big, o));
         if ((tid & 63) == 0) red[tid >> 6] = big;
         __syncthreads(); // also: every thread has read the old scale
 #pragma unroll
         for (int i = 0; i < THREADS / 64; ++i) big = max(big, red[i]);
-        const bool  bad = big >= 0x7F800000u || s0 != s0;
-        const float s = bad ? __builtin_nanf("") : fmaxf(s0, __uint_as_float(big) / 127.f), inv = 1.f / s;
+        const float largest = as_float<T>(big);
+        const bool  bad = !(largest < __builtin_inff()) || s0 != s0;
+        const float s = bad ? __builtin_nanf("") : fmaxf(s0, largest / 127.f), inv = 1.f / s;
         if (tid == 0) *scale = s;
         const bool  grown = !bad && s > s0 && w.n0 > 0;
         const float ratio = grown ? s0 / s : 1.f;
         const auto  again = [&](int q) { return (unsigned) (unsigned char) (int) rintf((float) (signed char) q * ratio); };
         const auto  again4 = [&](unsigned t) { return again(t & 255) | again(t >> 8 & 255) << 8 | again(t >> 16 & 255) << 16 | again(t >> 24) << 24; };
-        const auto  byte  = [&](T v) { return (unsigned) (unsigned char) (bad ? 0 : quantise((float) v, s, inv)); };
+        const auto  four  = [&](T v0, T v1, T v2, T v3) {
+            return bad ? 0u : low_bytes(quantise((float) v0, s, inv), quantise((float) v1, s, inv), quantise((float) v2, s, inv), quantise((float) v3, s, inv));
+        };
 
         if (!VALUES) {
             if (grown) {
@@ -127,10 +150,9 @@ namespace vkhip {
                 const Patch p = patch_of<THREADS>(r, quad0, dv);
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    unsigned o[2] = {0, 0};
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) o[j / 4] |= byte(x[r][k][j]) << (j % 4 * 8);
-                    if (p.token + k >= w.n0 && p.token + k < end) *reinterpret_cast<uint2 *>(page + (p.token + k) * Dp + p.channel) = make_uint2(o[0], o[1]);
+                    const V v = x[r][k];
+                    if (p.token + k >= w.n0 && p.token + k < end)
+                        *reinterpret_cast<uint2 *>(page + (p.token + k) * Dp + p.channel) = make_uint2(four(v[0], v[1], v[2], v[3]), four(v[4], v[5], v[6], v[7]));
                 }
             }
             return;
@@ -142,7 +164,7 @@ namespace vkhip {
             if (p.token >= end) continue;
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-                words[(p.channel + j) * pitch + p.token / 4] = byte(x[r][0][j]) | byte(x[r][1][j]) << 8 | byte(x[r][2][j]) << 16 | byte(x[r][3][j]) << 24;
+                words[(p.channel + j) * pitch + p.token / 4] = four(x[r][0][j], x[r][1][j], x[r][2][j], x[r][3][j]);
         }
         __syncthreads();
         if (w.n == P) { // a whole page: 16 tokens of a channel at a time
@@ -251,17 +273,18 @@ namespace vkhip {
         unsigned char *page   = (values ? a.c.v : a.c.k) + at * P * Dp;
         const float    s0     = w.n0 ? *scale : 0.f;
 
-        V        x {};
-        unsigned big = 0;
+        V      x {};
+        KvPair most = {0, 0};
         for (int i = lane; i < vectors; i += 64) {
-            x = *reinterpret_cast<const V *>(rows + i / dv * stride + i % dv * 8);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) big = max(big, __float_as_uint((float) x[j]) & 0x7FFFFFFFu);
+            x    = *reinterpret_cast<const V *>(rows + i / dv * stride + i % dv * 8);
+            most = magnitude(most, x);
         }
+        unsigned big = max((unsigned) most[0], (unsigned) most[1]);
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) big = max(big, (unsigned) __shfl_xor((int) big, o));
-        const bool  bad = big >= 0x7F800000u || s0 != s0;
-        const float s = bad ? __builtin_nanf("") : fmaxf(s0, __uint_as_float(big) / 127.f), inv = 1.f / s;
+        const float largest = as_float<T>(big);
+        const bool  bad = !(largest < __builtin_inff()) || s0 != s0;
+        const float s = bad ? __builtin_nanf("") : fmaxf(s0, largest / 127.f), inv = 1.f / s;
         if (lane == 0) *scale = s;
         if (!bad && s > s0 && w.n0 > 0) {
             // the page's old tokens; what lies behind them in a word is rewritten below or of no use
@@ -287,8 +310,10 @@ namespace vkhip {
             const int t = w.n0 + i / dv, d = i % dv * 8;
             if (vectors > 64) x = *reinterpret_cast<const V *>(rows + i / dv * stride + d);
             unsigned o[2] = {0, 0};
+            if (!bad)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) o[j / 4] |= (unsigned) (unsigned char) (bad ? 0 : quantise((float) x[j], s, inv)) << (j % 4 * 8);
+                for (int j = 0; j < 2; ++j)
+                    o[j] = low_bytes(quantise((float) x[4 * j], s, inv), quantise((float) x[4 * j + 1], s, inv), quantise((float) x[4 * j + 2], s, inv), quantise((float) x[4 * j + 3], s, inv));
             if (values) {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) page[(d + j) * P + t] = (unsigned char) (o[j / 4] >> (j % 4 * 8));
