@@ -49,8 +49,10 @@ namespace vkhip {
     constexpr int kStep = 64; // tokens a wave takes at a time
 
     // DJ = row / 64 channels, RT tiles of 16 rows, P32: pages of 32 tokens (two to a step), NW waves.
+    // Two row tiles of 64 channels are compiled for two waves a SIMD: 16 x 5000 tokens, 32 rows, 31.7 -> 29.1 us; of 128
+    // channels that costs more than it gives (4 x 40000, 64 rows, 132 -> 160 us), one row tile gains nothing.
     template <typename T, int DJ, int RT, bool P32, int NW>
-    __global__ __launch_bounds__(NW * 64) void kv_attention_kernel(KvAttnArgs a) {
+    __global__ __launch_bounds__(NW * 64, DJ == 1 && RT == 2 ? 2 : 1) void kv_attention_kernel(KvAttnArgs a) {
         constexpr int Dp = DJ * 64, DT = DJ * 4, NL = NW < 4 ? NW : 4; // NL: waves whose products lie in LDS at a time
         __shared__ float wave_m[NW][RT * 16], wave_l[NW][RT * 16];
         __shared__ float acc_lds[NL][16][Dp + 4];
