@@ -7,8 +7,8 @@
 //
 // Bound by memory. What a workgroup can hold in its registers (a group of one image) is read once, in one
 // launch (gn_slab_kernel). Larger groups take two launches, statistics of chunks of pixels and the output, and
-// read x twice: 64 x 256 x 56 x 56 fp16 74 us, the statistics 28 (103 MB at 3.7 TB/s) and the output 41 (206 MB at
-// 5.1 TB/s, a large copy's rate); one launch of slabs takes 102 there, since 16-byte pieces of 512-byte rows cost
+// read x twice: 64 x 256 x 56 x 56 fp16 63 us, the statistics 28 (103 MB at 3.7 TB/s) and the output the rest; one
+// launch of slabs takes 102 there, since 16-byte pieces of 512-byte rows cost
 // whole cache lines. The smallest calls are a launch: 1 x 128 x 40 x 40 6.0 us.
 #include "tokens.h"
 #include <type_traits>
@@ -76,13 +76,19 @@ namespace vkhip {
             for (int j = 0; j < VEC; ++j) t[j] = cv * VEC + j < a.C ? s[j] : (T) 0.f;
             return t;
         }
+        // STREAM: past the caches, for whole lines of a wave's store (from one format to the same; slabs of NC4HW4), so
+        // that x stays for its second read: 64 x 256 x 56 x 56 75 -> 63 us, NC4HW4 16 x 128 x 80 x 80 19.2 -> 14.9, with
+        // the next norm reading y at once 17.0 -> 15.6 (64 x 64 x 112 x 112 59.4 -> 60.8). Pieces of lines lose: to the
+        // other format 30 -> 67 us, the rows of 1 x 128 x 40 x 40 5.6 -> 6.3.
+        template <bool STREAM>
         static __device__ __forceinline__ void store(const GnArgs &a, int n, int p, int cv, const float *v) {
             T *d = (T *) a.y + at(a, a.y_row, n, p, cv);
             if constexpr (NC4 || AL) {
                 V t;
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) t[j] = (T) (!NC4 || cv * VEC + j < a.C ? v[j] : 0.f);
-                *reinterpret_cast<V *>(d) = t;
+                if constexpr (STREAM) __builtin_nontemporal_store(t, reinterpret_cast<V *>(d));
+                else *reinterpret_cast<V *>(d) = t;
             } else {
 #pragma unroll
                 for (int j = 0; j < VEC; ++j)
@@ -247,7 +253,7 @@ namespace vkhip {
                     float v[VEC];
 #pragma unroll
                     for (int j = 0; j < VEC; ++j) v[j] = gn_act<decltype(kind)::value>(a, ((float) x[j] - mean[j]) * mul[j] + add[j]);
-                    GnIo<T, VEC, YN4, YAL>::store(a, n, p0 + p, cv, v);
+                    GnIo<T, VEC, YN4, YAL>::template store<XN4 == YN4>(a, n, p0 + p, cv, v);
                 };
                 int base = 0;
                 for (; base + step <= np; base += step) {
@@ -358,7 +364,7 @@ namespace vkhip {
                 float o[VEC];
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) o[j] = gn_act<decltype(kind)::value>(a, ((float) x[k][j] - mean[j / SHARE]) * mul[j] + be[j]);
-                if (k < mine) GnIo<T, VEC, YN4, YAL>::store(a, n, pl + k * pls, cv, o);
+                if (k < mine) GnIo<T, VEC, YN4, YAL>::template store<XN4 && YN4>(a, n, pl + k * pls, cv, o);
             }
         });
     }
