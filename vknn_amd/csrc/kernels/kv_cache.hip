@@ -2,7 +2,9 @@
 //
 // Bound by memory: 2 bytes in and 1 out a value, and the other way round. A workgroup takes a page, head, and keys or
 // values, so that the largest magnitude is found and used without leaving it; the rows stay in registers
-// between. 8 x 4096 rows, 8 heads, D = 128: 43 us in (201 MB, 4.6 TB/s), 43 us back.
+// between. 8 x 4096 rows, 8 heads, D = 128: 40 us in (201 MB, 5.0 TB/s), 38 us back.
+// Rows in both directions and whole pages pass the caches (44 and 44 us otherwise; pages as they are read back are
+// better left to them: 15 thousand ragged rows 20 us, 23 past them).
 #include "kv_cache.h"
 
 namespace vkhip {
@@ -108,7 +110,7 @@ namespace vkhip {
                 const int t = p.token + k;
 #pragma unroll
                 for (int j = 0; j < 8; ++j) x[r][k][j] = (T) 0.f;
-                if (t >= w.n0 && t < end) x[r][k] = *reinterpret_cast<const V *>(rows + t * stride + p.channel);
+                if (t >= w.n0 && t < end) x[r][k] = __builtin_nontemporal_load(reinterpret_cast<const V *>(rows + t * stride + p.channel));
             }
         }
         const float s0 = w.n0 ? *scale : 0.f;
@@ -152,7 +154,7 @@ namespace vkhip {
                 for (int k = 0; k < 4; ++k) {
                     const V v = x[r][k];
                     if (p.token + k >= w.n0 && p.token + k < end)
-                        *reinterpret_cast<uint2 *>(page + (p.token + k) * Dp + p.channel) = make_uint2(four(v[0], v[1], v[2], v[3]), four(v[4], v[5], v[6], v[7]));
+                        __builtin_nontemporal_store((tk_u32x2) {four(v[0], v[1], v[2], v[3]), four(v[4], v[5], v[6], v[7])}, reinterpret_cast<tk_u32x2 *>(page + (p.token + k) * Dp + p.channel));
                 }
             }
             return;
@@ -171,7 +173,7 @@ namespace vkhip {
             for (int i = tid; i < D * (P / 16); i += THREADS) {
                 const int       d = i / (P / 16), c = i % (P / 16);
                 const unsigned *q = words + d * pitch + c * 4;
-                *reinterpret_cast<uint4 *>(page + d * P + c * 16) = make_uint4(q[0], q[1], q[2], q[3]);
+                __builtin_nontemporal_store((tk_u32x4) {q[0], q[1], q[2], q[3]}, reinterpret_cast<tk_u32x4 *>(page + d * P + c * 16));
             }
             return;
         }
@@ -252,7 +254,7 @@ namespace vkhip {
                 V o;
 #pragma unroll
                 for (int j = 0; j < 8; ++j) o[j] = (T) ((float) (signed char) (q[k][j >> 2] >> (8 * (j & 3))) * s);
-                if (p.token + k >= w.n0 && p.token + k < end) *reinterpret_cast<V *>(rows + (p.token + k) * stride + p.channel) = o;
+                if (p.token + k >= w.n0 && p.token + k < end) __builtin_nontemporal_store(o, reinterpret_cast<V *>(rows + (p.token + k) * stride + p.channel));
             }
         }
     }
