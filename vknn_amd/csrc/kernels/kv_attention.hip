@@ -11,8 +11,8 @@
 // The tokens of a sequence are split over workgroups and a workgroup's four waves; partial results
 // (maximum, sum, product) join in LDS and, across workgroups, in a second kernel.
 //
-// Measured, fp16, 32 heads on 8, D = 128: 8 x 131072 tokens 368 us (5.8 TB/s), 64 x 2048 48 us (5.6), 64 ragged
-// sequences up to 4000 61 us (4.4, the join 5 of it), 8 x 300 6.9 us. Loading the next step's keys and values while this
+// Measured, fp16, 32 heads on 8, D = 128: 8 x 131072 tokens 330 us (6.5 TB/s), 64 x 2048 44 us (6.2), 64 ragged
+// sequences up to 4000 56 us (4.8, the join 5 of it), 8 x 300 6.9 us. Loading the next step's keys and values while this
 // one's are multiplied gained nothing: it costs the registers of a third wave a SIMD, which does the same.
 #include "kv_cache.h"
 
@@ -148,14 +148,16 @@ namespace vkhip {
                     const int r = P32 ? 8 * (nn >> 2) + 4 * (t & 1) + (nn & 3) : 16 * (nn >> 2) + 4 * t + (nn & 3);
                     kr[t][j]    = *reinterpret_cast<const tk_u32x4 *>(kp[P32 ? t >> 1 : 0] + r * Dp + 64 * j + 16 * g);
                 }
+            // Values pass the caches: 8 x 131072 tokens 369 -> 330 us, 64 x 2048 48 -> 44. Keys too: 335 and 44, and four
+            // workgroups that share a cache (64 rows of 128 channels, 4 x 40000) 130 -> 157 us instead of 134.
 #pragma unroll
             for (int d = 0; d < DT; ++d) {
                 if constexpr (P32) {
-                    const tk_u32x2 x = *reinterpret_cast<const tk_u32x2 *>(vp[0] + (int64_t) (16 * d + nn) * P + 8 * g);
-                    const tk_u32x2 y = *reinterpret_cast<const tk_u32x2 *>(vp[1] + (int64_t) (16 * d + nn) * P + 8 * g);
+                    const tk_u32x2 x = __builtin_nontemporal_load(reinterpret_cast<const tk_u32x2 *>(vp[0] + (int64_t) (16 * d + nn) * P + 8 * g));
+                    const tk_u32x2 y = __builtin_nontemporal_load(reinterpret_cast<const tk_u32x2 *>(vp[1] + (int64_t) (16 * d + nn) * P + 8 * g));
                     vr[d]            = tk_u32x4 {x[0], x[1], y[0], y[1]};
                 } else {
-                    vr[d] = *reinterpret_cast<const tk_u32x4 *>(vp[0] + (int64_t) (16 * d + nn) * P + 16 * g);
+                    vr[d] = __builtin_nontemporal_load(reinterpret_cast<const tk_u32x4 *>(vp[0] + (int64_t) (16 * d + nn) * P + 16 * g));
                 }
             }
             float4v s[RT][4];
