@@ -369,9 +369,13 @@ namespace vkhip {
         const int64_t most = (int64_t) c->max_blocks * c->page_tokens;
         a.max_len  = (int) (d->max_len > 0 && d->max_len < most ? d->max_len : most);
         const int64_t len = a.max_len > 0 ? a.max_len : 1, base = (int64_t) c->batch * c->kv_heads * a.blocks;
-        // Waves of a workgroup: two where no sequence has more steps, eight and no split where one workgroup takes a short
-        // sequence in one round and there are few of them (a second launch costs about 3 us), four otherwise.
-        const bool few = base <= 256 && len <= 8 * kStep && row_tiles(a.rows) == 1;
+        // Waves of a workgroup: two where no sequence has more steps, eight and no split where one workgroup takes a
+        // sequence in few rounds (a second launch costs about 3 us), four otherwise. How many are few: one, as a round is
+        // 128 KB for a compute unit alone, two of 64 channels, and more where the workgroups nearly fill the card. Split /
+        // not, 128 and 64 channels: 1 x 1000 tokens 8.1 / 9.9, 7.4 / 6.9 us; 8 x 700 9.2 / 10.4, 8.3 / 7.0; 16 x 1500
+        // 15.3 / 16.1 (three rounds), 12.6 / 11.7; 32 x 1500 22.2 / 19.8, 16.0 / 12.8.
+        const int64_t once = (c->head_dim <= 64 ? 2 : 1) + base / 128;
+        const bool    few  = base <= 256 && len <= once * 8 * kStep && row_tiles(a.rows) == 1;
         a.waves        = len <= 2 * kStep ? 2 : (few ? 8 : 4);
         // Splits: two workgroups a compute unit, which all run at once; where that leaves more than 8 rounds to one,
         // which would wait for the longest sequence, spans of 8 rounds or 2048 workgroups. In between, workgroups that
