@@ -13,7 +13,7 @@
 // (fp16) or 2^-8 (bf16) of each term, where the output itself is rounded by as much. Their sum stays fp32.
 //
 // Bound by the matrix and vector units together, and by power: 16384 causal queries, 32 heads on 8, D = 128, fp16
-// 2.1 ms (1048 TFLOP/s; a 16384^3 library product 1246), the clock at 1.6 GHz, matrix units busy 62% of it, vector
+// 2.06 to 2.17 ms by the card's clock (1067 to 1014 TFLOP/s; a 16384^3 library product 1246), 1.6 to 1.5 GHz, matrix units busy 62% of it, vector
 // units 51%, no bank conflicts. 4 x 4096 not causal 1027, D = 64 bf16 952 TFLOP/s. 200 queries behind 50000 keys 96 us.
 // Two workgroups a compute unit (LDS 72 KB, up to 256 registers) overlap one's exponentials with the other's
 // products; raising a wave's priority around its products or loading V's first fragments earlier changed nothing.

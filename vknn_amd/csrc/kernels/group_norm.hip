@@ -7,8 +7,8 @@
 //
 // Bound by memory. What a workgroup can hold in its registers (a group of one image) is read once, in one
 // launch (gn_slab_kernel). Larger groups take two launches, statistics of chunks of pixels and the output, and
-// read x twice: 64 x 256 x 56 x 56 fp16 63 us, the statistics 28 (103 MB at 3.7 TB/s) and the output the rest; one
-// launch of slabs takes 102 there, since 16-byte pieces of 512-byte rows cost
+// read x twice: 64 x 256 x 56 x 56 fp16 62 us, the statistics 22 (103 MB at 4.6 TB/s) and the output 39 (206 MB
+// at 5.3 TB/s, a large copy's rate); one launch of slabs takes 112 there, since 16-byte pieces of 512-byte rows cost
 // whole cache lines. The smallest calls are a launch: 1 x 128 x 40 x 40 6.0 us.
 #include "tokens.h"
 #include <type_traits>
@@ -373,12 +373,12 @@ namespace vkhip {
     struct GnSlab {
         int vectors, groups, threads, pixels; // SV, GV, and a thread's pixels
     };
-    // Where a slab fits, it is taken from NC4HW4 always (its planes are contiguous; 8 x 108 x 75 x 75 to rows 12.1 us
-    // against 18.3 with two launches, 16 x 128 x 80 x 80 19.5 against 23.4), and from NHWC by the two sides' times as
+    // Where a slab fits, it is taken from NC4HW4 always (its planes are contiguous; 8 x 108 x 75 x 75 to rows 12.2 us
+    // against 18.2 with two launches, 16 x 128 x 80 x 80 15.1 against 21.3), and from NHWC by the two sides' times as
     // measured, in us: 4 and 1 + 3 / SV ns a vector and compute unit (a row's piece of SV vectors costs whole cache
     // lines), against 11.5 and three passes over the tensor at 5.5 TB/s. Measured slab / two launches:
-    // 1 x 128 x 40 x 40 5.7 / 13.0, 8 x 512 x 28 x 28 6.8 / 15.0, 64 x 256 x 28 x 28 23.8 / 27.4,
-    // 1 x 64 x 80 x 80 20.9 / 14.9, 64 x 256 x 56 x 56 101.6 / 75.1.
+    // 1 x 128 x 40 x 40 5.7 / 12.8, 8 x 512 x 28 x 28 6.9 / 14.6, 64 x 256 x 28 x 28 23.8 / 24.6,
+    // 1 x 64 x 80 x 80 20.8 / 11.5, 64 x 256 x 56 x 56 112 / 62.
     static GnSlab gn_slab(const GnArgs &a, int vec, int size, bool planes) {
         if (a.Cg % vec && vec % a.Cg) return {0, 0, 0, 0};
         const int    sv      = a.Cg < vec ? 1 : a.Cg / vec;

@@ -379,8 +379,9 @@ namespace vkhip {
         a.waves        = len <= 2 * kStep ? 2 : (few ? 8 : 4);
         // Splits: two workgroups a compute unit, which all run at once; where that leaves more than 8 rounds to one,
         // which would wait for the longest sequence, spans of 8 rounds or 2048 workgroups. In between, workgroups that
-        // nearly all run at once leave some for a second turn (8 x 131072 tokens: 362 us with 512, 404 with 1024, 370
-        // with 2048; 64 ragged sequences up to 4000: 71 us unsplit, 61 in two).
+        // nearly all run at once leave some for a second turn (before values passed the caches 8 x 131072 tokens 362 us
+        // with 512, 404 with 1024, 370 with 2048; 64 ragged sequences up to 4000 71 us unsplit, 61 in two; since then 64 x
+        // 2048 44 us, 53 with spans of four rounds).
         const int64_t rounds = ceil_div(len, a.waves * kStep);
         int64_t       splits = few || base >= 512 || base == 0 ? 1 : 512 / base;
         if (base > 0 && rounds > 8 * splits) {
