@@ -476,7 +476,8 @@ int    vkhip_group_norm(const vkhip_group_norm_desc *d, const void *x, const flo
  * clamped to it). Head h of q_heads reads key/value head h / (q_heads / kv_heads).
  *   o = sum_j softmax_j(scale * q . k_j) v_j over every key of the sequence or, with causal, over the keys
  *   j <= i + nk - nq for query i of nq (the last query sees the last key).
- * A query that sees no key gives zeros. What a query does not see never reaches it, NaN and
+ * A query that sees no key gives zeros; query rows in front of cu_q[0] and from cu_q[batch] on belong to no
+ * sequence, and theirs of o are not written. What a query does not see never reaches it, NaN and
  * infinities included. Weights are rounded to the 16-bit type before they multiply v, their sum is not.
  * F16 or BF16; head_dim a multiple of 8 up to 128; scale > 0; every row of every head starts on a
  * 16-byte boundary; k_row and v_row head_dim .. 2^23. o must not overlap q, k or v. workspace:

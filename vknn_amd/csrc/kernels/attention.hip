@@ -358,12 +358,14 @@ namespace vkhip {
 #endif
     }
 
-    // Joins the splits of a query and head: a wave each, two channels a lane.
+    // Joins the splits of a query and head: a wave each, two channels a lane. Queries in front of the first sequence or
+    // behind the last have no partial results, and their rows of o are not this call's.
     template <typename T>
     __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
         const int64_t rows = (int64_t) a.total_q * a.q_heads, at = (int64_t) blockIdx.x * 4 + (threadIdx.x >> 6);
         if (at >= rows) return;
-        const int lane = threadIdx.x & 63, D = a.head_dim, d = lane * 2;
+        const int lane = threadIdx.x & 63, D = a.head_dim, d = lane * 2, q = (int) (at / a.q_heads);
+        if (q < a.cu_q[0] || q >= a.cu_q[a.batch]) return;
         float     top = -__builtin_inff(), sum = 0.f, x0 = 0.f, x1 = 0.f;
         for (int k = 0; k < a.splits; ++k) top = fmaxf(top, a.part_s[(k * rows + at) * 2]);
         const float base = top == -__builtin_inff() ? 0.f : top;
@@ -379,7 +381,7 @@ namespace vkhip {
         }
         const float inv = sum == 0.f ? 0.f : 1.f / sum;
         if (d >= D) return;
-        T *o = (T *) a.o + at / a.q_heads * a.o_row + at % a.q_heads * a.o_head + d;
+        T *o = (T *) a.o + q * a.o_row + at % a.q_heads * a.o_head + d;
         o[0] = (T) (x0 * inv), o[1] = (T) (x1 * inv);
     }
 
