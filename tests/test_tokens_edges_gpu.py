@@ -42,3 +42,72 @@ def test_attention_rows_outside_every_sequence(gpu, nq, nk, split, causal):
     outside[front:front + sum(nq)] = False
     assert torch.equal(got[outside], was[outside])
     T.check_attention(got[~outside].double(), q, k, v, nq, nk, causal, "f16", d ** -0.5)
+
+
+# Weights far below a row's largest: fp16 holds them as multiples of 2^-24 (off by 2^-25 at most) of a reference. Where
+# they are raised so that the largest is 2^up or more, that is 2^-(25 + up) of the largest.
+def check_long_tail(out, q, k, v, scale, dtype, up):
+    """All heads of one sequence on one key/value head, last query last; out, q [n, heads, d], k, v [m, d] float64."""
+    n, m = q.shape[0], k.shape[0]
+    see = torch.arange(m)[None] <= torch.arange(n)[:, None] + m - n
+    u = T.DT[dtype][2]
+    for h in range(q.shape[1]):
+        want, pv, qk = T.attention64(q[:, h], k, v, see, scale)
+        e = (q.shape[2] + 16) * 2.0 ** -24 * qk + 2.0 ** -20 + (0.0 if dtype == "f16" else q.shape[2] * 2.0 ** -25) * qk
+        bound = u * want.abs() * 1.01 + T.TINY[dtype] + (2.0 ** -11 * 1.02 + 2 * e) * pv + m * 2.0 ** -(25 + up) * v.abs().amax(0, keepdim=True)
+        worst = ((out[:, h] - want).abs() / bound).max().item()
+        assert worst <= 1, (worst, h)
+
+
+def long_tail_cache(n, page, d, at):
+    """One sequence whose token `at` has a key that all the others are 2^25 or so below, and a value of zero."""
+    c = T.Cache(1, -(-n // page), page, 1, d, seed=n)
+    g = torch.Generator().manual_seed(n)
+    k = torch.zeros(c.k.shape, dtype=torch.int8)
+    v = torch.zeros(c.v.shape, dtype=torch.int8)
+    ids = c.table[0].long()
+    rows = torch.randint(-1, 2, (len(ids), page, d), generator=g, dtype=torch.int8)
+    rows[at // page, at % page] = 127
+    k[ids, 0, :, :d] = rows
+    vals = torch.randint(60, 128, (len(ids), d, page), generator=g, dtype=torch.int8)
+    vals[at // page, :, at % page] = 0
+    v[ids, 0, :d] = vals
+    c.k.put(k)
+    c.v.put(v)
+    c.ks.put(torch.full(c.ks.shape, 0.01))
+    c.vs.put(torch.full(c.vs.shape, 0.02))
+    return c
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("n,page,d,hq,t,at", [(150001, 64, 128, 4, 1, 0), (20000, 32, 64, 2, 1, 19000), (40000, 64, 64, 8, 3, 0), (70000, 128, 96, 20, 1, 69999), (500, 64, 128, 1, 1, 3)])
+def test_kv_attention_long_tail(gpu, n, page, d, hq, t, at, dtype):
+    """A key that owns a row, and a hundred thousand small weights that are the whole of the output."""
+    c = long_tail_cache(n, page, d, at)
+    q = (1 + 0.01 * T.rand(n, 1, t, hq, d)).to(T.DT[dtype][0]).float()
+    scale = 25.2 / 1.44269504 / (127 * 0.01 * d)
+    out = T.kv_attention(V.vkhip(), c, q, [n], dtype, scale)
+    (kq, ks), (vq, vs) = c.bytes_of(0, n)
+    check_long_tail(out[0], q[0].double(), (kq.double() * ks.double()[:, :, None])[:, 0], (vq.double() * vs.double()[:, :, None])[:, 0], scale, dtype, 14)
+
+
+@pytest.mark.parametrize("size", [2.0 ** 20, 2.0 ** 23, 2.0 ** 25, 2.0 ** 26, 2.0 ** 27, 2.0 ** 28, 2.0 ** 40, 2.0 ** 60])
+def test_kv_attention_huge_scores(gpu, size):
+    """Scores whose last places are whole powers of two or more: the row is its largest key's, or two equal ones'."""
+    d, n, page = 64, 200, 64
+    for keys in ([57], [0], [199], [3, 150], [64, 65]):
+        c = T.Cache(1, 4, page, 1, d, seed=1)
+        k, v = torch.zeros(c.k.shape, dtype=torch.int8), torch.randint(-127, 128, c.v.shape, generator=torch.Generator().manual_seed(5), dtype=torch.int8)
+        ids = c.table[0].long()
+        k[ids, 0, :, 0] = 100
+        for i in keys:
+            k[ids[i // page], 0, i % page, 0] = 101
+        c.k.put(k)
+        c.v.put(v)
+        c.ks.put(torch.full(c.ks.shape, size))
+        c.vs.put(torch.ones(c.vs.shape))
+        q = torch.zeros(1, 1, 2, d)
+        q[..., 0] = 1
+        out = T.kv_attention(V.vkhip(), c, q, [n], "f16", 1.0)
+        rows = torch.stack([v[ids[i // page], 0, :, i % page].double() for i in keys])
+        assert torch.equal(out[0, 0], rows.mean(0).expand(2, d)), (size, keys)

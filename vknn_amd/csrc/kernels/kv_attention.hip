@@ -7,9 +7,11 @@
 // contraction slot is free as long as both operands agree, so K's rows are taken in the order that leaves each
 // lane with the tokens whose values its V load brings (16 tokens of one channel, side by side in the page).
 // int8 becomes fp16 exactly; a page's key scale multiplies its scores, its value scale the fp32 product of the
-// page, so weights are rounded to fp16 unscaled (at most 1, the largest of a row exactly 1).
+// page. Weights are rounded to fp16, whose smallest step is 2^-24: a row's reference is 14 below its largest exponent,
+// so that its largest weight is 2^14 and what is lost lies under 2^-39 of it (a row of many small weights beside one
+// large one keeps them), and values come as multiples of 2^-14 in return, at no cost.
 // The tokens of a sequence are split over workgroups and a workgroup's four waves; partial results
-// (maximum, sum, product) join in LDS and, across workgroups, in a second kernel.
+// (reference, sum, product) join in LDS and, across workgroups, in a second kernel.
 //
 // Measured, fp16, 32 heads on 8, D = 128: 8 x 131072 tokens 330 us (6.5 TB/s), 64 x 2048 44 us (6.2), 64 ragged
 // sequences up to 4000 56 us (4.8, the join 5 of it), 8 x 300 6.9 us. Loading the next step's keys and values while this
@@ -23,7 +25,7 @@ namespace vkhip {
         const void    *q;
         void          *o;
         const int32_t *lens;
-        float         *part_o, *part_s; // [batch][head][row][split]: products [head_dim]; (maximum, sum)
+        float         *part_o, *part_s; // [batch][head][row][split]: products [head_dim]; (reference, sum)
         float          scale;
         int            group, rows, q_tokens; // query heads per kv head; rows = group * q_tokens
         int            blocks;                // blocks of 16 * RT rows
@@ -32,17 +34,24 @@ namespace vkhip {
         int64_t        q_row, q_head, o_row, o_head;
     };
 
-    // 4 int8 (as bits) -> 4 fp16, exactly: the byte with its sign flipped is the low byte of 1024 + (b + 128).
+    constexpr int kWeightBits = 14; // weights are up to 2^14, values b 2^-14
+
+    // 4 int8 (as bits) -> 4 fp16 b 2^-DOWN, exactly: the byte with its sign flipped is the low byte of
+    // (1024 + (b + 128)) 2^-DOWN, whose high byte is 0x64 less 4 for each power of two.
+    template <int DOWN>
     __device__ __forceinline__ void i8_to_h4(unsigned b, half2v &lo, half2v &hi) {
         b ^= 0x80808080u;
-        const half2v off = {(half_t) 1152.f, (half_t) 1152.f};
-        lo = __builtin_bit_cast(half2v, __builtin_amdgcn_perm(0x64646464u, b, 0x04010400u)) - off;
-        hi = __builtin_bit_cast(half2v, __builtin_amdgcn_perm(0x64646464u, b, 0x04030402u)) - off;
+        constexpr unsigned high = (0x64u - 4 * DOWN) * 0x01010101u;
+        constexpr float    zero = 1152.f / (1 << DOWN);
+        const half2v       off  = {(half_t) zero, (half_t) zero};
+        lo = __builtin_bit_cast(half2v, __builtin_amdgcn_perm(high, b, 0x04010400u)) - off;
+        hi = __builtin_bit_cast(half2v, __builtin_amdgcn_perm(high, b, 0x04030402u)) - off;
     }
+    template <int DOWN>
     __device__ __forceinline__ half8 i8_to_h8(unsigned a, unsigned b) {
         half2v x, y, z, w;
-        i8_to_h4(a, x, y);
-        i8_to_h4(b, z, w);
+        i8_to_h4<DOWN>(a, x, y);
+        i8_to_h4<DOWN>(b, z, w);
         return half8 {x[0], x[1], y[0], y[1], z[0], z[1], w[0], w[1]};
     }
 
@@ -113,7 +122,7 @@ namespace vkhip {
         }
 
         float4v acc[RT][DT];
-        float   m[RT], l[RT];
+        float   m[RT], l[RT]; // reference of the exponents, sum of the weights
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
             m[rt] = -__builtin_inff(), l[rt] = 0.f;
@@ -169,7 +178,7 @@ namespace vkhip {
                 for (int j = 0; j < DJ; ++j)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        const half8 kf = i8_to_h8(kr[t][j][2 * e], kr[t][j][2 * e + 1]);
+                        const half8 kf = i8_to_h8<0>(kr[t][j][2 * e], kr[t][j][2 * e + 1]);
 #pragma unroll
                         for (int rt = 0; rt < RT; ++rt) s[rt][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[rt][j][e], s[rt][t], 0, 0, 0);
                     }
@@ -193,7 +202,9 @@ namespace vkhip {
                 }
                 top               = fmaxf(top, __shfl_xor(top, 16));
                 top               = fmaxf(top, __shfl_xor(top, 32));
-                const float to    = fmaxf(m[rt], top), base = to == -__builtin_inff() ? 0.f : to;
+                float up          = top - kWeightBits;
+                if (top - up > 15.f) up = top; // exponents from 2^25 on, 4 or more apart: not rounded to where 2^16 would be a weight
+                const float to    = fmaxf(m[rt], up), base = to == -__builtin_inff() ? 0.f : to;
                 alpha[rt]         = exp2_hw(m[rt] - base);
                 m[rt]             = to;
                 float sum         = 0.f;
@@ -209,7 +220,7 @@ namespace vkhip {
             }
 #pragma unroll
             for (int d = 0; d < DT; ++d) {
-                const half8   v0 = i8_to_h8(vr[d][0], vr[d][1]), v1 = i8_to_h8(vr[d][2], vr[d][3]);
+                const half8   v0 = i8_to_h8<kWeightBits>(vr[d][0], vr[d][1]), v1 = i8_to_h8<kWeightBits>(vr[d][2], vr[d][3]);
                 const float4v zero = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt) {
@@ -235,6 +246,7 @@ namespace vkhip {
         for (int rt = 0; rt < RT; ++rt) {
             l[rt] += __shfl_xor(l[rt], 16);
             l[rt] += __shfl_xor(l[rt], 32);
+            l[rt] *= 1.f / (1 << kWeightBits); // the products have it in their values
             if (g == 0) wave_m[wave][rt * 16 + nn] = m[rt], wave_l[wave][rt * 16 + nn] = l[rt];
         }
         __syncthreads();
