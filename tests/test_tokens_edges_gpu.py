@@ -111,3 +111,21 @@ def test_kv_attention_huge_scores(gpu, size):
         out = T.kv_attention(V.vkhip(), c, q, [n], "f16", 1.0)
         rows = torch.stack([v[ids[i // page], 0, :, i % page].double() for i in keys])
         assert torch.equal(out[0, 0], rows.mean(0).expand(2, d)), (size, keys)
+
+
+@pytest.mark.parametrize("nq,nk,hq,at,causal", [(1, 40000, 2, 0, 1), (130, 20000, 1, 0, 1), (3, 300, 300, 7, 0), (70, 9000, 520, 0, 0), (257, 3001, 1, 2990, 1)])
+def test_attention_long_tail(gpu, nq, nk, hq, at, causal):
+    """fp16 rows where one key of value zero owns each row and the small weights are the whole of the output; with the
+    keys split and not."""
+    d, heads = 64, min(hq, 3)
+    q = (1 + 0.01 * T.rand(nk, nq, 1, d)).half().float().expand(nq, hq, d)
+    k, v = (0.005 * T.rand(nk + 1, nk, d)).half().float(), (1 + 0.2 * T.rand(nk + 2, nk, d)).half().float()
+    k[at], v[at] = 1, 0
+    scale = 25.2 / 1.44269504 / d
+    out = T.attention(V.vkhip(), q, k[:, None], v[:, None], [nq], [nk], causal, "f16", scale)
+    assert torch.equal(out, out[:, :1].expand_as(out))
+    if causal:
+        check_long_tail(out[:, :heads], q[:, :heads].double(), k.double(), v.double(), scale, "f16", 7)
+    else:  # every query sees every key, as if each were the last
+        for i in range(0, nq, 23):
+            check_long_tail(out[i:i + 1, :heads], q[i:i + 1, :heads].double(), k.double(), v.double(), scale, "f16", 7)

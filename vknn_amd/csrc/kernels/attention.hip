@@ -10,7 +10,8 @@
 // with their 16-byte pieces permuted (xor with the row) so that neither read pattern meets a bank twice.
 //
 // The weights are rounded to the type of V, since both operands of a product have one type: an error of 2^-11
-// (fp16) or 2^-8 (bf16) of each term, where the output itself is rounded by as much. Their sum stays fp32.
+// (fp16) or 2^-8 (bf16) of each term, where the output itself is rounded by as much. Their sum stays fp32. fp16
+// weights are raised by 2^7 to 2^15, so that many small ones beside a large one are not lost.
 //
 // Bound by the matrix and vector units together, and by power: 16384 causal queries, 32 heads on 8, D = 128, fp16
 // 2.06 to 2.17 ms by the card's clock (1067 to 1014 TFLOP/s; a 16384^3 library product 1246), 1.6 to 1.5 GHz, matrix units busy 62% of it, vector
@@ -40,6 +41,9 @@ namespace vkhip {
         typedef half8 V8;
         typedef half4 V4;
         static constexpr unsigned kExp = 0x7C00u; // bits of infinity
+        // The exponents' reference lies this far below a maximum when it is set, and up to 8 further as the maximum grows:
+        // fp16 weights from 2^7 up to 2^15 for the largest, whose smallest step, 2^-24, is then 2^-31 of it or less.
+        static constexpr float kUp = 7.f;
         static __device__ __forceinline__ float16v mfma(V8 a, V8 b, float16v c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
     };
     template <>
@@ -47,6 +51,7 @@ namespace vkhip {
         typedef bf8 V8;
         typedef bf4 V4;
         static constexpr unsigned kExp = 0x7F80u;
+        static constexpr float    kUp  = 0.f; // fp32's range
         static __device__ __forceinline__ float16v mfma(V8 a, V8 b, float16v c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
     };
 
@@ -182,8 +187,8 @@ namespace vkhip {
             for (int r = 0; r < 16; ++r) acc[d][r] = 0.f;
         // sign bits of the two values whose exponent is all ones: a carry goes there
         const auto not_finite = [](unsigned two) { return ((two & (A::kExp * 0x10001u)) + (0x8000u - A::kExp) * 0x10001u) & 0x80008000u; };
-        // the reference of the exponents, at most 8 below the largest one seen: weights up to 2^8 cost no digits, and
-        // O is rescaled only where a maximum grows by more than that
+        // the reference of the exponents, kUp to kUp + 8 below the largest one seen: weights up to 2^8 times as large cost
+        // no digits, and O is rescaled only where a maximum grows by more than that
         float m = -__builtin_inff(), l = 0.f;
 
         // A weight of zero does not keep a NaN or an infinity of V out of a product. Where something is masked, each wave
@@ -215,8 +220,8 @@ namespace vkhip {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) top = fmaxf(top, s[kk][r]);
             top = max_halves(top) * a.c2;
-            if (__any(top > m + 8.f)) {
-                const float to    = fmaxf(m, top);
+            if (__any(top - m > 8.f + A::kUp)) {
+                const float to    = fmaxf(m, top - A::kUp);
                 const float alpha = exp2_hw(m - (to == -__builtin_inff() ? 0.f : to));
                 l *= alpha;
 #pragma unroll
