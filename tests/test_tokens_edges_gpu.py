@@ -129,3 +129,25 @@ def test_attention_long_tail(gpu, nq, nk, hq, at, causal):
     else:  # every query sees every key, as if each were the last
         for i in range(0, nq, 23):
             check_long_tail(out[i:i + 1, :heads], q[i:i + 1, :heads].double(), k.double(), v.double(), scale, "f16", 7)
+
+
+@pytest.mark.parametrize("dtype,size", [("f16", 2.0 ** 12), ("f16", 2.0 ** 13), ("f16", 2.0 ** 14), ("f16", 2.0 ** 15), ("bf16", 2.0 ** 14), ("bf16", 2.0 ** 20), ("bf16", 2.0 ** 40)])
+@pytest.mark.parametrize("nk", [64, 150, 2304])
+def test_attention_huge_scores(gpu, dtype, size, nk):
+    """Scores of 2^30 to 2^86, whose neighbours in fp32 are whole numbers apart: a row is its largest key's value, or the
+    mean of two equal ones' (exact but for the output's rounding and the weights': equal weights, rounded alike, over
+    their unrounded sum)."""
+    d, nq = 64, 130
+    u = T.DT[dtype][2]
+    for keys in ([nk // 2], [0], [nk - 1], [1, nk - 2]):
+        q = torch.full((nq, 1, d), size)
+        k = torch.full((nk, 1, d), size * 0.75)
+        k -= size * 2.0 ** -6 * (torch.arange(nk) % 5)[:, None, None]
+        k[keys] = size
+        v = T.rand(nk, nk, 1, d).to(T.DT[dtype][0]).float()
+        for causal in (False, True):
+            out = T.attention(V.vkhip(), q, k, v, [nq], [nk], causal, dtype, 1.0)
+            # queries that see all of `keys`
+            seen = out[max(0, nq - nk + max(keys)):] if causal else out
+            want = v[keys].double().mean(0)
+            assert ((seen - want).abs() <= 1.01 * u * want.abs() + 1.02 * u * v[keys].double().abs().mean(0) + T.TINY[dtype]).all(), (keys, causal)

@@ -190,6 +190,7 @@ namespace vkhip {
         // the reference of the exponents, kUp to kUp + 8 below the largest one seen: weights up to 2^8 times as large cost
         // no digits, and O is rescaled only where a maximum grows by more than that
         float m = -__builtin_inff(), l = 0.f;
+        bool  far = false; // a reference of the wave is 2^20 or more, either way
 
         // A weight of zero does not keep a NaN or an infinity of V out of a product. Where something is masked, each wave
         // looks through the piece of V that it copied and clears what it finds (`spoiled`: something was); what the
@@ -228,17 +229,28 @@ namespace vkhip {
                 for (int d = 0; d < DB; ++d)
 #pragma unroll
                     for (int r = 0; r < 16; ++r) acc[d][r] *= alpha;
-                m = to;
+                m   = to;
+                far = __any(fabsf(m) >= 0x1p20f && m > -__builtin_inff());
             }
-            const float base = m == -__builtin_inff() ? 0.f : m;
-            V8          pf[4];
+            float base = m == -__builtin_inff() ? 0.f : m, mul = a.c2;
+            if (far) {
+                // fp32 is 1/8 or coarser there: the products are rounded as the maximum's was, which one rounding of
+                // product and difference together would miss by up to half a step, any power of two
+#pragma clang fp contract(off)
+#pragma unroll
+                for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s[kk][r] = s[kk][r] * a.c2 - base;
+                mul = 1.f, base = 0.f;
+            }
+            V8 pf[4];
 #pragma unroll
             for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
                 for (int r = 0; r < 16; r += 2) {
                     typedef float F2 __attribute__((ext_vector_type(2)));
                     typedef T     T2 __attribute__((ext_vector_type(2)));
-                    const F2      p = {exp2_hw(__builtin_fmaf(s[kk][r], a.c2, -base)), exp2_hw(__builtin_fmaf(s[kk][r + 1], a.c2, -base))};
+                    const F2      p = {exp2_hw(__builtin_fmaf(s[kk][r], mul, -base)), exp2_hw(__builtin_fmaf(s[kk][r + 1], mul, -base))};
                     l += p[0];
                     l += p[1];
                     const T2 x = __builtin_convertvector(p, T2);
