@@ -151,3 +151,14 @@ def test_attention_huge_scores(gpu, dtype, size, nk):
             seen = out[max(0, nq - nk + max(keys)):] if causal else out
             want = v[keys].double().mean(0)
             assert ((seen - want).abs() <= 1.01 * u * want.abs() + 1.02 * u * v[keys].double().abs().mean(0) + T.TINY[dtype]).all(), (keys, causal)
+
+
+@pytest.mark.parametrize("c,groups,p", [(20, 4, 301), (64, 2, 6400), (7, 1, 900), (24, 1, 40000)])
+def test_group_norm_far_out(gpu, c, groups, p):
+    """Means whose square leaves fp32: the variance is about the mean, so the norm of such rows is in range."""
+    x = T.rand(p, 2, p, c) * 1e16 + 3e19
+    T.check_gn(T.group_norm(V.vkhip(), x, groups, None, None, "f32"), x, groups, None, None, "f32", 0)
+    x = torch.full((1, p, c), -1.0 * 2 ** 66)
+    x[:, :, : c // groups] = 2.0 ** 70
+    y = T.group_norm(V.vkhip(), x, groups, None, None, "bf16")
+    T.check_gn(y, x, groups, None, None, "bf16", 0)

@@ -3,7 +3,8 @@
 // The mean and variance of a group are joined from parts (Chan's update): each thread forms the exact mean
 // and the squared deviations M2 of a few loaded values, and parts (n, mean, M2) merge as
 //   d = mean_b - mean_a,  mean = mean_a + d n_b / n,  M2 = M2_a + M2_b + d^2 n_a n_b / n
-// so a mean far from zero costs no digits of the variance, as the difference of two sums would.
+// so a mean far from zero costs no digits of the variance, as the difference of two sums would. d n_a n_b / n is
+// formed before its product with d: 0 for a first part, whose d is the whole mean and whose square may leave fp32.
 //
 // Bound by memory. What a workgroup can hold in its registers (a group of one image) is read once, in one
 // launch (gn_slab_kernel). Larger groups take two launches, statistics of chunks of pixels and the output, and
@@ -49,7 +50,7 @@ namespace vkhip {
         const float n = a.n + b.n;
         if (n == 0.f) return a;
         const float r = b.n * __builtin_amdgcn_rcpf(n), d = b.mean - a.mean; // 1 ulp of the share: 1e-7 of a part's weight
-        return {n, a.mean + d * r, a.m2 + b.m2 + d * d * a.n * r};
+        return {n, a.mean + d * r, a.m2 + b.m2 + d * (d * (a.n * r))};
     }
 
     // `lanes` (a power of two up to 64) neighbouring lanes each hold moments: merged in all of them.
@@ -139,7 +140,7 @@ namespace vkhip {
                 for (int u = 0; u < kGnBatch; ++u) q = __builtin_fmaf((float) v[u][j] - s, (float) v[u][j] - s, q);
                 const float d = s - mean[j];
                 mean[j]       = __builtin_fmaf(d, share, mean[j]);
-                m2[j] += __builtin_fmaf(d * d, cross, q);
+                m2[j] += __builtin_fmaf(d, d * cross, q);
             }
             count += kGnBatch;
         }
@@ -160,7 +161,7 @@ namespace vkhip {
             for (int u = 0; u < kGnBatch; ++u) q += u < left ? ((float) v[u][j] - s) * ((float) v[u][j] - s) : 0.f;
             const float d = s - mean[j];
             mean[j]       = __builtin_fmaf(d, share, mean[j]);
-            m2[j] += __builtin_fmaf(d * d, cross, q);
+            m2[j] += __builtin_fmaf(d, d * cross, q);
         }
     }
     __device__ __forceinline__ float gn_thread_count(int np, int pl, int pls) { return pl < np ? (float) ((np - pl + pls - 1) / pls) : 0.f; }
