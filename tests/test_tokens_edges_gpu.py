@@ -162,3 +162,13 @@ def test_group_norm_far_out(gpu, c, groups, p):
     x[:, :, : c // groups] = 2.0 ** 70
     y = T.group_norm(V.vkhip(), x, groups, None, None, "bf16")
     T.check_gn(y, x, groups, None, None, "bf16", 0)
+
+
+def test_group_norm_many_workgroups(gpu):
+    """More groups of images than a launch has work items in one dimension (65535 x 257 workgroups of 256 threads)."""
+    n, c, groups = 65535, 1028, 257
+    some = T.rand(1, 51, 1, c).half().float()
+    x = some.repeat(1285, 1, 1)
+    y = T.group_norm(V.vkhip(), x, groups, None, None, "f16", 2, 2)
+    T.check_gn(y[:51], some, groups, None, None, "f16", 0)
+    assert torch.equal(y, y[:51].repeat(1285, 1, 1))

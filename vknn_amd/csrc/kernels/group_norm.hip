@@ -313,12 +313,12 @@ namespace vkhip {
     // were slower (64 x 256 x 28 x 28: 34 us with four groups, 24 with one): one workgroup a compute unit has nothing
     // to read while it writes.
     template <typename T, int VEC, bool XN4, bool YN4, bool XAL, bool YAL, int THREADS, int R, int GV>
-    __global__ __launch_bounds__(THREADS) void gn_slab_kernel(GnArgs a, int SV, int slabs, int spread) {
+    __global__ __launch_bounds__(THREADS) void gn_slab_kernel(GnArgs a, int SV, int spread) {
         using X             = GnIo<T, VEC, XN4, XAL>;
         constexpr int SHARE = VEC / GV; // channels of a vector in one group
         __shared__ float red[2][THREADS / 64][GV];
         // images over the XCDs, the slabs of one on the same: their pieces of a cache line meet in its L2
-        const int n = blockIdx.x / (slabs * spread) * spread + blockIdx.x % spread, slab = blockIdx.x / spread % slabs;
+        const int n = blockIdx.y * spread + blockIdx.x % spread, slab = blockIdx.x / spread;
         if (n >= a.N) return;
         const int pls = THREADS / SV, v = XN4 ? threadIdx.x / pls : threadIdx.x % SV, pl = XN4 ? threadIdx.x % pls : threadIdx.x / SV;
         const int cv = slab * SV + v;
@@ -395,10 +395,10 @@ namespace vkhip {
     template <typename T, int VEC, bool XN4, bool YN4, bool XAL, bool YAL, int GV>
     static int gn_slab_launch(const GnArgs &a, const GnSlab &c, hipStream_t s) {
         const int  slabs = (int) ceil_div(a.CV, c.vectors), spread = a.N >= 8 ? 8 : 1;
-        const dim3 grid((unsigned) (round_up(a.N, spread) * slabs));
-        if (c.threads == 256) gn_slab_kernel<T, VEC, XN4, YN4, XAL, YAL, 256, 8, GV><<<grid, 256, 0, s>>>(a, c.vectors, slabs, spread);
-        else if (c.pixels == 8) gn_slab_kernel<T, VEC, XN4, YN4, XAL, YAL, 1024, 8, GV><<<grid, 1024, 0, s>>>(a, c.vectors, slabs, spread);
-        else gn_slab_kernel<T, VEC, XN4, YN4, XAL, YAL, 1024, 16, GV><<<grid, 1024, 0, s>>>(a, c.vectors, slabs, spread);
+        const dim3 grid((unsigned) (spread * slabs), (unsigned) ceil_div(a.N, spread)); // a dimension of a launch has fewer than 2^32 threads
+        if (c.threads == 256) gn_slab_kernel<T, VEC, XN4, YN4, XAL, YAL, 256, 8, GV><<<grid, 256, 0, s>>>(a, c.vectors, spread);
+        else if (c.pixels == 8) gn_slab_kernel<T, VEC, XN4, YN4, XAL, YAL, 1024, 8, GV><<<grid, 1024, 0, s>>>(a, c.vectors, spread);
+        else gn_slab_kernel<T, VEC, XN4, YN4, XAL, YAL, 1024, 16, GV><<<grid, 1024, 0, s>>>(a, c.vectors, spread);
         return check_launch("group_norm");
     }
 
