@@ -172,3 +172,19 @@ def test_group_norm_many_workgroups(gpu):
     y = T.group_norm(V.vkhip(), x, groups, None, None, "f16", 2, 2)
     T.check_gn(y[:51], some, groups, None, None, "f16", 0)
     assert torch.equal(y, y[:51].repeat(1285, 1, 1))
+
+
+@pytest.mark.parametrize("batch,heads", [(64, (1 << 18) + 64), (70001, 3)])
+def test_attention_many_workgroups(gpu, batch, heads):
+    """More tiles and heads than a launch has work items in one dimension, and more tiles than workgroups in the second:
+    sequences of one token, each its own only key, so that every head gives that token's value."""
+    lib, d = V.vkhip(), 8
+    q, v = T.Dev(T.rand(1, batch, d).half()), T.rand(2, batch, d).half()
+    dv, out = T.Dev(v), T.Dev.zeros((batch, heads, d), torch.float16)
+    desc = V.AttentionDesc(batch=batch, q_heads=heads, kv_heads=1, head_dim=d, total_q=batch, total_k=batch, dtype=V.DT_F16, causal=1, scale=0.5, q_row=d, q_head=0,
+                           k_row=d, k_head=d, v_row=d, v_head=d, o_row=heads * d, o_head=d)
+    cu, ws = T.ints(list(range(batch + 1))), T.workspace(lib.vkhip_attention_workspace_bytes(R(desc)))
+    T.sync()
+    check(lib.vkhip_attention_packed(R(desc), q.data_ptr(), q.data_ptr(), dv.data_ptr(), cu.data_ptr(), cu.data_ptr(), out.data_ptr(), ws.data_ptr(), None))
+    T.sync()
+    assert torch.equal(out.get(), v[:, None].expand(batch, heads, d))

@@ -102,10 +102,11 @@ namespace vkhip {
         const auto v_tile = [&](auto odd_c) { return odd_c ? (LdsPtr) sm_v1 : (LdsPtr) sm_v0; };
 
         const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, col = lane & 31;
-        // heads of one key/value head next to each other in the grid: workgroups go to the 8 XCDs in turn
+        // heads of one key/value head next to each other in the grid: workgroups go to the 8 XCDs in turn; then splits, and
+        // tiles over the other dimensions
         const int head_kv = blockIdx.x % a.kv_heads, group = a.q_heads / a.kv_heads;
-        const int head_q = head_kv * group + blockIdx.x / a.kv_heads % group, split = blockIdx.x / a.q_heads % a.splits;
-        const int item   = (int) (blockIdx.x / a.q_heads / a.splits);
+        const int head_q = head_kv * group + blockIdx.x / a.kv_heads % group, split = blockIdx.x / a.q_heads;
+        const int item   = (int) (blockIdx.z * gridDim.y + blockIdx.y);
         // the most work first, where that is known: with causal a sequence's last queries see the most keys
         const auto count = [&](int b) { return (clampi(a.cu_q[b + 1], 0, a.total_q) - clampi(a.cu_q[b], 0, a.total_q) + kAttnQ - 1) / kAttnQ; };
         SeqTile w = a.causal && a.batch <= 64 ? find_tile_falling(item, a.batch, count) : find_tile(item, a.batch, count);
@@ -424,7 +425,8 @@ namespace vkhip {
         for (int64_t v: st)
             if (v < 0 || v % 8) return "strides are not multiples of 8";
         if (d->k_row < d->head_dim || d->v_row < d->head_dim || d->k_row > (1 << 23) || d->v_row > (1 << 23)) return "k_row or v_row under head_dim or over 2^23";
-        if ((ceil_div(d->total_q, kAttnQ) + d->batch) * (int64_t) d->q_heads > 0x3FFFFFF) return "too many queries and heads";
+        // a dimension of a launch has fewer than 2^32 threads, 256 of them a head
+        if ((ceil_div(d->total_q, kAttnQ) + d->batch) * (int64_t) d->q_heads > 0x3FFFFFF || d->q_heads > 0xFFFFFF) return "too many queries and heads";
         return nullptr;
     }
 
@@ -458,7 +460,8 @@ int vkhip_attention_packed(const vkhip_attention_desc *d, const void *q, const v
     // sequences have fewer than total_q / 128 + batch tiles together
     int64_t tiles = d->total_q / kAttnQ + d->batch;
     if (tiles > d->total_q) tiles = d->total_q;
-    const dim3  grid((unsigned) (tiles * d->q_heads * splits));
+    const int64_t layers = ceil_div(tiles, 65535); // the second dimension's limit
+    const dim3  grid((unsigned) (d->q_heads * splits), (unsigned) ceil_div(tiles, layers), (unsigned) layers);
     hipStream_t st = resolve_stream(s);
     if (d->dtype == VKHIP_DT_F16) {
         if (d->head_dim <= 64) attn_packed_kernel<half_t, 64><<<grid, 256, 0, st>>>(a);
