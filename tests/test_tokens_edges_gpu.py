@@ -188,3 +188,26 @@ def test_attention_many_workgroups(gpu, batch, heads):
     check(lib.vkhip_attention_packed(R(desc), q.data_ptr(), q.data_ptr(), dv.data_ptr(), cu.data_ptr(), cu.data_ptr(), out.data_ptr(), ws.data_ptr(), None))
     T.sync()
     assert torch.equal(out.get(), v[:, None].expand(batch, heads, d))
+
+
+@pytest.mark.parametrize("page", [32, 256])
+def test_append_many_blocks(gpu, page):
+    """More blocks of rows than a launch has workgroups in one dimension: 2^30 rows (one, read again and again), of which
+    only the last block's have a page."""
+    total, d = 1 << 30, 8
+    c = T.Cache(1, 1, page, 1, d)
+    c.blocks = total // page
+    names = torch.full((1, c.blocks), -1, dtype=torch.int32)
+    names[0, -1] = c.pages - 1
+    c.gpu_table = T.Dev(names)
+    k, v = T.rand(1, 1, d).half(), T.rand(2, 1, d).half()
+    dk, dv, cu, at = T.Dev(k), T.Dev(v), T.ints([0, total]), T.ints([0])
+    rows = V.KvRows(dtype=V.DT_F16, total=total, k_row=0, k_head=d, v_row=0, v_head=d)
+    T.sync()
+    check(V.vkhip().vkhip_kv_append(R(c.desc()), R(rows), dk.data_ptr(), dv.data_ptr(), cu.data_ptr(), at.data_ptr(), None))
+    T.sync()
+    for x, cells, scales in ((k, c.k.get()[-1, 0, :, :d], c.ks.get()), (v, c.v.get()[-1, 0, :d].T, c.vs.get())):
+        assert torch.isnan(scales[:-1]).all()
+        quot, scale = T.append64(torch.zeros(0, 1, d), torch.zeros(0, 1), x[None], 0, page)
+        assert torch.allclose(scales[-1].double(), scale[0], rtol=2.0 ** -23, atol=0)
+        assert ((cells.double() - quot[0]).abs() <= 0.5 + 127 * 2.0 ** -22).all()

@@ -51,7 +51,8 @@ namespace vkhip {
         return (float) __builtin_bit_cast(T, (unsigned short) bits);
     }
 
-    // Sequence, block of page_tokens tokens, and the rows of the call that lie in it.
+    // Blocks go over the grid's first dimension, which holds 2^24 workgroups of 256 threads, and on over its third, whose
+    // lowest bit says keys or values. Sequence, block of page_tokens tokens, and the rows of the call that lie in it.
     struct KvSpan {
         int     b, n0, n; // tokens of the block before the call's rows (append) or in front of them (read), rows
         int     row, page;
@@ -63,7 +64,7 @@ namespace vkhip {
             from = clampi(a.at[b], 0, most);
             len  = min(clampi(a.cu[b + 1], 0, a.total) - row, most - from);
         };
-        const SeqTile t = find_tile((int) blockIdx.x, a.c.batch, [&](int b) {
+        const SeqTile t = find_tile((int) ((blockIdx.z >> 1) * gridDim.x + blockIdx.x), a.c.batch, [&](int b) {
             int from, len, row;
             range(b, from, len, row);
             return len > 0 ? ((from + len - 1) >> a.c.page_shift) - (from >> a.c.page_shift) + 1 : 0;
@@ -197,7 +198,7 @@ namespace vkhip {
         __shared__ unsigned        red[THREADS / 64];
         const KvSpan w = kv_span(a);
         if (w.b < 0 || w.page < 0) return;
-        if (blockIdx.z) append_block<T, THREADS, R, true>(a, w, blockIdx.y, words, red);
+        if (blockIdx.z & 1) append_block<T, THREADS, R, true>(a, w, blockIdx.y, words, red);
         else append_block<T, THREADS, R, false>(a, w, blockIdx.y, words, red);
     }
 
@@ -208,7 +209,7 @@ namespace vkhip {
         const KvSpan w = kv_span(a);
         if (w.b < 0) return;
         const int     P = a.c.page_tokens, D = a.c.head_dim, Dp = a.c.row, dv = D / 8, tid = threadIdx.x, head = blockIdx.y, end = w.n0 + w.n, quad0 = w.n0 / 4;
-        const bool    values = blockIdx.z, none = w.page < 0;
+        const bool    values = blockIdx.z & 1, none = w.page < 0;
         const int64_t stride = values ? a.v_row : a.k_row, at = (int64_t) (none ? 0 : w.page) * a.c.heads + head;
         T            *rows   = (T *) (values ? a.v : a.k) + (int64_t) (w.row - w.n0) * stride + (int64_t) head * (values ? a.v_head : a.k_head);
         const float   s      = none ? 0.f : (values ? a.c.v_scale : a.c.k_scale)[at];
@@ -383,7 +384,8 @@ namespace vkhip {
         // n rows touch fewer than n / page_tokens + 2 blocks and no more than n
         int64_t tiles = (int64_t) r->total / c->page_tokens + 2 * (int64_t) c->batch;
         if (tiles > r->total) tiles = r->total;
-        const dim3   grid((unsigned) tiles, (unsigned) c->kv_heads, 2);
+        const int64_t layers = ceil_div(tiles, 0xFFFFFF);
+        const dim3   grid((unsigned) ceil_div(tiles, layers), (unsigned) c->kv_heads, (unsigned) (2 * layers));
         const size_t lds = (size_t) a.c.head_dim * (c->page_tokens / 4 + 1) * 4;
         hipStream_t  q   = resolve_stream(s);
         if (append) {
