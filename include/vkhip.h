@@ -480,7 +480,7 @@ int    vkhip_group_norm(const vkhip_group_norm_desc *d, const void *x, const flo
  * sequence, and theirs of o are not written. What a query does not see never reaches it, NaN and
  * infinities included. Weights are rounded to the 16-bit type before they multiply v, their sum is not.
  * F16 or BF16; head_dim a multiple of 8 up to 128; scale > 0; every row of every head starts on a
- * 16-byte boundary; k_row and v_row head_dim .. 2^23. o must not overlap q, k or v. workspace:
+ * 16-byte boundary; k_row and v_row head_dim .. 2^23. o must not overlap q, k or v, nor its rows each other. workspace:
  * vkhip_attention_workspace_bytes (0: NULL is taken), 16-byte aligned, contents undefined. */
 typedef struct vkhip_attention_desc {
     int32_t batch, q_heads, kv_heads, head_dim;
@@ -525,11 +525,12 @@ typedef struct vkhip_kv_rows {
 int vkhip_kv_append(const vkhip_kv_cache *c, const vkhip_kv_rows *r, const void *k, const void *v, const int32_t *cu, const int32_t *lens,
                     vkhip_stream_t s);
 /* The tokens start[b] .. start[b] + cu[b+1] - cu[b] of sequence b as the rows cu[b] .. cu[b+1]: what prompt
- * attention behind a cached prefix takes. Rows of tokens past max_blocks * page_tokens are not written. */
+ * attention behind a cached prefix takes. Rows of tokens past max_blocks * page_tokens are not written; rows must not
+ * overlap each other. */
 int vkhip_kv_read(const vkhip_kv_cache *c, const vkhip_kv_rows *r, const int32_t *start, const int32_t *cu, void *k, void *v, vkhip_stream_t s);
 /* Attention over the cache: the last q_tokens (1 .. 64) tokens of each sequence of lens[b] tokens, query t at
  * position lens[b] - q_tokens + t, over the tokens up to its own position. q and o: row b * q_tokens + t,
- * F16 or BF16, 16-byte aligned rows per head. max_len: no length is larger (0: max_blocks * page_tokens);
+ * F16 or BF16, 16-byte aligned rows per head, those of o apart from each other. max_len: no length is larger (0: max_blocks * page_tokens);
  * it sizes the launch, longer sequences are cut to it. A query that sees no token gives zeros. workspace:
  * vkhip_kv_attention_workspace_bytes (0: NULL is taken), 16-byte aligned, contents undefined. */
 typedef struct vkhip_kv_attention_desc {

@@ -425,6 +425,7 @@ namespace vkhip {
         for (int64_t v: st)
             if (v < 0 || v % 8) return "strides are not multiples of 8";
         if (d->k_row < d->head_dim || d->v_row < d->head_dim || d->k_row > (1 << 23) || d->v_row > (1 << 23)) return "k_row or v_row under head_dim or over 2^23";
+        if (rows_overlap(d->total_q, d->o_row, d->q_heads, d->o_head, d->head_dim)) return "rows of o share memory";
         // a dimension of a launch has fewer than 2^32 threads, 256 of them a head
         if ((ceil_div(d->total_q, kAttnQ) + d->batch) * (int64_t) d->q_heads > 0x3FFFFFF || d->q_heads > 0xFFFFFF) return "too many queries and heads";
         return nullptr;

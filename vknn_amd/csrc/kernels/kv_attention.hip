@@ -367,6 +367,7 @@ namespace vkhip {
         if (d->dtype != VKHIP_DT_F16 && d->dtype != VKHIP_DT_BF16) return "q and o are F16 or BF16";
         if (!(d->scale > 0.f) || d->scale > 1e30f || d->max_len < 0) return "scale is not positive or max_len negative";
         if (d->q_row < 0 || d->q_head < 0 || d->o_row < 0 || d->o_head < 0 || (d->q_row | d->q_head | d->o_row | d->o_head) % 8) return "strides are not multiples of 8";
+        if (rows_overlap((int64_t) c->batch * d->q_tokens, d->o_row, d->q_heads, d->o_head, c->head_dim)) return "rows of o share memory";
         return nullptr;
     }
 

@@ -374,6 +374,8 @@ namespace vkhip {
         if (r->dtype != VKHIP_DT_F16 && r->dtype != VKHIP_DT_BF16) return set_error(VKHIP_ERR_INVALID, "%s: rows are F16 or BF16", what);
         if (r->k_row < 0 || r->v_row < 0 || r->k_head < 0 || r->v_head < 0 || (r->k_row | r->v_row | r->k_head | r->v_head) % 8)
             return set_error(VKHIP_ERR_INVALID, "%s: strides are not multiples of 8", what);
+        if (!append && (rows_overlap(r->total, r->k_row, c->kv_heads, r->k_head, c->head_dim) || rows_overlap(r->total, r->v_row, c->kv_heads, r->v_head, c->head_dim)))
+            return set_error(VKHIP_ERR_INVALID, "%s: rows share memory", what);
         if (r->total == 0 || c->batch == 0 || c->max_blocks == 0) return VKHIP_OK;
         if (!k || !v || !cu || !at) return set_error(VKHIP_ERR_INVALID, "%s: null pointer", what);
         if (misaligned16(k) || misaligned16(v) || ((uintptr_t) cu | (uintptr_t) at) % 4) return set_error(VKHIP_ERR_INVALID, "%s: misaligned pointer", what);

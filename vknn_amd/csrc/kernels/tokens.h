@@ -98,6 +98,11 @@ namespace vkhip {
 
     __device__ __forceinline__ int clampi(int v, int lo, int hi) { return v < lo ? lo : (v > hi ? hi : v); }
 
+    // Whether an output's first two rows or heads of `dim` values share memory (strides in elements).
+    inline bool rows_overlap(int64_t rows, int64_t row, int64_t heads, int64_t head, int64_t dim) {
+        return (rows > 1 && row < dim) || (heads > 1 && head < dim) || (rows > 1 && heads > 1 && row - head < dim && head - row < dim);
+    }
+
     inline bool misaligned16(const void *p) { return ((uintptr_t) p) % 16 != 0; }
 
 } // namespace vkhip
