@@ -211,3 +211,53 @@ def test_append_many_blocks(gpu, page):
         quot, scale = T.append64(torch.zeros(0, 1, d), torch.zeros(0, 1), x[None], 0, page)
         assert torch.allclose(scales[-1].double(), scale[0], rtol=2.0 ** -23, atol=0)
         assert ((cells.double() - quot[0]).abs() <= 0.5 + 127 * 2.0 ** -22).all()
+
+
+@pytest.mark.parametrize("page,heads,d,dtype", [(32, 3, 64, "f16"), (64, 2, 128, "bf16"), (128, 1, 72, "f16"), (256, 2, 40, "bf16"), (64, 5, 8, "f16")])
+def test_append_few_rows_to_filled_pages(gpu, page, heads, d, dtype):
+    """Four rows a sequence or fewer, onto pages that hold tokens: the middle of a word, the last place of a page, a new
+    page, several rows of one sequence over a page's end; scales that grow under the old tokens and that do not."""
+    lens = [3, 1, 13, page - 1, page, page + 5, 2 * page - 3, 0]
+    c = T.Cache(8, 4, page, heads, d)
+    seen = [[(torch.zeros(0, heads, d, dtype=torch.int8), torch.zeros(0, heads)) for _ in range(2)] for _ in range(8)]
+    fill, held = list(lens), [0] * 8
+    steps = [fill, [1] * 8, [1] * 8, [0, 9, 0, 1, 0, 0, 13, 4], [1, 1, 1, 1, 1, 1, 1, 0], [0, 0, 31, 0, 0, 0, 0, 1], [4] * 8]
+    for step, new in enumerate(steps):
+        assert step == 0 or sum(new) <= 4 * len(new)
+        # louder at every other step, quieter between; one head much louder, so that only its scale grows
+        size = torch.ones(heads, 1) * (1.0 if step % 2 else 0.25)
+        size[step % heads] = 2.0 ** step
+        k = (T.rand(step, sum(new), heads, d) * size).to(T.DT[dtype][0]).float()
+        v = (T.rand(step + 50, sum(new), heads, d) * size.flip(0)).to(T.DT[dtype][0]).float()
+        c.append(k, v, new, held, dtype)
+        at = 0
+        for b, n in enumerate(new):
+            got = c.bytes_of(b, held[b] + n)
+            for which, x in enumerate((k, v)):
+                quot, scale = T.append64(*seen[b][which], x[at:at + n], held[b], page)
+                q, s = got[which]
+                assert torch.allclose(s.double(), scale, rtol=2.0 ** -23, atol=0)
+                assert ((q.double() - quot).abs() <= 0.5 + 127 * 2.0 ** -22).all()
+                old, old_s = seen[b][which]
+                same = (s[:held[b]] == old_s)[:, :, None].expand_as(old)
+                assert torch.equal(q[:held[b]][same], old[same])
+            seen[b] = got
+            held[b] += n
+            at += n
+
+
+@pytest.mark.parametrize("n,p,c,groups", [(1, 1301, 20, 4), (2, 7001, 12, 1), (3, 1301, 21, 7), (1, 2049, 10, 1), (2, 512, 44, 4), (1, 30000, 24, 2), (1, 48000, 8, 2)])
+@pytest.mark.parametrize("xf,yf", [(2, 1), (2, 2), (1, 2)])
+def test_group_norm_planes_of_several_chunks(gpu, monkeypatch, n, p, c, groups, xf, yf):
+    """NC4HW4 norms that no workgroup holds: several chunks of pixels, whole batches and a remainder; what lies past the
+    channels is NaN."""
+    def planes(x):
+        y = torch.full((x.shape[0], x.shape[1], (c + 3) // 4 * 4), float("nan"), dtype=x.dtype)
+        y[:, :, :c] = x
+        return y.view(*x.shape[:2], -1, 4).permute(0, 2, 1, 3).contiguous()
+
+    monkeypatch.setattr(T, "to_nc4", planes)
+    x = (T.rand(p + c, n, p, c) * (1 + torch.arange(c) % 5) + torch.arange(c) % 3).half().float()
+    gamma, beta = T.rand(1, c), T.rand(2, c)
+    y = T.group_norm(V.vkhip(), x, groups, gamma, beta, "f16", xf, yf, 5)
+    T.check_gn(y, x, groups, gamma, beta, "f16", 5)
