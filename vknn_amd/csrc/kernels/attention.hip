@@ -14,8 +14,11 @@
 // weights are raised by 2^7 to 2^15, so that many small ones beside a large one are not lost.
 //
 // Bound by the matrix and vector units together, and by power: 16384 causal queries, 32 heads on 8, D = 128, fp16
-// 2.06 to 2.17 ms by the card's clock (1067 to 1014 TFLOP/s; a 16384^3 library product 1246), 1.6 to 1.5 GHz, matrix units busy 62% of it, vector
-// units 51%, no bank conflicts. 4 x 4096 not causal 1027, D = 64 bf16 952 TFLOP/s. 200 queries behind 50000 keys 96 us.
+// 2.06 to 2.17 ms by the card's clock (1067 to 1014 TFLOP/s; a 16384^3 library product 1246), 1.65 to 1.5 GHz, matrix
+// units busy 61% of it, vector units 51%, no bank conflicts. 4 x 4096 not causal 1031, D = 64 bf16 954 TFLOP/s. Head dims
+// other than 64 and 128 take the next width's products: 4 x 4096 causal, fp16, TFLOP/s of D's own products at D = 32,
+// 64, 80, 96, 112, 128: 422, 820, 674, 780, 855, 951. A tile of 128 queries of one head is mostly padding where queries
+// are few, and each head reads the keys again: 200 queries behind 50000 keys 96 us, 16 behind 9000 (32 heads) 30.
 // Two workgroups a compute unit (LDS 72 KB, up to 256 registers) overlap one's exponentials with the other's
 // products; raising a wave's priority around its products or loading V's first fragments earlier changed nothing.
 #include "tokens.h"
@@ -125,7 +128,7 @@ namespace vkhip {
         const int k_end = max(0, a.causal ? min(nk, min(i0 + kAttnQ, nq) + shift) : nk);
         const int all = (k_end + kAttnK - 1) / kAttnK, per = ((all + a.splits - 1) / a.splits + 1) & ~1;
         const int first = min(all, split * per), tiles = min(all, first + per); // this split's tiles
-        // the first tiles, an even number, are seen whole by every query of the workgroup
+        // the first tiles, an even number, are seen whole by every query of the workgroup (an odd one goes with the masked)
         const int plain = min(tiles, max(0, a.causal ? min(nk, i0 + shift + 1) : nk) / kAttnK) & ~1;
         // and this wave has no use for tiles from `used` on
         const int w_first = i0 + wave * 32;
@@ -236,7 +239,8 @@ namespace vkhip {
             float base = m == -__builtin_inff() ? 0.f : m, mul = a.c2;
             if (far) {
                 // fp32 is 1/8 or coarser there: the products are rounded as the maximum's was, which one rounding of
-                // product and difference together would miss by up to half a step, any power of two
+                // product and difference together would miss by up to half a step, any power of two. The branch costs
+                // up to 1% (4 x 4096 causal 570 -> 576 us).
 #pragma clang fp contract(off)
 #pragma unroll
                 for (int kk = 0; kk < 2; ++kk)

@@ -211,6 +211,9 @@ namespace vkhip {
         }
     }
 
+    // From NC4HW4 every workgroup joins the entries of all channels of its groups, chunks * Cg of each, 64 lanes a group at
+    // most. That is little next to its pixels but for wide groups: 1 x 512 x 112 x 112 in 32 groups 17 us, in two 50, in one
+    // 88.
     template <typename T, int VEC, bool XN4, bool YN4, bool XAL, bool YAL>
     __global__ __launch_bounds__(kGnThreads) void gn_apply_kernel(GnArgs a) {
         extern __shared__ float sm[];
@@ -307,11 +310,15 @@ namespace vkhip {
         }
     }
 
-    // One launch: a workgroup owns a slab of one image and keeps all of its pixels in registers: mean, then
+    // One launch: a workgroup owns a slab of one image and keeps all of its pixels to itself: mean, then
     // deviations from it, then the output, x read once. A slab is a group of SV whole vectors of channels or
-    // (GV > 1) a vector of GV whole groups. Slabs of several groups side by side, whose rows' pieces are longer,
-    // were slower (64 x 256 x 28 x 28: 34 us with four groups, 24 with one): one workgroup a compute unit has nothing
-    // to read while it writes.
+    // (GV > 1) a vector of GV whole groups. Every thread loads R pixels, those past its own the last one again: at 7 x 7
+    // seven loads of eight. The compiler keeps x's fp32 values from the first sum to the output beside x itself. 256
+    // threads hold them in registers; 1024 threads (128 registers each) hold 8 pixels of 4 channels, 16 where they are one
+    // group's, and 8 pixels of 8 channels of one group (fp16: of two). The other variants of 1024 threads put up to 976
+    // bytes a lane into scratch.
+    // Slabs of several groups side by side, whose rows' pieces are longer, measured 34 us against 24 (64 x 256 x 28 x 28,
+    // four groups), in a form that may have used scratch too: not settled.
     template <typename T, int VEC, bool XN4, bool YN4, bool XAL, bool YAL, int THREADS, int R, int GV>
     __global__ __launch_bounds__(THREADS) void gn_slab_kernel(GnArgs a, int SV, int spread) {
         using X             = GnIo<T, VEC, XN4, XAL>;
@@ -422,9 +429,11 @@ namespace vkhip {
         return check_launch("group_norm");
     }
 
-    // Pixels of a chunk: workgroups for every compute unit, whole batches of the threads' pixels where there are
-    // enough, and no more than 48 chunks or so, since each workgroup of the second launch joins them all (1 x 64 x 80 x 80:
-    // 11.6 us, 15.0 with up to 128).
+    // Pixels of a chunk: workgroups for every compute unit, and no more than 48 chunks, since each workgroup of the
+    // second launch joins them all (1 x 64 x 80 x 80: 11.6 us, 15.0 with up to 128); then whole batches of the threads'
+    // pixels where there are enough, rounded down, which makes up to 96 chunks. Rounded up there instead, rows lose (1 x
+    // 64 x 150 x 150 12.2 -> 14.1 us, 1 x 512 x 60 x 60 15.1 -> 17.7) and NC4HW4 of wide groups gains (1 x 256 x 200 x 240,
+    // four groups, 54 -> 35).
     static int gn_chunk(const vkhip_group_norm_desc *d) {
         const int64_t hw = (int64_t) d->H * d->W, vectors = ceil_div((int64_t) d->C * (d->dtype == VKHIP_DT_F32 ? 4 : 2), 16);
         const int64_t batch = kGnBatch * (d->x_fmt == 2 ? 64 : kGnThreads / (vectors < kGnThreads ? vectors : kGnThreads));

@@ -14,7 +14,8 @@
 // (reference, sum, product) join in LDS and, across workgroups, in a second kernel.
 //
 // Measured, fp16, 32 heads on 8, D = 128: 8 x 131072 tokens 330 us (6.5 TB/s), 64 x 2048 44 us (6.2), 64 ragged
-// sequences up to 4000 56 us (4.8, the join 5 of it), 8 x 300 6.9 us. Loading the next step's keys and values while this
+// sequences up to 4000 56 us (4.8, the join 5 of it), 8 x 300 7.5 us. Head dims between the two widths read the wider
+// one's values: 64 x 2048 at D = 64, 80, 96, 128 27, 44, 43, 43 us. Loading the next step's keys and values while this
 // one's are multiplied gained nothing: it costs the registers of a third wave a SIMD, which does the same.
 #include "kv_cache.h"
 

@@ -11,8 +11,8 @@ namespace vkhip {
     typedef uint32_t tk_u32x2 __attribute__((ext_vector_type(2)));
     typedef uint32_t tk_u32x4 __attribute__((ext_vector_type(4)));
 
-    // exp2 of a difference to a running maximum: the hardware instruction (1 ulp), arguments <= 0 or NaN.
-    // Below -126 it gives 0 for what would be subnormal: weights under 2^-126 of the largest one.
+    // exp2 of a difference to a running reference: the hardware instruction (1 ulp), arguments up to 16 or NaN.
+    // Below -126 it gives 0 for what would be subnormal: weights under 2^-126, where the largest is 2^-1 or more.
     __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 
     // Sums over the lanes up to each, and over all 64 (row shifts within 16 lanes, then the rows' last lanes).
