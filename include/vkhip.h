@@ -542,6 +542,96 @@ size_t vkhip_kv_attention_workspace_bytes(const vkhip_kv_attention_desc *d, cons
 int    vkhip_kv_attention(const vkhip_kv_attention_desc *d, const vkhip_kv_cache *c, const void *q, const int32_t *lens, void *o,
                           void *workspace, vkhip_stream_t s);
 
+/* ---------------------------------------------------------------- a token step of many requests
+ * What stands between the products and the cache of a step: positions of rows, pages for them, attention
+ * that reads a shared prompt once, and the norms around a block. No counterpart in the reference's
+ * backends; forward only; strides in elements; arithmetic in fp32, outputs rounded once, to nearest even. */
+
+/* Rotary positions with up to four axes (time, height, width): the first rotary_dim channels of every head
+ * of q and k, in pairs, are turned by an angle that belongs to the row and the pair:
+ *   (a, b) -> (a cos - b sin, b cos + a sin), angle = pos[axis of the pair][row] * frequency of the pair;
+ * channels from rotary_dim on are copied.
+ *   neighbours: 0 channel i of the first half with i of the second, 1 channels 2i and 2i + 1.
+ *   sections: pairs of each axis (their sum is rotary_dim / 2), one axis's after the other's or, with
+ *           interleaved, dealt to the axes in turn, past those that have theirs.
+ *   freq:   host doubles, one a pair, read before the call returns; NULL: theta^(-i / n) over all n pairs or, with
+ *           spectra, theta^(-j / n_axis) for pair j of its axis. theta is not used beside freq.
+ *   pos:    device int32 [axes][rows], pos_axis elements from one axis to the next; any value (angles are
+ *           reduced exactly: they are as good at 2^31 as at 0).
+ * F16, BF16 or F32; head_dim up to 256, rotary_dim even; any strides that keep the rows of qo and ko apart, so that
+ * rows may be slices of wider ones. qo may be q and ko k where their strides agree; otherwise nothing may
+ * overlap. k_heads of 0: no k. */
+typedef struct vkhip_rotary_desc {
+    int32_t rows, q_heads, k_heads, head_dim, rotary_dim, dtype;
+    int32_t neighbours, axes, sections[4], interleaved, spectra;
+    double  theta;
+    int64_t pos_axis;
+    int64_t q_row, q_head, k_row, k_head, qo_row, qo_head, ko_row, ko_head;
+} vkhip_rotary_desc;
+int vkhip_rotary(const vkhip_rotary_desc *d, const int32_t *pos, const double *freq, const void *q, const void *k, void *qo, void *ko, vkhip_stream_t s);
+
+/* Pages of a cache that belong to no sequence: free[0 .. state[0]) are their names, taken from the end and
+ * given back to it; state[1] counts the blocks that found none, over all calls (the caller clears it). free
+ * holds `capacity` names. Both lie on the device. */
+typedef struct vkhip_kv_pool {
+    int32_t *free, *state;
+    int32_t  capacity;
+} vkhip_kv_pool;
+/* A step's pages and rows: sequence b holds lens[b] tokens and gets add[b] more (both device int32 [batch];
+ * negative counts as 0; rows past `total` are not made, and tokens past max_blocks * page_tokens have no memory).
+ *   table: the blocks that the new tokens begin, ceil(lens / page_tokens) .. ceil((lens + add) / page_tokens),
+ *          sequence by sequence, take the list's pages from its end; those that find none become -1 (a
+ *          block without memory). Other entries stay. The table is written although the struct has it const.
+ *   cu:    int32 [batch + 1], sums of add up to `total`: the rows of each sequence, as kv_append takes them.
+ *   now:   int32 [batch], lens + rows: what kv_attention takes behind kv_append. Not lens itself.
+ *   pos, slot: of each row its token's position, int32 [total], and its place in the cache, int64 [total],
+ *          page * page_tokens + token in the page (-1: no memory). Rows from cu[batch] on are not written.
+ * now, pos and slot may be NULL. Of the cache only table, pages, page_tokens, batch and max_blocks are used here
+ * (kv_heads and head_dim have to be ones that it may have). Calls that use a pool are ordered by the caller. */
+int vkhip_kv_reserve(const vkhip_kv_cache *c, const vkhip_kv_pool *p, const int32_t *lens, const int32_t *add, int32_t total, int32_t *cu, int32_t *now,
+                     int32_t *pos, int64_t *slot, vkhip_stream_t s);
+/* The pages behind the first keep[b] of the lens[b] tokens of each sequence go back to the list (all with keep 0;
+ * rejected drafts; what lies behind a shared prefix): blocks ceil(keep / page_tokens) .. ceil(lens / page_tokens),
+ * the first of them on top, so that a reserve of the same takes them back. Their table entries become -1; entries
+ * that name no page are passed over, and pages that the list has no room for are dropped. A page goes back
+ * once: where several sequences name it, one of them gives it. */
+int vkhip_kv_release(const vkhip_kv_cache *c, const vkhip_kv_pool *p, const int32_t *lens, const int32_t *keep, vkhip_stream_t s);
+
+/* vkhip_kv_attention where sequences share their first tokens' pages: neighbouring sequences cu[g] .. cu[g+1] (device
+ * int32 [groups + 1], rising, clamped to [0, batch]) share the pages of the first tokens[g] tokens (device int32
+ * [groups], rounded down to whole pages), which are read once for all of them, through the table of the first.
+ * Sequences in no group share nothing. The result is that of vkhip_kv_attention but for rounding: what a query may
+ * see goes by its own sequence's length, also inside the prefix.
+ * max_tokens: no prefix is longer (0: max_len); longer ones are read sequence by sequence from there on. max_tail: no
+ * sequence has more tokens behind its prefix (0: max_len); it only sizes the launch. workspace as for
+ * vkhip_kv_attention, from vkhip_kv_attention_shared_workspace_bytes. */
+typedef struct vkhip_kv_prefix {
+    const int32_t *cu, *tokens;
+    int32_t        groups, max_tokens, max_tail;
+} vkhip_kv_prefix;
+size_t vkhip_kv_attention_shared_workspace_bytes(const vkhip_kv_attention_desc *d, const vkhip_kv_cache *c, const vkhip_kv_prefix *p);
+int    vkhip_kv_attention_shared(const vkhip_kv_attention_desc *d, const vkhip_kv_cache *c, const vkhip_kv_prefix *p, const void *q, const int32_t *lens, void *o,
+                                 void *workspace, vkhip_stream_t s);
+
+/* What lies between two blocks, on rows of `dim` values (up to 32768):
+ *   h = r + alpha * gate[m] * N_post(x),  y = N_pre(h) * (1 + scale[m]) + shift[m]
+ * N_post and N_pre: VKHIP_NORM_NONE (the values), _RMS (z / sqrt(mean z^2 + eps) * w + b) or _LAYER ((z - mean) /
+ * sqrt(var + eps) * w + b, biased variance); w and b fp32 [dim], NULL = 1 and 0. N_pre takes h before it is rounded.
+ *   x NULL: h = r; r NULL: h = the block's part alone (not both). h or y may be NULL: not written (not both).
+ *   gate, scale, shift: vectors of dtype, `mods` of them, mod_row elements apart, or NULL: 1, 0, 0. Row i uses
+ *           vector m = mod[i] (device int32 [rows], clamped to the vectors) or, with mod NULL, i / mod_rows.
+ * h and y may be x or r where their rows agree (and not each other); nothing else may overlap. */
+#define VKHIP_NORM_NONE 0
+#define VKHIP_NORM_RMS 1
+#define VKHIP_NORM_LAYER 2
+typedef struct vkhip_residual_norm_desc {
+    int32_t rows, dim, dtype, post, pre, mods, mod_rows;
+    float   alpha, post_eps, pre_eps;
+    int64_t x_row, r_row, h_row, y_row, mod_row;
+} vkhip_residual_norm_desc;
+int vkhip_residual_norm(const vkhip_residual_norm_desc *d, const void *x, const void *r, const float *post_w, const float *post_b, const void *gate, const float *pre_w,
+                        const float *pre_b, const void *scale, const void *shift, const int32_t *mod, void *h, void *y, vkhip_stream_t s);
+
 #ifdef __cplusplus
 }
 #endif

@@ -25,6 +25,7 @@ c_dbl = ctypes.c_double
 
 ACT = {"none": 0, "relu": 1, "relu6": 2, "clip": 3, "hardswish": 4, "silu": 5}
 DT_F16, DT_BF16, DT_F32 = 0, 1, 2
+NORM = {"none": 0, "rms": 1, "layer": 2}
 CONV_AUTO, CONV_GEMM, CONV_SPLITK, CONV_WINOGRAD, CONV_DEPTHWISE, CONV_SPLITK_LAST = 0, 1, 2, 3, 4, 5
 
 
@@ -79,6 +80,25 @@ class KvRows(ctypes.Structure):
 class KvAttentionDesc(ctypes.Structure):
     _fields_ = [(n, c_i32) for n in ("q_heads", "q_tokens", "dtype", "max_len")] + [("scale", c_f)] + \
                [(n, c_i64) for n in ("q_row", "q_head", "o_row", "o_head")]
+
+
+class RotaryDesc(ctypes.Structure):
+    _fields_ = [(n, c_i32) for n in ("rows", "q_heads", "k_heads", "head_dim", "rotary_dim", "dtype", "neighbours", "axes")] + \
+               [("sections", c_i32 * 4), ("interleaved", c_i32), ("spectra", c_i32), ("theta", c_dbl)] + \
+               [(n, c_i64) for n in ("pos_axis", "q_row", "q_head", "k_row", "k_head", "qo_row", "qo_head", "ko_row", "ko_head")]
+
+
+class KvPool(ctypes.Structure):
+    _fields_ = [("free", c_vp), ("state", c_vp), ("capacity", c_i32)]
+
+
+class KvPrefix(ctypes.Structure):
+    _fields_ = [("cu", c_vp), ("tokens", c_vp)] + [(n, c_i32) for n in ("groups", "max_tokens", "max_tail")]
+
+
+class ResidualNormDesc(ctypes.Structure):
+    _fields_ = [(n, c_i32) for n in ("rows", "dim", "dtype", "post", "pre", "mods", "mod_rows")] + \
+               [(n, c_f) for n in ("alpha", "post_eps", "pre_eps")] + [(n, c_i64) for n in ("x_row", "r_row", "h_row", "y_row", "mod_row")]
 
 
 P = ctypes.POINTER
@@ -182,6 +202,12 @@ VKHIP_API = {
     "vkhip_kv_read": (c_int, [P(KvCache), P(KvRows), c_vp, c_vp, c_vp, c_vp, c_vp]),
     "vkhip_kv_attention_workspace_bytes": (c_sz, [P(KvAttentionDesc), P(KvCache)]),
     "vkhip_kv_attention": (c_int, [P(KvAttentionDesc), P(KvCache), c_vp, c_vp, c_vp, c_vp, c_vp]),
+    "vkhip_rotary": (c_int, [P(RotaryDesc)] + [c_vp] * 7),
+    "vkhip_kv_reserve": (c_int, [P(KvCache), P(KvPool), c_vp, c_vp, c_i32] + [c_vp] * 5),
+    "vkhip_kv_release": (c_int, [P(KvCache), P(KvPool), c_vp, c_vp, c_vp]),
+    "vkhip_kv_attention_shared_workspace_bytes": (c_sz, [P(KvAttentionDesc), P(KvCache), P(KvPrefix)]),
+    "vkhip_kv_attention_shared": (c_int, [P(KvAttentionDesc), P(KvCache), P(KvPrefix)] + [c_vp] * 5),
+    "vkhip_residual_norm": (c_int, [P(ResidualNormDesc)] + [c_vp] * 13),
 }
 
 VKNN_API = {

@@ -17,51 +17,18 @@
 // sequences up to 4000 56 us (4.8, the join 5 of it), 8 x 300 7.5 us. Head dims between the two widths read the wider
 // one's values: 64 x 2048 at D = 64, 80, 96, 128 27, 44, 43, 43 us. Loading the next step's keys and values while this
 // one's are multiplied gained nothing: it costs the registers of a third wave a SIMD, which does the same.
-#include "kv_cache.h"
+#include "kv_attention.h"
 
 namespace vkhip {
 
-    struct KvAttnArgs {
-        KvArgs         c;
-        const void    *q;
-        void          *o;
-        const int32_t *lens;
-        float         *part_o, *part_s; // [batch][head][row][split]: products [head_dim]; (reference, sum)
-        float          scale;
-        int            group, rows, q_tokens; // query heads per kv head; rows = group * q_tokens
-        int            blocks;                // blocks of 16 * RT rows
-        int            max_len, span, splits; // tokens per workgroup
-        int            waves;                 // of a workgroup
-        int64_t        q_row, q_head, o_row, o_head;
-    };
-
-    constexpr int kWeightBits = 14; // weights are up to 2^14, values b 2^-14
-
-    // 4 int8 (as bits) -> 4 fp16 b 2^-DOWN, exactly: the byte with its sign flipped is the low byte of
-    // (1024 + (b + 128)) 2^-DOWN, whose high byte is 0x64 less 4 for each power of two.
-    template <int DOWN>
-    __device__ __forceinline__ void i8_to_h4(unsigned b, half2v &lo, half2v &hi) {
-        b ^= 0x80808080u;
-        constexpr unsigned high = (0x64u - 4 * DOWN) * 0x01010101u;
-        constexpr float    zero = 1152.f / (1 << DOWN);
-        const half2v       off  = {(half_t) zero, (half_t) zero};
-        lo = __builtin_bit_cast(half2v, __builtin_amdgcn_perm(high, b, 0x04010400u)) - off;
-        hi = __builtin_bit_cast(half2v, __builtin_amdgcn_perm(high, b, 0x04030402u)) - off;
-    }
-    template <int DOWN>
-    __device__ __forceinline__ half8 i8_to_h8(unsigned a, unsigned b) {
-        half2v x, y, z, w;
-        i8_to_h4<DOWN>(a, x, y);
-        i8_to_h4<DOWN>(b, z, w);
-        return half8 {x[0], x[1], y[0], y[1], z[0], z[1], w[0], w[1]};
-    }
-
-    constexpr int kStep = 64; // tokens a wave takes at a time
 
     // DJ = row / 64 channels, RT tiles of 16 rows, P32: pages of 32 tokens (two to a step), NW waves.
     // Two row tiles of 64 channels are compiled for two waves a SIMD: 16 x 5000 tokens, 32 rows, 31.7 -> 29.1 us; of 128
     // channels that costs more than it gives (4 x 40000, 64 rows, 132 -> 160 us), one row tile gains nothing.
-    template <typename T, int DJ, int RT, bool P32, int NW>
+    // MODE: a sequence's tokens (kAll), those behind the prefix that it shares (kTail), or a group's prefix (kPrefix), whose
+    // rows are those of all its sequences; the last two leave parts for the join.
+    enum { kAll, kTail, kPrefix };
+    template <typename T, int DJ, int RT, bool P32, int NW, int MODE>
     __global__ __launch_bounds__(NW * 64, DJ == 1 && RT == 2 ? 2 : 1) void kv_attention_kernel(KvAttnArgs a) {
         constexpr int Dp = DJ * 64, DT = DJ * 4, NL = NW < 4 ? NW : 4; // NL: waves whose products lie in LDS at a time
         __shared__ float wave_m[NW][RT * 16], wave_l[NW][RT * 16];
@@ -69,11 +36,27 @@ namespace vkhip {
         const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, nn = lane & 15;
         // heads, then sequences, then splits: workgroups go to the 8 XCDs in turn, and with splits first the later ones,
         // which short sequences do not have, would all meet on some of them
-        const int head = blockIdx.x / a.blocks, row0 = blockIdx.x % a.blocks * (16 * RT), b = blockIdx.y, split = blockIdx.z;
+        const int head = MODE == kPrefix ? blockIdx.x : blockIdx.x / a.blocks, split = blockIdx.z;
         const int P   = a.c.page_tokens, D = a.c.head_dim;
-        const int len = clampi(a.lens[b], 0, min(a.max_len, a.c.max_blocks * P));
-        const int t0 = split * a.span, t1 = min(len, t0 + a.span);
-        if (t0 >= len && split > 0) return; // split 0 also answers for a sequence without tokens
+        int       b = blockIdx.y, row0 = blockIdx.x % a.blocks * (16 * RT), rows = a.rows, len, t0, t1; // kPrefix: b is the group's first sequence
+        if constexpr (MODE == kPrefix) {
+            const auto    bound = [&](int i) { return clampi(a.cu[i], 0, a.c.batch); };
+            const SeqTile w = find_tile(blockIdx.y, a.groups, [&](int g) { return prefix_of(a, g) > 0 ? (max(0, bound(g + 1) - bound(g)) * a.rows + 16 * RT - 1) / (16 * RT) : 0; });
+            if (w.b < 0) return;
+            const int g = __builtin_amdgcn_readfirstlane(w.b);
+            b = bound(g), rows = (bound(g + 1) - b) * a.rows, row0 = __builtin_amdgcn_readfirstlane(w.tile) * (16 * RT);
+            len = prefix_of(a, g), t0 = split * a.shared_span, t1 = min(len, t0 + a.shared_span);
+            if (t0 >= len) return;
+        } else {
+            len = clampi(a.lens[b], 0, min(a.max_len, a.c.max_blocks * P));
+            t0 = split * a.span, t1 = min(len, t0 + a.span);
+            if constexpr (MODE == kTail) {
+                const int prefix = prefix_at(a, b);
+                t0 += prefix, t1 = split == a.splits - 1 ? len : min(len, t1 + prefix);
+                if (t0 >= len) return;
+            }
+            if (t0 >= len && split > 0) return; // split 0 also answers for a sequence without tokens
+        }
 
         // queries: lane holds row nn, channels 64 j + 16 g + 8 e .. + 7; bf16 rows are brought into fp16's range by
         // a power of two each (their 8 bits fit its 11; what falls below 2^-24 of a row's largest is lost)
@@ -82,10 +65,14 @@ namespace vkhip {
         float c2[RT];    // factor from a score to the exponent of 2
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
-            const int  row = row0 + rt * 16 + nn, t = row / a.group, h = head * a.group + row % a.group;
-            const bool in  = row < a.rows;
-            limit[rt]      = in ? len - a.q_tokens + t + 1 : 0;
-            const T *src   = (const T *) a.q + ((int64_t) b * a.q_tokens + t) * a.q_row + h * a.q_head;
+            int        row = row0 + rt * 16 + nn, seq = b;
+            const bool in  = row < rows;
+            if constexpr (MODE == kPrefix) seq += row / a.rows, row %= a.rows;
+            const int t = row / a.group, h = head * a.group + row % a.group;
+            limit[rt]   = in ? len - a.q_tokens + t + 1 : 0;
+            if constexpr (MODE == kPrefix)
+                if (in) limit[rt] = min(len, clampi(a.lens[seq], 0, min(a.max_len, a.c.max_blocks * P)) - a.q_tokens + t + 1);
+            const T *src = (const T *) a.q + ((int64_t) seq * a.q_tokens + t) * a.q_row + h * a.q_head;
             float    v[DJ][2][8], big = 0.f;
 #pragma unroll
             for (int j = 0; j < DJ; ++j)
@@ -280,8 +267,9 @@ namespace vkhip {
             __syncthreads();
             // VPT neighbouring channels of one row a thread
             constexpr int VPT = Dp / (4 * NW);
-            const int     n = threadIdx.x / (4 * NW), d0 = threadIdx.x % (4 * NW) * VPT, row = row0 + rt * 16 + n, q = rt * 16 + n;
-            if (row < a.rows && d0 < D) {
+            const int     n = threadIdx.x / (4 * NW), d0 = threadIdx.x % (4 * NW) * VPT, q = rt * 16 + n;
+            int           row = row0 + q, seq = b;
+            if (row < rows && d0 < D) {
                 const float tm = row_max(q), tb = tm == -__builtin_inff() ? 0.f : tm;
                 float       sum = 0.f, x[VPT];
 #pragma unroll
@@ -292,7 +280,8 @@ namespace vkhip {
 #pragma unroll
                     for (int w = 0; w < NL; ++w) x[i] += acc_lds[w][n][d0 + i];
                 }
-                if (a.splits == 1) {
+                if constexpr (MODE == kPrefix) seq += row / a.rows, row %= a.rows;
+                if (MODE == kAll && a.splits == 1) {
                     const int   t = row / a.group, h = head * a.group + row % a.group;
                     const float inv = sum == 0.f ? 0.f : 1.f / sum;
                     T          *o = (T *) a.o + ((int64_t) b * a.q_tokens + t) * a.o_row + h * a.o_head + d0;
@@ -300,7 +289,8 @@ namespace vkhip {
                     for (int i = 0; i < VPT; ++i)
                         if (d0 + i < D) o[i] = (T) (x[i] * inv);
                 } else {
-                    const int64_t at = (((int64_t) b * a.c.heads + head) * a.rows + row) * a.splits + split;
+                    const int     shared = MODE == kAll ? 0 : a.shared_splits;
+                    const int64_t at = (((int64_t) seq * a.c.heads + head) * a.rows + row) * (shared + a.splits) + (MODE == kTail ? shared : 0) + split;
 #pragma unroll
                     for (int i = 0; i < VPT; ++i)
                         if (d0 + i < D) a.part_o[at * D + d0 + i] = x[i];
@@ -313,30 +303,37 @@ namespace vkhip {
 
     // Joins the splits of a row: WPR waves each, two channels a lane; the splits' weights are formed a lane each, so
     // that the products' loads wait for nothing.
-    template <typename T, int WPR>
+    template <typename T, int WPR, bool SHARED>
     __global__ __launch_bounds__(256) void kv_join_kernel(KvAttnArgs a) {
         __shared__ float2 half[4][64];
         const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, D = a.c.head_dim, d = lane * 2;
         const int row = blockIdx.x * (4 / WPR) + wave / WPR, head = blockIdx.y, b = blockIdx.z, part = wave % WPR;
         const int len = clampi(a.lens[b], 0, min(a.max_len, a.c.max_blocks * a.c.page_tokens));
-        const int n   = row < a.rows ? max(1, (len + a.span - 1) / a.span) : 0;
-        const int64_t at = (((int64_t) b * a.c.heads + head) * a.rows + row) * a.splits;
+        int       n   = row < a.rows ? max(1, (len + a.span - 1) / a.span) : 0, shared = 0; // parts: of the prefix, which go first, and all
+        if constexpr (SHARED) {
+            const int prefix = prefix_at(a, b), tail = max(0, len - prefix);
+            shared = (prefix + a.shared_span - 1) / a.shared_span;
+            n      = row < a.rows ? shared + min(a.splits, (tail + a.span - 1) / a.span) : 0;
+        }
+        const int     skip = SHARED ? a.shared_splits - shared : 0; // slots of longer prefixes
+        const int64_t at   = (((int64_t) b * a.c.heads + head) * a.rows + row) * ((SHARED ? a.shared_splits : 0) + a.splits);
+        const auto    slot = [&](int k) { return at + (SHARED && k >= shared ? k + skip : k); };
         float top = -__builtin_inff(), sum = 0.f;
-        for (int k = lane; k < n; k += 64) top = fmaxf(top, a.part_s[(at + k) * 2]);
+        for (int k = lane; k < n; k += 64) top = fmaxf(top, a.part_s[slot(k) * 2]);
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) top = fmaxf(top, __shfl_xor(top, o));
         const float base = top == -__builtin_inff() ? 0.f : top;
         float2      x = make_float2(0.f, 0.f);
         for (int k0 = 0; k0 < n; k0 += 64) {
             const int    k = k0 + lane;
-            const float2 s = k < n ? *reinterpret_cast<const float2 *>(a.part_s + (at + k) * 2) : make_float2(-__builtin_inff(), 0.f);
+            const float2 s = k < n ? *reinterpret_cast<const float2 *>(a.part_s + slot(k) * 2) : make_float2(-__builtin_inff(), 0.f);
             const float  f = exp2_hw(s.x - base);
             sum += s.y * f;
             const int end = min(64, n - k0);
 #pragma unroll 8
             for (int i = part; i < end; i += WPR) {
                 const float w = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), i));
-                const float2 y = *reinterpret_cast<const float2 *>(a.part_o + (at + k0 + i) * D + min(d, D - 2));
+                const float2 y = *reinterpret_cast<const float2 *>(a.part_o + slot(k0 + i) * D + min(d, D - 2));
                 x.x += y.x * w, x.y += y.y * w;
             }
         }
@@ -411,9 +408,9 @@ namespace vkhip {
     template <typename T, int DJ, int RT, bool P32>
     static void kv_attention_launch(const KvAttnArgs &a, hipStream_t s) {
         const dim3 grid((unsigned) (a.c.heads * a.blocks), (unsigned) a.c.batch, (unsigned) a.splits);
-        if (a.waves == 2) kv_attention_kernel<T, DJ, RT, P32, 2><<<grid, 128, 0, s>>>(a);
-        else if (a.waves == 4) kv_attention_kernel<T, DJ, RT, P32, 4><<<grid, 256, 0, s>>>(a);
-        else if constexpr (RT == 1) kv_attention_kernel<T, DJ, RT, P32, 8><<<grid, 512, 0, s>>>(a);
+        if (a.waves == 2) kv_attention_kernel<T, DJ, RT, P32, 2, kAll><<<grid, 128, 0, s>>>(a);
+        else if (a.waves == 4) kv_attention_kernel<T, DJ, RT, P32, 4, kAll><<<grid, 256, 0, s>>>(a);
+        else if constexpr (RT == 1) kv_attention_kernel<T, DJ, RT, P32, 8, kAll><<<grid, 512, 0, s>>>(a);
     }
     template <typename T, int DJ>
     static void kv_attention_tiles(const KvAttnArgs &a, hipStream_t s) {
@@ -430,10 +427,64 @@ namespace vkhip {
         if (rc || a.splits == 1) return rc;
         const bool wide = a.splits > 8; // below, a row's products are few loads of one wave
         const dim3 grid((unsigned) (wide ? a.rows : ceil_div(a.rows, 4)), (unsigned) a.c.heads, (unsigned) a.c.batch);
-        if (wide) kv_join_kernel<T, 4><<<grid, 256, 0, s>>>(a);
-        else kv_join_kernel<T, 1><<<grid, 256, 0, s>>>(a);
+        if (wide) kv_join_kernel<T, 4, false><<<grid, 256, 0, s>>>(a);
+        else kv_join_kernel<T, 1, false><<<grid, 256, 0, s>>>(a);
         return check_launch("kv_attention join");
     }
+
+    // Groups of sequences: the prefixes for all rows of a group, then every sequence's tail, then the join.
+    template <typename T, int DJ, int RT, bool P32>
+    static int kv_shared_launch(const KvAttnArgs &a, hipStream_t s) {
+        kv_attention_kernel<T, DJ, 2, P32, 4, kPrefix><<<dim3((unsigned) a.c.heads, (unsigned) a.shared_blocks, (unsigned) a.shared_splits), 256, 0, s>>>(a);
+        if (int rc = check_launch("kv_attention_shared prefix")) return rc;
+        const dim3 grid((unsigned) (a.c.heads * a.blocks), (unsigned) a.c.batch, (unsigned) a.splits);
+        if (a.waves == 2) kv_attention_kernel<T, DJ, RT, P32, 2, kTail><<<grid, 128, 0, s>>>(a);
+        else kv_attention_kernel<T, DJ, RT, P32, 4, kTail><<<grid, 256, 0, s>>>(a);
+        return check_launch("kv_attention_shared");
+    }
+    template <typename T, int DJ>
+    static int kv_shared_tiles(const KvAttnArgs &a, hipStream_t s) {
+        const bool p32 = a.c.page_tokens == 32;
+        if (row_tiles(a.rows) == 1) return p32 ? kv_shared_launch<T, DJ, 1, true>(a, s) : kv_shared_launch<T, DJ, 1, false>(a, s);
+        return p32 ? kv_shared_launch<T, DJ, 2, true>(a, s) : kv_shared_launch<T, DJ, 2, false>(a, s);
+    }
+    template <typename T>
+    static int kv_shared_run(const KvAttnArgs &a, hipStream_t s) {
+        if (int rc = a.c.row == 64 ? kv_shared_tiles<T, 1>(a, s) : kv_shared_tiles<T, 2>(a, s)) return rc;
+        const bool wide = a.shared_splits + a.splits > 8;
+        const dim3 grid((unsigned) (wide ? a.rows : ceil_div(a.rows, 4)), (unsigned) a.c.heads, (unsigned) a.c.batch);
+        if (wide) kv_join_kernel<T, 4, true><<<grid, 256, 0, s>>>(a);
+        else kv_join_kernel<T, 1, true><<<grid, 256, 0, s>>>(a);
+        return check_launch("kv_attention_shared join");
+    }
+
+    static const char *kv_shared_refusal(const vkhip_kv_attention_desc *d, const vkhip_kv_cache *c, const vkhip_kv_prefix *p) {
+        if (const char *why = kv_attention_refusal(d, c)) return why;
+        if (!p || p->groups < 0 || p->groups > 65535) return "groups are not 0 .. 65535";
+        if (p->max_tokens < 0 || p->max_tail < 0) return "max_tokens or max_tail negative";
+        return nullptr;
+    }
+
+    // Whether a call has nothing to share, and the cut of its prefixes and tails where it has. Tails are cut like whole
+    // sequences of the longest tail.
+    static KvAttnArgs kv_shared_cut(const vkhip_kv_attention_desc *d, const vkhip_kv_cache *c, const vkhip_kv_prefix *p) {
+        const KvAttnArgs whole = kv_attention_cut(d, c);
+        vkhip_kv_attention_desc tail = *d;
+        tail.max_len = p->max_tail > 0 && p->max_tail < whole.max_len ? p->max_tail : whole.max_len;
+        KvAttnArgs a = kv_attention_cut(&tail, c);
+        if (a.waves == 8) a.waves = 4; // the span of 8 is one of 4's, twice as often
+        a.max_len    = whole.max_len;
+        a.groups     = p->groups;
+        a.max_prefix = p->max_tokens > 0 && p->max_tokens < whole.max_len ? p->max_tokens : whole.max_len;
+        a.shared_blocks = (int) ((int64_t) c->batch * a.rows / 32 + p->groups);
+        const int64_t rounds = ceil_div(a.max_prefix > 0 ? a.max_prefix : 1, 4 * kStep), base = (int64_t) a.shared_blocks * c->kv_heads;
+        int64_t       splits = base >= 512 || base == 0 ? 1 : 512 / base;
+        if (splits > rounds) splits = rounds;
+        a.shared_span   = (int) (ceil_div(rounds, splits) * 4 * kStep);
+        a.shared_splits = (int) ceil_div(a.max_prefix > 0 ? a.max_prefix : 1, a.shared_span);
+        return a;
+    }
+    static bool kv_nothing_shared(const KvAttnArgs &a) { return a.groups == 0 || a.max_prefix < a.c.page_tokens; }
 
 } // namespace vkhip
 
@@ -461,6 +512,34 @@ int vkhip_kv_attention(const vkhip_kv_attention_desc *d, const vkhip_kv_cache *c
     a.part_s = a.part_o + (size_t) c->batch * c->kv_heads * a.rows * a.splits * c->head_dim;
     a.q_row = d->q_row, a.q_head = d->q_head, a.o_row = d->o_row, a.o_head = d->o_head;
     return d->dtype == VKHIP_DT_F16 ? kv_attention_run<half_t>(a, resolve_stream(s)) : kv_attention_run<bf16_t>(a, resolve_stream(s));
+}
+
+size_t vkhip_kv_attention_shared_workspace_bytes(const vkhip_kv_attention_desc *d, const vkhip_kv_cache *c, const vkhip_kv_prefix *p) {
+    if (kv_shared_refusal(d, c, p)) return 0;
+    const KvAttnArgs a = kv_shared_cut(d, c, p);
+    if (kv_nothing_shared(a)) return vkhip_kv_attention_workspace_bytes(d, c);
+    return (size_t) c->batch * c->kv_heads * a.rows * (a.shared_splits + a.splits) * (c->head_dim + 2) * sizeof(float);
+}
+
+int vkhip_kv_attention_shared(const vkhip_kv_attention_desc *d, const vkhip_kv_cache *c, const vkhip_kv_prefix *p, const void *q, const int32_t *lens, void *o,
+                              void *workspace, vkhip_stream_t s) {
+    const char *what = "kv_attention_shared: %s";
+    if (const char *why = kv_shared_refusal(d, c, p)) return set_error(VKHIP_ERR_INVALID, what, why);
+    if (c->batch == 0) return VKHIP_OK;
+    if (const char *why = kv_bad_pointers(c)) return set_error(VKHIP_ERR_INVALID, what, why);
+    KvAttnArgs a = kv_shared_cut(d, c, p);
+    if (p->groups && (!p->cu || !p->tokens)) return set_error(VKHIP_ERR_INVALID, what, "null pointer");
+    if (((uintptr_t) p->cu | (uintptr_t) p->tokens) % 4) return set_error(VKHIP_ERR_INVALID, what, "misaligned pointer");
+    if (!q || !lens || !o) return set_error(VKHIP_ERR_INVALID, what, "null pointer");
+    if (misaligned16(q) || misaligned16(o) || misaligned16(workspace) || ((uintptr_t) lens) % 4) return set_error(VKHIP_ERR_INVALID, what, "misaligned pointer");
+    if (kv_nothing_shared(a)) return vkhip_kv_attention(d, c, q, lens, o, workspace, s);
+    if (c->pages == 0) a.max_len = a.max_prefix = 0; // no block has memory: every query gives zeros
+    if (!workspace) return set_error(VKHIP_ERR_INVALID, what, "null pointer");
+    if ((int64_t) c->kv_heads * a.blocks > 65535 || a.shared_blocks > 65535) return set_error(VKHIP_ERR_INVALID, what, "too many heads, sequences and query tokens");
+    a.q = q, a.o = o, a.lens = lens, a.part_o = (float *) workspace, a.scale = d->scale, a.cu = p->cu, a.prefix = p->tokens;
+    a.part_s = a.part_o + (size_t) c->batch * c->kv_heads * a.rows * (a.shared_splits + a.splits) * c->head_dim;
+    a.q_row = d->q_row, a.q_head = d->q_head, a.o_row = d->o_row, a.o_head = d->o_head;
+    return d->dtype == VKHIP_DT_F16 ? kv_shared_run<half_t>(a, resolve_stream(s)) : kv_shared_run<bf16_t>(a, resolve_stream(s));
 }
 
 } // extern "C"

@@ -1,0 +1,217 @@
+// Rotary positions with several axes: pairs of channels of query and key rows turned by the row's positions.
+//
+// Angles are kept as fractions of a turn in 64 bits: a pair's frequency is f 2^64 / 2 pi rounded to a whole number, the
+// angle its product with the position modulo 2^64, which is the fraction of the turn but for position * 2^-65: no bits
+// are lost at far positions, and no 64-bit floats are needed. The upper 32 bits go on to cosine and sine: the nearest
+// quarter turn is taken off as a whole number, the rest, within an eighth of a turn, goes into Taylor's series up to x^11
+// (its next terms are below 2^-34). One pair's sine and cosine serve all heads that a thread takes.
+#include "tokens.h"
+#include <math.h>
+
+namespace vkhip {
+
+    constexpr int kRotaryPairs = 128;
+
+    struct RotaryArgs {
+        const void    *q, *k;
+        void          *qo, *ko;
+        const int32_t *pos;
+        int            rows, q_heads, heads, head_dim, pairs; // heads: of q and k together
+        int            units, turned;   // of a head: pieces of VEC pairs or 2 VEC copied channels; the first `turned` are pairs
+        int            slots, per;      // threads that share a row's unit, heads of each
+        int            block_rows;      // rows of a workgroup, where several fit
+        int64_t        pos_axis, q_row, q_head, k_row, k_head, qo_row, qo_head, ko_row, ko_head;
+        uint64_t       freq[kRotaryPairs]; // turns * 2^64 per position
+        uint8_t        axis[kRotaryPairs];
+    };
+
+    __device__ __forceinline__ void turn_of(uint64_t freq, int pos, float &c, float &s) {
+        const unsigned at = (unsigned) (freq * (uint64_t) (int64_t) pos >> 32), quarter = (at + 0x20000000u) >> 30;
+        const float    x = (float) (int) (at - (quarter << 30)) * (6.283185307179586f / 4294967296.f), z = x * x;
+        float          sx = __builtin_fmaf(z, -1.f / 39916800, 1.f / 362880), cx = __builtin_fmaf(z, -1.f / 3628800, 1.f / 40320);
+        sx = __builtin_fmaf(sx, z, -1.f / 5040);
+        cx = __builtin_fmaf(cx, z, -1.f / 720);
+        sx = __builtin_fmaf(sx, z, 1.f / 120);
+        cx = __builtin_fmaf(cx, z, 1.f / 24);
+        sx = __builtin_fmaf(sx, z, -1.f / 6);
+        cx = __builtin_fmaf(cx, z, -.5f);
+        sx = __builtin_fmaf(sx * z, x, x);
+        cx = __builtin_fmaf(cx, z, 1.f);
+        c  = quarter & 1 ? sx : cx;
+        s  = quarter & 1 ? cx : sx;
+        if ((quarter + 1) & 2) c = -c;
+        if (quarter & 2) s = -s;
+    }
+
+    // A thread takes one unit of a row in several heads: VEC pairs, which are two vectors of VEC channels (a half of the
+    // rotated channels apart, or side by side), or 2 VEC channels behind them that are copied.
+    template <typename T, int VEC, bool NEAR>
+    __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
+        typedef T V __attribute__((ext_vector_type(VEC)));
+        const int     each = a.units * a.slots;
+        const int64_t block = (int64_t) blockIdx.y * gridDim.x + blockIdx.x;
+        const int     r = (int) threadIdx.x / each;
+        const int64_t row = block * a.block_rows + r;
+        if (r >= a.block_rows || row >= a.rows) return;
+        for (int i = (int) threadIdx.x - r * each; i < each; i += 256) {
+            const int  unit = i % a.units, h0 = i / a.units * a.per, h1 = min(a.heads, h0 + a.per);
+            const bool turned = unit < a.turned;
+            const int  copied = 2 * a.pairs + (unit - a.turned) * 2 * VEC; // first channel of a copied unit
+            const int  c0 = turned ? (NEAR ? unit * 2 * VEC : unit * VEC) : copied, c1 = turned && !NEAR ? a.pairs + unit * VEC : c0 + VEC;
+            const bool second = c1 < a.head_dim;
+            float      c[VEC], s[VEC];
+            if (turned)
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) {
+                    const int p = unit * VEC + j;
+                    turn_of(a.freq[p], a.pos[a.axis[p] * a.pos_axis + row], c[j], s[j]);
+                }
+#pragma unroll 2
+            for (int h = h0; h < h1; ++h) {
+                const bool    key = h >= a.q_heads;
+                const int     n = key ? h - a.q_heads : h;
+                const int64_t from = key ? row * a.k_row + n * a.k_head : row * a.q_row + n * a.q_head;
+                const int64_t to = key ? row * a.ko_row + n * a.ko_head : row * a.qo_row + n * a.qo_head;
+                const T      *x = (const T *) (key ? a.k : a.q) + from;
+                T            *y = (T *) (key ? a.ko : a.qo) + to;
+                V             u = *reinterpret_cast<const V *>(x + c0), w = u;
+                if (second) w = *reinterpret_cast<const V *>(x + c1);
+                if (turned) {
+                    if constexpr (NEAR) {
+                        float v[2 * VEC];
+#pragma unroll
+                        for (int j = 0; j < VEC; ++j) v[j] = (float) u[j], v[VEC + j] = (float) w[j];
+#pragma unroll
+                        for (int j = 0; j < VEC; ++j) {
+                            const float p = v[2 * j] * c[j] - v[2 * j + 1] * s[j], q = v[2 * j + 1] * c[j] + v[2 * j] * s[j];
+                            v[2 * j] = p, v[2 * j + 1] = q;
+                        }
+#pragma unroll
+                        for (int j = 0; j < VEC; ++j) u[j] = (T) v[j], w[j] = (T) v[VEC + j];
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < VEC; ++j) {
+                            const float p = (float) u[j], q = (float) w[j];
+                            u[j] = (T) (p * c[j] - q * s[j]), w[j] = (T) (q * c[j] + p * s[j]);
+                        }
+                    }
+                }
+                *reinterpret_cast<V *>(y + c0) = u;
+                if (second) *reinterpret_cast<V *>(y + c1) = w;
+            }
+        }
+    }
+
+    // Of each pair its axis and its fraction of a turn per position, times 2^64.
+    static void rotary_pairs(const vkhip_rotary_desc *d, const double *freq, RotaryArgs &a) {
+        // 2 pi and what it lacks: whole turns come off a frequency without its fraction losing digits
+        const long double two64 = 18446744073709551616.0L, turn = 6.28318530717958647692528676655900577L, rest = -1.0033115225336664538847901e-19L;
+        int               had[4] = {0, 0, 0, 0}, axis = 0;
+        long double       step[4], now[4]; // the next pair's angle per position, by axis; all pairs' in [0]
+        for (int i = 0; i < 4; ++i) {
+            const int n = d->spectra ? (i < d->axes ? d->sections[i] : 0) : a.pairs;
+            step[i] = n > 0 && !freq ? powl((long double) d->theta, -1.0L / n) : 1.0L, now[i] = 1.0L;
+        }
+        for (int p = 0; p < a.pairs; ++p) {
+            while (had[axis] == d->sections[axis]) axis = (axis + 1) % d->axes;
+            const int   of = d->spectra ? axis : 0;
+            const long double f = freq ? (long double) freq[p] : now[of], n = floorl(f / turn);
+            now[of] *= step[of];
+            long double t = (fmal(-n, turn, f) - n * rest) / turn;
+            t -= floorl(t); // rounding may leave it outside 0 .. 1
+            const long double whole = roundl(t * two64);
+            a.freq[p] = whole >= two64 ? 0 : (uint64_t) whole;
+            a.axis[p] = (uint8_t) axis;
+            ++had[axis];
+            if (d->interleaved) axis = (axis + 1) % d->axes;
+        }
+    }
+
+    static bool rotary_strides(int64_t row, int64_t head) { return row >= 0 && head >= 0 && row <= (int64_t) 1 << 31 && head <= (int64_t) 1 << 40; }
+
+    // Whether an output's heads lie apart within its rows, or its rows within its heads.
+    static bool rotary_apart(const vkhip_rotary_desc *d, int heads, int64_t row, int64_t head) {
+        const int64_t dim = d->head_dim, in_row = (heads - 1) * head + dim, in_head = (d->rows - 1) * row + dim;
+        const bool    one_row = d->rows <= 1, one_head = heads <= 1;
+        return ((one_head || head >= dim) && (one_row || row >= in_row)) || ((one_row || row >= dim) && (one_head || head >= in_head));
+    }
+
+    static const char *rotary_refusal(const vkhip_rotary_desc *d) {
+        if (!d || d->rows < 0 || d->q_heads <= 0 || d->k_heads < 0) return "bad sizes";
+        if (d->q_heads > 65535 || d->k_heads > 65535) return "over 65535 heads";
+        if (d->head_dim < 2 || d->head_dim > 256) return "head_dim is not 2 .. 256";
+        if (d->rotary_dim < 2 || d->rotary_dim % 2 || d->rotary_dim > d->head_dim) return "rotary_dim is not even or not 2 .. head_dim";
+        if (d->dtype < VKHIP_DT_F16 || d->dtype > VKHIP_DT_F32) return "dtype is not F16, BF16 or F32";
+        if (d->axes < 1 || d->axes > 4) return "axes is not 1 .. 4";
+        int64_t pairs = 0;
+        for (int i = 0; i < d->axes; ++i) {
+            if (d->sections[i] < 0) return "a section is negative";
+            pairs += d->sections[i];
+        }
+        if (pairs != d->rotary_dim / 2) return "sections do not sum to rotary_dim / 2";
+        if (d->axes > 1 && d->pos_axis < 0) return "pos_axis is negative";
+        if (!rotary_strides(d->q_row, d->q_head) || !rotary_strides(d->qo_row, d->qo_head)) return "a stride of q or qo is negative or too large";
+        if (!rotary_apart(d, d->q_heads, d->qo_row, d->qo_head)) return "rows of qo share memory";
+        if (d->k_heads == 0) return nullptr;
+        if (!rotary_strides(d->k_row, d->k_head) || !rotary_strides(d->ko_row, d->ko_head)) return "a stride of k or ko is negative or too large";
+        if (!rotary_apart(d, d->k_heads, d->ko_row, d->ko_head)) return "rows of ko share memory";
+        return nullptr;
+    }
+
+    template <typename T, int VEC>
+    static void rotary_launch(const vkhip_rotary_desc *d, RotaryArgs &a, hipStream_t s) {
+        a.turned = a.pairs / VEC;
+        a.units  = a.turned + (int) ceil_div(d->head_dim - d->rotary_dim, 2 * VEC);
+        // Heads of a thread: as many as leave the card full, at most 8.
+        const int64_t items = (int64_t) a.rows * a.heads * a.units, fill = 256 * 2048;
+        a.per   = (int) (items / fill < 1 ? 1 : items / fill > 8 ? 8 : items / fill);
+        a.slots = (int) ceil_div(a.heads, a.per);
+        const int each = a.units * a.slots;
+        a.block_rows   = each >= 256 ? 1 : 256 / each;
+        const int64_t blocks = ceil_div(a.rows, a.block_rows), layers = ceil_div(blocks, 0xFFFFFF);
+        const dim3    grid((unsigned) ceil_div(blocks, layers), (unsigned) layers);
+        if (d->neighbours) rotary_kernel<T, VEC, true><<<grid, 256, 0, s>>>(a);
+        else rotary_kernel<T, VEC, false><<<grid, 256, 0, s>>>(a);
+    }
+
+} // namespace vkhip
+
+using namespace vkhip;
+
+extern "C" {
+
+int vkhip_rotary(const vkhip_rotary_desc *d, const int32_t *pos, const double *freq, const void *q, const void *k, void *qo, void *ko, vkhip_stream_t s) {
+    if (const char *why = rotary_refusal(d)) return set_error(VKHIP_ERR_INVALID, "rotary: %s", why);
+    RotaryArgs a {};
+    a.pairs = d->rotary_dim / 2;
+    if (!freq && !(d->theta > 0.0 && d->theta < 1e30)) return set_error(VKHIP_ERR_INVALID, "rotary: theta is not positive");
+    if (freq)
+        for (int i = 0; i < a.pairs; ++i)
+            if (!(fabs(freq[i]) < 1e6)) return set_error(VKHIP_ERR_INVALID, "rotary: a frequency is not finite or 10^6 or more");
+    if (d->rows == 0) return VKHIP_OK;
+    const bool with_k = d->k_heads > 0;
+    if (!pos || !q || !qo || (with_k && (!k || !ko))) return set_error(VKHIP_ERR_INVALID, "rotary: null pointer");
+    const uintptr_t elem = d->dtype == VKHIP_DT_F32 ? 4 : 2, places = (uintptr_t) q | (uintptr_t) qo | (with_k ? (uintptr_t) k | (uintptr_t) ko : 0);
+    if ((uintptr_t) pos % 4 || places % elem) return set_error(VKHIP_ERR_INVALID, "rotary: misaligned pointer");
+    if ((q == qo && (d->q_row != d->qo_row || d->q_head != d->qo_head)) || (with_k && k == ko && (d->k_row != d->ko_row || d->k_head != d->ko_head)))
+        return set_error(VKHIP_ERR_INVALID, "rotary: in place with other strides");
+    a.q = q, a.k = k, a.qo = qo, a.ko = ko, a.pos = pos;
+    a.rows = d->rows, a.q_heads = d->q_heads, a.heads = d->q_heads + d->k_heads, a.head_dim = d->head_dim, a.pos_axis = d->pos_axis;
+    a.q_row = d->q_row, a.q_head = d->q_head, a.qo_row = d->qo_row, a.qo_head = d->qo_head;
+    a.k_row = d->k_row, a.k_head = d->k_head, a.ko_row = d->ko_row, a.ko_head = d->ko_head;
+    rotary_pairs(d, freq, a);
+    // vectors of 8 or 4 channels where pairs, rows, heads and pointers come in such
+    int64_t all = d->q_row | d->q_head | d->qo_row | d->qo_head | (with_k ? d->k_row | d->k_head | d->ko_row | d->ko_head : 0);
+    const auto fits = [&](int vec) {
+        const int64_t bytes = (int64_t) vec * (int64_t) elem;
+        return a.pairs % vec == 0 && d->head_dim % vec == 0 && all % vec == 0 && places % (uintptr_t) (bytes < 16 ? bytes : 16) == 0;
+    };
+    const int   vec = fits(8) ? 8 : fits(4) ? 4 : 1;
+    hipStream_t st  = resolve_stream(s);
+    if (d->dtype == VKHIP_DT_F16) vec == 8 ? rotary_launch<half_t, 8>(d, a, st) : vec == 4 ? rotary_launch<half_t, 4>(d, a, st) : rotary_launch<half_t, 1>(d, a, st);
+    else if (d->dtype == VKHIP_DT_BF16) vec == 8 ? rotary_launch<bf16_t, 8>(d, a, st) : vec == 4 ? rotary_launch<bf16_t, 4>(d, a, st) : rotary_launch<bf16_t, 1>(d, a, st);
+    else vec == 8 ? rotary_launch<float, 8>(d, a, st) : vec == 4 ? rotary_launch<float, 4>(d, a, st) : rotary_launch<float, 1>(d, a, st);
+    return check_launch("rotary");
+}
+
+} // extern "C"
