@@ -20,6 +20,7 @@ namespace vkhip {
         const int32_t *cu, *prefix;           // groups of neighbouring sequences, tokens that each shares
         int            groups, max_prefix;
         int            shared_span, shared_splits, shared_blocks; // tokens a workgroup, splits (the first of a row's), blocks of rows
+        int            wide;                                      // blocks of 1 or 2 times kWideRows rows; 0: of 32
     };
 
     // Tokens that group g shares, as every kernel counts them: whole pages.
@@ -58,5 +59,8 @@ namespace vkhip {
     }
 
     constexpr int kStep = 64; // tokens a wave takes at a time
+
+    constexpr int kWideRows = 128;
+    int kv_wide_run(const KvAttnArgs &a, bool bf16, hipStream_t s); // the prefixes, in blocks of `wide` kWideRows
 
 } // namespace vkhip

@@ -36,12 +36,12 @@ namespace vkhip {
         const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, nn = lane & 15;
         // heads, then sequences, then splits: workgroups go to the 8 XCDs in turn, and with splits first the later ones,
         // which short sequences do not have, would all meet on some of them
-        const int head = MODE == kPrefix ? blockIdx.x : blockIdx.x / a.blocks, split = blockIdx.z;
+        const int head = MODE == kPrefix ? blockIdx.x : blockIdx.x / a.blocks, split = MODE == kPrefix ? blockIdx.y : blockIdx.z;
         const int P   = a.c.page_tokens, D = a.c.head_dim;
         int       b = blockIdx.y, row0 = blockIdx.x % a.blocks * (16 * RT), rows = a.rows, len, t0, t1; // kPrefix: b is the group's first sequence
         if constexpr (MODE == kPrefix) {
             const auto    bound = [&](int i) { return clampi(a.cu[i], 0, a.c.batch); };
-            const SeqTile w = find_tile(blockIdx.y, a.groups, [&](int g) { return prefix_of(a, g) > 0 ? (max(0, bound(g + 1) - bound(g)) * a.rows + 16 * RT - 1) / (16 * RT) : 0; });
+            const SeqTile w = find_tile(blockIdx.z, a.groups, [&](int g) { return prefix_of(a, g) > 0 ? (max(0, bound(g + 1) - bound(g)) * a.rows + 16 * RT - 1) / (16 * RT) : 0; });
             if (w.b < 0) return;
             const int g = __builtin_amdgcn_readfirstlane(w.b);
             b = bound(g), rows = (bound(g + 1) - b) * a.rows, row0 = __builtin_amdgcn_readfirstlane(w.tile) * (16 * RT);
@@ -435,8 +435,8 @@ namespace vkhip {
     // Groups of sequences: the prefixes for all rows of a group, then every sequence's tail, then the join.
     template <typename T, int DJ, int RT, bool P32>
     static int kv_shared_launch(const KvAttnArgs &a, hipStream_t s) {
-        kv_attention_kernel<T, DJ, 2, P32, 4, kPrefix><<<dim3((unsigned) a.c.heads, (unsigned) a.shared_blocks, (unsigned) a.shared_splits), 256, 0, s>>>(a);
-        if (int rc = check_launch("kv_attention_shared prefix")) return rc;
+        if (!a.wide) kv_attention_kernel<T, DJ, 2, P32, 4, kPrefix><<<dim3((unsigned) a.c.heads, (unsigned) a.shared_splits, (unsigned) a.shared_blocks), 256, 0, s>>>(a);
+        if (int rc = a.wide ? kv_wide_run(a, !__is_same(T, half_t), s) : check_launch("kv_attention_shared prefix")) return rc;
         const dim3 grid((unsigned) (a.c.heads * a.blocks), (unsigned) a.c.batch, (unsigned) a.splits);
         if (a.waves == 2) kv_attention_kernel<T, DJ, RT, P32, 2, kTail><<<grid, 128, 0, s>>>(a);
         else kv_attention_kernel<T, DJ, RT, P32, 4, kTail><<<grid, 256, 0, s>>>(a);
@@ -476,11 +476,17 @@ namespace vkhip {
         a.max_len    = whole.max_len;
         a.groups     = p->groups;
         a.max_prefix = p->max_tokens > 0 && p->max_tokens < whole.max_len ? p->max_tokens : whole.max_len;
-        a.shared_blocks = (int) ((int64_t) c->batch * a.rows / 32 + p->groups);
-        const int64_t rounds = ceil_div(a.max_prefix > 0 ? a.max_prefix : 1, 4 * kStep), base = (int64_t) a.shared_blocks * c->kv_heads;
-        int64_t       splits = base >= 512 || base == 0 ? 1 : 512 / base;
+        const int64_t each = p->groups > 0 ? (int64_t) c->batch * a.rows / p->groups : 0; // rows of a group
+        a.wide            = each > 192 && a.c.row == 128 ? 2 : each > 32;
+        const int height  = a.wide ? a.wide * kWideRows : 32;
+        a.shared_blocks   = (int) ((int64_t) c->batch * a.rows / height + p->groups);
+        const int     round = (a.wide ? 1 : 4) * kStep; // tokens that a workgroup takes at a time
+        const int64_t rounds = ceil_div(a.max_prefix > 0 ? a.max_prefix : 1, round), full = ceil_div((int64_t) c->batch * a.rows, height);
+        const int64_t base = (full > p->groups ? full : p->groups) * c->kv_heads; // blocks, if groups fill theirs
+        const int64_t places = a.wide == 2 ? 256 : 512;
+        int64_t       splits = base >= places || base == 0 ? 1 : places / base;
         if (splits > rounds) splits = rounds;
-        a.shared_span   = (int) (ceil_div(rounds, splits) * 4 * kStep);
+        a.shared_span   = (int) (ceil_div(rounds, splits) * round);
         a.shared_splits = (int) ceil_div(a.max_prefix > 0 ? a.max_prefix : 1, a.shared_span);
         return a;
     }
