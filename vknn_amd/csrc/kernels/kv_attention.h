@@ -60,7 +60,7 @@ namespace vkhip {
 
     constexpr int kStep = 64; // tokens a wave takes at a time
 
-    constexpr int kWideRows = 128;
+    constexpr int kWideRows = 128, kWideUnits = 256; // tiles of 64 tokens, or of smaller pages, that a workgroup takes
     int kv_wide_run(const KvAttnArgs &a, bool bf16, hipStream_t s); // the prefixes, in blocks of `wide` kWideRows
 
 } // namespace vkhip

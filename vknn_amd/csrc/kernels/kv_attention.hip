@@ -432,6 +432,8 @@ namespace vkhip {
         return check_launch("kv_attention join");
     }
 
+    constexpr int kWideLeast = 4; // tiles of a workgroup, if the prefix has them
+
     // Groups of sequences: the prefixes for all rows of a group, then every sequence's tail, then the join.
     template <typename T, int DJ, int RT, bool P32>
     static int kv_shared_launch(const KvAttnArgs &a, hipStream_t s) {
@@ -451,7 +453,7 @@ namespace vkhip {
     template <typename T>
     static int kv_shared_run(const KvAttnArgs &a, hipStream_t s) {
         if (int rc = a.c.row == 64 ? kv_shared_tiles<T, 1>(a, s) : kv_shared_tiles<T, 2>(a, s)) return rc;
-        const bool wide = a.shared_splits + a.splits > 8;
+        const bool wide = a.shared_splits + a.splits > 32;
         const dim3 grid((unsigned) (wide ? a.rows : ceil_div(a.rows, 4)), (unsigned) a.c.heads, (unsigned) a.c.batch);
         if (wide) kv_join_kernel<T, 4, true><<<grid, 256, 0, s>>>(a);
         else kv_join_kernel<T, 1, true><<<grid, 256, 0, s>>>(a);
@@ -480,12 +482,16 @@ namespace vkhip {
         a.wide            = each > 192 && a.c.row == 128 ? 2 : each > 32;
         const int height  = a.wide ? a.wide * kWideRows : 32;
         a.shared_blocks   = (int) ((int64_t) c->batch * a.rows / height + p->groups);
+        const int wide_tiles = kWideUnits / (c->page_tokens == 32 ? 2 : 1);
+        if (a.wide && a.max_prefix > 4096 * wide_tiles * kStep) a.max_prefix = 4096 * wide_tiles * kStep; // 4096 splits; the rest with the tails
         const int     round = (a.wide ? 1 : 4) * kStep; // tokens that a workgroup takes at a time
         const int64_t rounds = ceil_div(a.max_prefix > 0 ? a.max_prefix : 1, round), full = ceil_div((int64_t) c->batch * a.rows, height);
         const int64_t base = (full > p->groups ? full : p->groups) * c->kv_heads; // blocks, if groups fill theirs
         const int64_t places = a.wide == 2 ? 256 : 512;
         int64_t       splits = base >= places || base == 0 ? 1 : places / base;
-        if (splits > rounds) splits = rounds;
+        const int64_t most = a.wide ? rounds / kWideLeast : rounds;
+        if (splits > most) splits = most > 0 ? most : 1;
+        if (a.wide && splits < ceil_div(rounds, wide_tiles)) splits = ceil_div(rounds, wide_tiles);
         a.shared_span   = (int) (ceil_div(rounds, splits) * round);
         a.shared_splits = (int) ceil_div(a.max_prefix > 0 ? a.max_prefix : 1, a.shared_span);
         return a;

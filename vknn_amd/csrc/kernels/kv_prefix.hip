@@ -26,7 +26,7 @@ namespace vkhip {
         return x;
     }
 
-    // NW: waves of a workgroup, 4 or, where a group has the rows, 8, which share what is converted.
+    // NW: waves of a workgroup, 4 (two of them a compute unit) or, where a group has the rows, 8, which share what is converted.
     template <typename T, int DP, bool P32, int NW>
     __global__ __launch_bounds__(NW * 64, 2) void kv_wide_kernel(KvAttnArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -58,10 +58,6 @@ namespace vkhip {
         // are smaller): a scalar load would make every wait for LDS a wait for memory.
         float vref = 0x1p-126f; // the scale that O is in units of: a power of two, no page's so far was larger
         float16v acc[DB];
-#pragma unroll
-        for (int d = 0; d < DB; ++d)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) acc[d][r] = 0.f;
         int   unit_page = -1; // this thread's unit
         float unit_ks = 0.f, unit_vs = 0.f;
         const auto page_of = [&](int tok) { // -1: no memory, or nothing there
@@ -84,14 +80,7 @@ namespace vkhip {
             __syncthreads();
 #pragma unroll
             for (int i = 0; i < 4; ++i) larger = fmaxf(larger, wave_vs[i]);
-            if (larger > vref) {
-                const float to = __uint_as_float((__float_as_uint(larger) + 0x7FFFFFu) & 0x7F800000u), less = vref / to;
-#pragma unroll
-                for (int d = 0; d < DB; ++d)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) acc[d][r] *= less;
-                vref = to;
-            }
+            vref = fmaxf(__uint_as_float((__float_as_uint(larger) + 0x7FFFFFu) & 0x7F800000u), 0x1p-126f);
             // a page far below the largest has a unit of its own, a power of two under vref that O takes for its tile; a page
             // of zeros or of a scale that is no number is dealt with there too
             const bool none = vs == 0.f, lost = !(vs <= vref), plain = none || lost || vs >= vref * 0x1p-8f;
@@ -101,41 +90,52 @@ namespace vkhip {
             unit_id[tid] = unit_page < 0 ? -1 : none || lost || !plain || !(ks > 0.f) ? unit_page | 0x40000000 : unit_page;
             unit[tid]    = float4v {ks, none ? 0.f : lost ? __builtin_nanf("") : under, __builtin_amdgcn_logf(ratio), 1.f / ratio};
         };
-        // the names of a tile's pages, the same in every lane; from: the first token of the units in LDS
-        const auto names = [&](int tok, int from) {
-            const int i = (tok - from) / UNIT;
-            return make_int2(__builtin_amdgcn_readfirstlane(unit_id[i]), P32 ? __builtin_amdgcn_readfirstlane(unit_id[i + 1]) : 0);
+        // the names of the pages of tile i of those in LDS, the same in every lane
+        const auto names = [&](int i) {
+            return make_int2(__builtin_amdgcn_readfirstlane(unit_id[i * (kStep / UNIT)]), P32 ? __builtin_amdgcn_readfirstlane(unit_id[i * 2 + 1]) : 0);
         };
+        const auto page = [](int id) { return id < 0 ? 0 : id & 0x3FFFFFFF; }; // one without memory is read elsewhere and masked
+        const auto odd_page = [](int2 n) { return n.x < 0 || n.x >= 0x40000000 || (P32 && (n.y < 0 || n.y >= 0x40000000)); };
 
         const auto first_names = [&](int tok) { return make_int2(page_of(tok), P32 ? page_of(tok + UNIT) : 0); }; // before they are in LDS
         // a tile's bytes: piece p of K is token p / (DP / 16), 16 channels from p % (DP / 16) on; of V channel p / 4, 16 tokens
         // from p % 4 on
         tk_u32x4      kr[LOADS], vr[LOADS];
         const int64_t page_bytes = (int64_t) P * DP;
-        const auto    fetch = [&](int tok, int2 n) __attribute__((always_inline)) {
-            const unsigned char *kp[2], *vp[2];
+        const auto    fetch_k = [&](int tok, int2 n, tk_u32x4 (&to)[LOADS]) __attribute__((always_inline)) {
+            const unsigned char *kp[2];
 #pragma unroll
-            for (int u = 0; u < (P32 ? 2 : 1); ++u) {
-                const int     id = u ? n.y : n.x, at = P32 ? 0 : tok & (P - 1);
-                const int64_t hp = (int64_t) (id < 0 ? 0 : id & 0x3FFFFFFF) * a.c.heads + head;
-                kp[u] = a.c.k + hp * page_bytes + at * DP, vp[u] = a.c.v + hp * page_bytes + at;
-            }
+            for (int u = 0; u < (P32 ? 2 : 1); ++u) kp[u] = a.c.k + ((int64_t) page(u ? n.y : n.x) * a.c.heads + head) * page_bytes + (P32 ? 0 : tok & (P - 1)) * DP;
 #pragma unroll
             for (int i = 0; i < LOADS; ++i) {
-                const int p = i * (NW * 64) + tid, kt = p / (DP / 16), kc = p % (DP / 16) * 16, vc = p / 4, vt = p % 4 * 16;
-                if constexpr (P32) {
-                    kr[i] = *reinterpret_cast<const tk_u32x4 *>((kt >> 5 ? kp[1] : kp[0]) + (unsigned) ((kt & 31) * DP + kc));
-                    vr[i] = *reinterpret_cast<const tk_u32x4 *>((vt >> 5 ? vp[1] : vp[0]) + (unsigned) (vc * P + (vt & 31)));
-                } else {
-                    kr[i] = *reinterpret_cast<const tk_u32x4 *>(kp[0] + (unsigned) (kt * DP + kc));
-                    vr[i] = *reinterpret_cast<const tk_u32x4 *>(vp[0] + (unsigned) (vc * P + vt));
-                }
+                const int p = i * (NW * 64) + tid, kt = p / (DP / 16), kc = p % (DP / 16) * 16;
+                if constexpr (P32) to[i] = *reinterpret_cast<const tk_u32x4 *>((kt >> 5 ? kp[1] : kp[0]) + (unsigned) ((kt & 31) * DP + kc));
+                else to[i] = *reinterpret_cast<const tk_u32x4 *>(kp[0] + (unsigned) (kt * DP + kc));
+            }
+        };
+        const auto fetch_v = [&](int tok, int2 n) __attribute__((always_inline)) {
+            const unsigned char *vp[2];
+#pragma unroll
+            for (int u = 0; u < (P32 ? 2 : 1); ++u) vp[u] = a.c.v + ((int64_t) page(u ? n.y : n.x) * a.c.heads + head) * page_bytes + (P32 ? 0 : tok & (P - 1));
+#pragma unroll
+            for (int i = 0; i < LOADS; ++i) {
+                const int p = i * (NW * 64) + tid, vc = p / 4, vt = p % 4 * 16;
+                if constexpr (P32) vr[i] = *reinterpret_cast<const tk_u32x4 *>((vt >> 5 ? vp[1] : vp[0]) + (unsigned) (vc * P + (vt & 31)));
+                else vr[i] = *reinterpret_cast<const tk_u32x4 *>(vp[0] + (unsigned) (vc * P + vt));
             }
         };
         // the first tile's bytes and the pages' scales are on their way while the queries are
-        int from = t0;
-        ask(from);
-        fetch(from, first_names(from));
+        // (K of a tile is needed one round before its V)
+        const int from = t0;
+        tk_u32x4 k0[LOADS];
+        const auto begin = [&]() __attribute__((always_inline)) {
+            ask(from);
+            const int2 n0 = first_names(from), n1 = first_names(from + kStep);
+            fetch_k(from, n0, k0);
+            fetch_k(from + kStep, n1, kr);
+            fetch_v(from, n0);
+        };
+        begin();
 
         int        limit = t1; // tokens below it are seen
         half8      qf[KS];
@@ -183,32 +183,67 @@ namespace vkhip {
         // 16-byte pieces are permuted by their row so that the rows of a read meet no bank twice
         const auto k_at = [](int token, int piece) { return token * ROW + ((piece ^ (DP == 128 ? token & 15 : token >> 1 & 7)) << 4); };
         const auto v_at = [](int channel, int piece) { return channel * (kStep * 2) + ((piece ^ (channel >> 1 & 7)) << 4); };
-        unsigned   ka[KS], va[4]; // where a lane's operands lie
+        // where a lane's first operands lie, and this thread's pieces go: c pieces on is an xor of bits from 5 on
+        const unsigned ka = k_at(col, h), va = v_at(col, h), kw = k_at(tid / (DP / 16), tid % (DP / 16) * 2), vw = v_at(tid / 4, tid % 4 * 2);
+        const auto stage_k = [&](unsigned char *sk, tk_u32x4 (&x)[LOADS]) __attribute__((always_inline)) {
 #pragma unroll
-        for (int c = 0; c < KS; ++c) ka[c] = k_at(col, 2 * c + h);
+            for (int i = 0; i < LOADS; ++i) { // 32 tokens on: rows of the same permutation
+                *reinterpret_cast<half8 *>(sk + kw + i * 8192)        = i8_to_h8<0>(x[i][0], x[i][1]);
+                *reinterpret_cast<half8 *>(sk + (kw ^ 16) + i * 8192) = i8_to_h8<0>(x[i][2], x[i][3]);
+            }
+        };
+        const auto stage_v = [&](unsigned char *sv) __attribute__((always_inline)) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) va[k] = v_at(col, 2 * k + h);
-        const auto stage = [&](auto odd_c) __attribute__((always_inline)) {
-            unsigned char *sk = sm_k[decltype(odd_c)::value], *sv = sm_v[decltype(odd_c)::value];
-            const int      kt = tid / (DP / 16), kc = tid % (DP / 16) * 2, vc = tid / 4, vt = tid % 4 * 2;
-            const unsigned kw[2] = {(unsigned) k_at(kt, kc), (unsigned) k_at(kt, kc + 1)}, vw[2] = {(unsigned) v_at(vc, vt), (unsigned) v_at(vc, vt + 1)};
-#pragma unroll
-            for (int i = 0; i < LOADS; ++i) { // 256 pieces on are 32 tokens or 64 channels: rows of the same permutation
-                *reinterpret_cast<half8 *>(sk + kw[0] + i * 8192) = i8_to_h8<0>(kr[i][0], kr[i][1]);
-                *reinterpret_cast<half8 *>(sk + kw[1] + i * 8192) = i8_to_h8<0>(kr[i][2], kr[i][3]);
-                *reinterpret_cast<half8 *>(sv + vw[0] + i * 8192) = i8_to_h8<kWeightBits>(vr[i][0], vr[i][2]);
-                *reinterpret_cast<half8 *>(sv + vw[1] + i * 8192) = i8_to_h8<kWeightBits>(vr[i][1], vr[i][3]);
+            for (int i = 0; i < LOADS; ++i) { // 64 channels on
+                *reinterpret_cast<half8 *>(sv + vw + i * 8192)        = i8_to_h8<kWeightBits>(vr[i][0], vr[i][2]);
+                *reinterpret_cast<half8 *>(sv + (vw ^ 16) + i * 8192) = i8_to_h8<kWeightBits>(vr[i][1], vr[i][3]);
             }
         };
 
-        float m = -__builtin_inff(), l = 0.f;
-        bool  far = false;
+        float    m = -__builtin_inff(), l = 0.f;
+        bool     far = false;
+        float16v s[2];
+        half8    pf[4];
 
-        const auto tile = [&](int tok, int from, int2 n, auto odd_c, auto other_c) __attribute__((always_inline)) {
-            const unsigned char *sk = sm_k[decltype(odd_c)::value], *sv = sm_v[decltype(odd_c)::value];
-            const int            ui = (tok - from) / UNIT;
-            const float4v        u0 = unit[ui], u1 = unit[P32 ? ui + 1 : ui];
-            float16v             s[2];
+        // Round i of a wave: the products O += V P of tile i - 1 and S = K Q of tile i, beside them K of tile i + 1 and V of
+        // tile i into LDS, whose places tiles i - 1 and i - 2 have left; then the exponentials of tile i, and a barrier.
+        const auto in_units = [&](float by) __attribute__((always_inline)) {
+            __asm__ volatile("" : "+v"(by));
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) acc[d][r] *= by;
+        };
+        const auto values = [&](int i, int2 n, int place) __attribute__((always_inline)) {
+            const unsigned at = va + place * (kStep * 2 * DP);
+            const bool     odd = odd_page(n);
+            float          of = 1.f;
+            const auto     product = [&](int k) __attribute__((always_inline)) {
+#pragma unroll
+                for (int d = 0; d < DB; ++d)
+                    acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const half8 *>(sm_v[0] + (at ^ k << 5) + d * (32 * kStep * 2)), pf[k], acc[d], 0, 0, 0);
+            };
+            const auto none = [&](int k) __attribute__((always_inline)) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) pf[k][j] = (half_t) 0.f;
+            };
+            if (odd) {
+                const float u0 = unit[i * (kStep / UNIT)][1], u1 = unit[P32 ? i * 2 + 1 : i][1], of0 = u0 > 0.f ? u0 : 1.f;
+                of = u1 > 0.f ? u1 : 1.f;
+                if (u0 == 0.f) none(0), none(1); // whatever the bytes of a page of zeros are
+                if (u1 == 0.f) none(2), none(3);
+                in_units(of0);
+                if (P32 && of0 != of) { // the first page by itself
+                    product(0), product(1), none(0), none(1);
+                    in_units(of / of0);
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) product(k);
+            return 1.f / of;
+        };
+        const auto scores = [&](int place) __attribute__((always_inline)) {
+            const unsigned at = ka + place * (kStep * ROW);
 #pragma unroll
             for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
@@ -217,28 +252,37 @@ namespace vkhip {
             for (int c = 0; c < KS; ++c)
 #pragma unroll
                 for (int kk = 0; kk < 2; ++kk)
-                    s[kk] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const half8 *>(sk + ka[c] + kk * 32 * ROW), qf[c], s[kk], 0, 0, 0);
-            // reads stay AHEAD operands in front of their products
-            __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 1);
+                    s[kk] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const half8 *>(sm_k[0] + (at ^ c << 5) + kk * 32 * ROW), qf[c], s[kk], 0, 0, 0);
+        };
+        // the order of the products and what is beside them: reads AHEAD of their products, and after each a read, a few
+        // conversions, every other time a write
+        const auto beside = [&](auto products) __attribute__((always_inline)) {
+            constexpr int N = decltype(products)::value, EACH = (80 * LOADS / 2 + N - 1) / N + 1;
+            __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0);
 #pragma unroll
-            for (int i = 0; i < 2 * KS; ++i) {
-                __builtin_amdgcn_sched_group_barrier(0x008, 1, 1);
-                __builtin_amdgcn_sched_group_barrier(0x100, 1, 1);
+            for (int i = 0; i < N; ++i) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x002, EACH, 0);
+                if (i & 1) __builtin_amdgcn_sched_group_barrier(0x200, 1, 0);
             }
-            const bool odd = n.x < 0 || n.x >= 0x40000000 || (P32 && (n.y < 0 || n.y >= 0x40000000));
-            float      f[2] = {u0[0] * c2, u1[0] * c2};
-            if (odd || tok + kStep > seen_by_all) {
+        };
+        const auto weights = [&](int i, int2 n) __attribute__((always_inline)) {
+            const int     tok = from + i * kStep;
+            const float4v u0 = unit[i * (kStep / UNIT)], u1 = unit[P32 ? i * 2 + 1 : i];
+            float         f[2] = {u0[0] * c2, u1[0] * c2};
+            if (odd_page(n) || tok + kStep > seen_by_all) {
                 int upto = limit;
                 __asm__ volatile("" : "+v"(upto), "+v"(f[0]), "+v"(f[1])); // a branch, not selects in every tile
                 // what is not seen first, since its product with a scale of zero would be NaN; what is seen of a page whose
                 // value scale is no number is none
 #pragma unroll
                 for (int kk = 0; kk < 2; ++kk) {
-                    const bool  none = (P32 && kk ? n.y : n.x) < 0;
+                    const int   seen = (P32 && kk ? n.y : n.x) < 0 ? 0 : upto - tok - 32 * kk - 4 * h; // of the block's tokens, from 4 h on
                     const float poison = (kk ? u1 : u0)[1] * 0.f;
 #pragma unroll
                     for (int r = 0; r < 16; ++r)
-                        s[kk][r] = none || tok + 32 * kk + 8 * (r >> 2) + 4 * h + (r & 3) >= upto ? -__builtin_inff() : __builtin_fmaf(s[kk][r], f[kk], poison);
+                        s[kk][r] = 8 * (r >> 2) + (r & 3) >= seen ? -__builtin_inff() : __builtin_fmaf(s[kk][r], f[kk], poison);
                     f[kk] = 1.f;
                 }
             }
@@ -274,7 +318,6 @@ namespace vkhip {
                 }
                 base = 0.f;
             }
-            half8 pf[4];
 #pragma unroll
             for (int kk = 0; kk < 2; ++kk) {
                 const float away = base - (kk ? u1 : u0)[2];
@@ -290,89 +333,73 @@ namespace vkhip {
                 }
                 l = __builtin_fmaf(sum, (kk ? u1 : u0)[3], l);
             }
-            const auto v_frag = [&](int d, int k) { return *reinterpret_cast<const half8 *>(sv + va[k] + d * (32 * kStep * 2)); };
-            const auto in_units = [&](float by) __attribute__((always_inline)) {
-                __asm__ volatile("" : "+v"(by));
-#pragma unroll
-                for (int d = 0; d < DB; ++d)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) acc[d][r] *= by;
-            };
-            const float of0 = u0[1] > 0.f ? u0[1] : 1.f, of1 = u1[1] > 0.f ? u1[1] : 1.f;
-            if (odd) {
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    if ((k >> 1 ? u1 : u0)[1] == 0.f)
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) pf[k][j] = (half_t) 0.f; // whatever the bytes of a page of zeros are
-                in_units(of0);
-            }
-            // the next tile's bytes become halves beside the products, or nobody's do
-            stage(other_c);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                if (P32 && k == 2 && odd) in_units(of1 / of0);
-#pragma unroll
-                for (int d = 0; d < DB; ++d) acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v_frag(d, k), pf[k], acc[d], 0, 0, 0);
-            }
-            if constexpr (!P32) {
-                __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0);
-#pragma unroll
-                for (int i = 0; i < 4 * DB; ++i) {
-                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0); // a product, a read, conversions, a write
-                    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-                    __builtin_amdgcn_sched_group_barrier(0x002, 7, 0);
-                    if (i & 1) __builtin_amdgcn_sched_group_barrier(0x200, 1, 0);
-                }
-            }
-            if (odd) in_units(1.f / of1);
         };
-
-        const std::integral_constant<int, 0> even;
-        const std::integral_constant<int, 1> odd;
-        for (;;) {
+        // loads stay under way across these
+        const auto barrier = [] __attribute__((always_inline)) {
+            __builtin_amdgcn_s_waitcnt(0xC07F); // lgkmcnt(0): this wave's writes
+            __asm__ volatile("s_barrier" ::: "memory");
+        };
+        {
             settle();
-            stage(even);
+            stage_k(sm_k[0], k0);
             __syncthreads();
-            const int end = min(t1, from + 256 * UNIT);
-            int2      n0 = names(from, from), n1 = n0;
-            for (int tok = from; tok < end; tok += 2 * kStep) {
-                const bool second = tok + kStep < end, third = tok + 2 * kStep < end;
-                if (second) {
-                    n1 = names(tok + kStep, from);
-                    fetch(tok + kStep, n1);
-                }
-                tile(tok, from, n0, even, odd);
-                __syncthreads();
-                if (!second) break;
-                if (third) {
-                    n0 = names(tok + 2 * kStep, from);
-                    fetch(tok + 2 * kStep, n0);
-                }
-                tile(tok + kStep, from, n1, odd, even);
-                __syncthreads();
+            const int tiles = (t1 - t0 + 2 * kStep - 1) / (2 * kStep) * 2; // an even number: one without pages behind an odd one
+            int2      before, now = names(0), next = names(min(1, tiles - 1)); // tiles i - 1, i, i + 1
+            const auto ahead = [&](int i) __attribute__((always_inline)) {  // K of tile i + 2, V of tile i + 1; the last ones again behind them
+                const int v = min(i + 1, tiles - 1), k = min(i + 2, tiles - 1);
+                before = now, now = next, next = names(k);
+                fetch_v(from + v * kStep, now);
+                fetch_k(from + k * kStep, next, kr);
+            };
+            scores(0);
+            stage_k(sm_k[1], kr), stage_v(sm_v[0]);
+            ahead(0);
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) acc[d][r] = 0.f;
+            const auto round = [&](int i, auto odd_c) __attribute__((always_inline)) {
+                constexpr int ODD = decltype(odd_c)::value;
+                weights(i, before);
+                barrier();
+                const float back = values(i, before, ODD);
+                scores(ODD ^ 1); // behind the last tile its scores are formed again, for nobody
+                stage_k(sm_k[ODD], kr), stage_v(sm_v[ODD ^ 1]);
+                beside(std::integral_constant<int, 4 * DB + 2 * KS>());
+                if (odd_page(before)) in_units(back);
+                ahead(i + 1);
+            };
+#pragma unroll 1
+            for (int i = 0; i < tiles; i += 2) {
+                round(i, std::integral_constant<int, 0>());
+                round(i + 1, std::integral_constant<int, 1>());
             }
-            from += 256 * UNIT;
-            if (from >= t1) break;
-            ask(from);
-            fetch(from, first_names(from));
         }
 
         l += __shfl_xor(l, 32);
         l *= 1.f / (1 << kWeightBits); // the products have it in their values
         const int3 me = row_of(again(lane));
-        const int  seq = me.x, r0 = me.y;
-        if (!me.z) return;
-        const int64_t at = (((int64_t) seq * a.c.heads + head) * a.rows + r0) * (a.shared_splits + a.splits) + split;
-        float        *o = a.part_o + at * D;
+        const int  at = me.z ? (int) ((((int64_t) me.x * a.c.heads + head) * a.rows + me.y) * (a.shared_splits + a.splits) + split) : -1; // fewer than 2^31 parts
+        if (h == 0 && at >= 0) *reinterpret_cast<float2 *>(a.part_s + (int64_t) at * 2) = make_float2(m, l);
+        // through LDS, 64 channels at a time, so that rows leave in whole lines (4 of 11 us for a call of 4 tiles otherwise)
+        __syncthreads();
+        unsigned char *own = (wave < NW / 2 ? sm_k[0] : sm_v[0]) + wave % (NW / 2) * 8192;
 #pragma unroll
-        for (int d = 0; d < DB; ++d)
+        for (int e = 0; e < DP / 64; ++e) {
 #pragma unroll
-            for (int r = 0; r < 16; r += 4) {
-                const int ch = 32 * d + 2 * r + 4 * h;
-                if (ch < D) *reinterpret_cast<float4v *>(o + ch) = float4v {acc[d][r] * vref, acc[d][r + 1] * vref, acc[d][r + 2] * vref, acc[d][r + 3] * vref};
+            for (int d = 2 * e; d < 2 * e + 2; ++d)
+#pragma unroll
+                for (int r = 0; r < 16; r += 4) // channels 32 d + 2 r + 4 h .. + 3
+                    *reinterpret_cast<float4v *>(own + col * 256 + ((8 * (d & 1) + r / 2 + h ^ (col & 15)) << 4)) =
+                        float4v {acc[d][r] * vref, acc[d][r + 1] * vref, acc[d][r + 2] * vref, acc[d][r + 3] * vref};
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int     row = 4 * i + (lane >> 4), piece = lane & 15, ch = 64 * e + 4 * piece;
+                const float4v x = *reinterpret_cast<const float4v *>(own + row * 256 + ((piece ^ (row & 15)) << 4));
+                const int     to = __shfl(at, row);
+                if (to >= 0 && ch < D) *reinterpret_cast<float4v *>(a.part_o + (int64_t) to * D + ch) = x;
             }
-        if (h == 0) *reinterpret_cast<float2 *>(a.part_s + at * 2) = make_float2(m, l);
+        }
 #endif
     }
 
