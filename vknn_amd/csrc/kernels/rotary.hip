@@ -10,14 +10,15 @@
 
 namespace vkhip {
 
-    constexpr int kRotaryPairs = 128;
+    constexpr int     kRotaryPairs = 128;
+    constexpr int64_t kRotaryPast = (int64_t) 64 << 20; // bytes of rows from which they pass the caches
 
     struct RotaryArgs {
         const void    *q, *k;
         void          *qo, *ko;
         const int32_t *pos;
         int            rows, q_heads, heads, head_dim, pairs; // heads: of q and k together
-        int            units, turned;   // of a head: pieces of VEC pairs or 2 VEC copied channels; the first `turned` are pairs
+        int            units, turned;   // pieces of a head; the first `turned` are pairs, the others copied
         int            slots, per;      // threads that share a row's unit, heads of each
         int            block_rows;      // rows of a workgroup, where several fit
         int64_t        pos_axis, q_row, q_head, k_row, k_head, qo_row, qo_head, ko_row, ko_head;
@@ -43,30 +44,43 @@ namespace vkhip {
         if (quarter & 2) s = -s;
     }
 
-    // A thread takes one unit of a row in several heads: VEC pairs, which are two vectors of VEC channels (a half of the
-    // rotated channels apart, or side by side), or 2 VEC channels behind them that are copied.
-    template <typename T, int VEC, bool NEAR>
+    template <bool PAST, typename V>
+    __device__ __forceinline__ V rotary_load(const void *p) {
+        if constexpr (PAST) return __builtin_nontemporal_load(reinterpret_cast<const V *>(p));
+        else return *reinterpret_cast<const V *>(p);
+    }
+    template <bool PAST, typename V>
+    __device__ __forceinline__ void rotary_store(V v, void *p) {
+        if constexpr (PAST) __builtin_nontemporal_store(v, reinterpret_cast<V *>(p));
+        else *reinterpret_cast<V *>(p) = v;
+    }
+
+    // A thread takes one unit of a row in several heads. A unit of halves is VEC pairs, two vectors of VEC channels that lie
+    // half of the rotated channels apart; of neighbours VEC channels, or a pair; behind the rotated channels as many that
+    // are copied. PAST: rows pass the caches.
+    template <typename T, int VEC, bool NEAR, bool PAST>
     __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
         typedef T V __attribute__((ext_vector_type(VEC)));
-        const int     each = a.units * a.slots;
-        const int64_t block = (int64_t) blockIdx.y * gridDim.x + blockIdx.x;
-        const int     r = (int) threadIdx.x / each;
-        const int64_t row = block * a.block_rows + r;
+        constexpr int  PAIRS = NEAR ? (VEC > 1 ? VEC / 2 : 1) : VEC;
+        constexpr bool TWO   = !NEAR || VEC == 1; // vectors of a unit
+        const int      each  = a.units * a.slots;
+        const int64_t  block = (int64_t) blockIdx.y * gridDim.x + blockIdx.x;
+        const int      r = (int) threadIdx.x / each;
+        const int64_t  row = block * a.block_rows + r;
         if (r >= a.block_rows || row >= a.rows) return;
         for (int i = (int) threadIdx.x - r * each; i < each; i += 256) {
             const int  unit = i % a.units, h0 = i / a.units * a.per, h1 = min(a.heads, h0 + a.per);
             const bool turned = unit < a.turned;
-            const int  copied = 2 * a.pairs + (unit - a.turned) * 2 * VEC; // first channel of a copied unit
-            const int  c0 = turned ? (NEAR ? unit * 2 * VEC : unit * VEC) : copied, c1 = turned && !NEAR ? a.pairs + unit * VEC : c0 + VEC;
-            const bool second = c1 < a.head_dim;
-            float      c[VEC], s[VEC];
+            const int  c0 = turned && !NEAR ? unit * VEC : unit * 2 * PAIRS, c1 = turned && !NEAR ? a.pairs + unit * VEC : c0 + VEC;
+            const bool second = TWO && c1 < a.head_dim;
+            float      c[PAIRS], s[PAIRS];
             if (turned)
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) {
-                    const int p = unit * VEC + j;
+                for (int j = 0; j < PAIRS; ++j) {
+                    const int p = unit * PAIRS + j;
                     turn_of(a.freq[p], a.pos[a.axis[p] * a.pos_axis + row], c[j], s[j]);
                 }
-#pragma unroll 2
+#pragma unroll 4
             for (int h = h0; h < h1; ++h) {
                 const bool    key = h >= a.q_heads;
                 const int     n = key ? h - a.q_heads : h;
@@ -74,30 +88,18 @@ namespace vkhip {
                 const int64_t to = key ? row * a.ko_row + n * a.ko_head : row * a.qo_row + n * a.qo_head;
                 const T      *x = (const T *) (key ? a.k : a.q) + from;
                 T            *y = (T *) (key ? a.ko : a.qo) + to;
-                V             u = *reinterpret_cast<const V *>(x + c0), w = u;
-                if (second) w = *reinterpret_cast<const V *>(x + c1);
-                if (turned) {
-                    if constexpr (NEAR) {
-                        float v[2 * VEC];
+                V             u = rotary_load<PAST, V>(x + c0), w = u;
+                if (second) w = rotary_load<PAST, V>(x + c1);
+                if (turned)
 #pragma unroll
-                        for (int j = 0; j < VEC; ++j) v[j] = (float) u[j], v[VEC + j] = (float) w[j];
-#pragma unroll
-                        for (int j = 0; j < VEC; ++j) {
-                            const float p = v[2 * j] * c[j] - v[2 * j + 1] * s[j], q = v[2 * j + 1] * c[j] + v[2 * j] * s[j];
-                            v[2 * j] = p, v[2 * j + 1] = q;
-                        }
-#pragma unroll
-                        for (int j = 0; j < VEC; ++j) u[j] = (T) v[j], w[j] = (T) v[VEC + j];
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < VEC; ++j) {
-                            const float p = (float) u[j], q = (float) w[j];
-                            u[j] = (T) (p * c[j] - q * s[j]), w[j] = (T) (q * c[j] + p * s[j]);
-                        }
+                    for (int j = 0; j < PAIRS; ++j) {
+                        const float p = (float) (TWO ? u[j] : u[2 * j]), q = (float) (TWO ? w[j] : u[2 * j + (VEC > 1)]);
+                        const T     p1 = (T) (p * c[j] - q * s[j]), q1 = (T) (q * c[j] + p * s[j]);
+                        if constexpr (TWO) u[j] = p1, w[j] = q1;
+                        else u[2 * j] = p1, u[2 * j + (VEC > 1)] = q1;
                     }
-                }
-                *reinterpret_cast<V *>(y + c0) = u;
-                if (second) *reinterpret_cast<V *>(y + c1) = w;
+                rotary_store<PAST>(u, y + c0);
+                if (second) rotary_store<PAST>(w, y + c1);
             }
         }
     }
@@ -115,11 +117,15 @@ namespace vkhip {
         for (int p = 0; p < a.pairs; ++p) {
             while (had[axis] == d->sections[axis]) axis = (axis + 1) % d->axes;
             const int   of = d->spectra ? axis : 0;
-            const long double f = freq ? (long double) freq[p] : now[of], n = floorl(f / turn);
+            const long double f = freq ? (long double) freq[p] : now[of];
             now[of] *= step[of];
-            long double t = (fmal(-n, turn, f) - n * rest) / turn;
-            t -= floorl(t); // rounding may leave it outside 0 .. 1
-            const long double whole = roundl(t * two64);
+            long double t = f * (1.0L / turn);
+            if (f < 0 || f >= turn) {
+                const long double n = floorl(f / turn);
+                t = (fmal(-n, turn, f) - n * rest) / turn;
+                t -= floorl(t); // rounding may leave it outside 0 .. 1
+            }
+            const long double whole = t * two64 + 0.5L;
             a.freq[p] = whole >= two64 ? 0 : (uint64_t) whole;
             a.axis[p] = (uint8_t) axis;
             ++had[axis];
@@ -160,18 +166,21 @@ namespace vkhip {
 
     template <typename T, int VEC>
     static void rotary_launch(const vkhip_rotary_desc *d, RotaryArgs &a, hipStream_t s) {
-        a.turned = a.pairs / VEC;
-        a.units  = a.turned + (int) ceil_div(d->head_dim - d->rotary_dim, 2 * VEC);
-        // Heads of a thread: as many as leave the card full, at most 8.
+        const int pairs = d->neighbours ? (VEC > 1 ? VEC / 2 : 1) : VEC; // of a unit
+        a.turned = a.pairs / pairs;
+        a.units  = a.turned + (int) ceil_div(d->head_dim - d->rotary_dim, 2 * pairs);
+        // Heads of a thread: as many as leave the card full, at most 4 (50176 rows of 40 heads of 128, bf16, 2, 4, 8, 10 of them: 201,
+        // 193, 197, 206 us; neighbours 210, 187, 181, 186).
         const int64_t items = (int64_t) a.rows * a.heads * a.units, fill = 256 * 2048;
-        a.per   = (int) (items / fill < 1 ? 1 : items / fill > 8 ? 8 : items / fill);
+        a.per   = (int) (items / fill < 1 ? 1 : items / fill > 4 ? 4 : items / fill);
         a.slots = (int) ceil_div(a.heads, a.per);
         const int each = a.units * a.slots;
         a.block_rows   = each >= 256 ? 1 : 256 / each;
         const int64_t blocks = ceil_div(a.rows, a.block_rows), layers = ceil_div(blocks, 0xFFFFFF);
         const dim3    grid((unsigned) ceil_div(blocks, layers), (unsigned) layers);
-        if (d->neighbours) rotary_kernel<T, VEC, true><<<grid, 256, 0, s>>>(a);
-        else rotary_kernel<T, VEC, false><<<grid, 256, 0, s>>>(a);
+        const bool past = (int64_t) a.rows * a.heads * d->head_dim * (int64_t) sizeof(T) >= kRotaryPast;
+        if (d->neighbours) past ? rotary_kernel<T, VEC, true, true><<<grid, 256, 0, s>>>(a) : rotary_kernel<T, VEC, true, false><<<grid, 256, 0, s>>>(a);
+        else past ? rotary_kernel<T, VEC, false, true><<<grid, 256, 0, s>>>(a) : rotary_kernel<T, VEC, false, false><<<grid, 256, 0, s>>>(a);
     }
 
 } // namespace vkhip
@@ -204,7 +213,7 @@ int vkhip_rotary(const vkhip_rotary_desc *d, const int32_t *pos, const double *f
     int64_t all = d->q_row | d->q_head | d->qo_row | d->qo_head | (with_k ? d->k_row | d->k_head | d->ko_row | d->ko_head : 0);
     const auto fits = [&](int vec) {
         const int64_t bytes = (int64_t) vec * (int64_t) elem;
-        return a.pairs % vec == 0 && d->head_dim % vec == 0 && all % vec == 0 && places % (uintptr_t) (bytes < 16 ? bytes : 16) == 0;
+        return (d->neighbours ? d->rotary_dim : a.pairs) % vec == 0 && d->head_dim % vec == 0 && all % vec == 0 && places % (uintptr_t) (bytes < 16 ? bytes : 16) == 0;
     };
     const int   vec = fits(8) ? 8 : fits(4) ? 4 : 1;
     hipStream_t st  = resolve_stream(s);
