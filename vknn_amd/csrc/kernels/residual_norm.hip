@@ -33,8 +33,8 @@ namespace vkhip {
         return v;
     }
 
-    // GT threads a row, N vectors of VEC values each, vector i of thread t at (i GT + t) VEC.
-    template <typename T, int VEC, int N, int GT>
+    // GT threads a row, N vectors of VEC values each, vector i of thread t at (i GT + t) VEC. PAST: rows pass the caches.
+    template <typename T, int VEC, int N, int GT, bool PAST>
     __global__ __launch_bounds__(GT < 256 ? 256 : GT) void residual_norm_kernel(NormArgs a) {
         typedef T     V __attribute__((ext_vector_type(VEC)));
         typedef float F __attribute__((ext_vector_type(VEC)));
@@ -51,6 +51,15 @@ namespace vkhip {
         const auto    load = [&](const void *p, int64_t offset, int i) {
             const V v = *reinterpret_cast<const V *>((const T *) p + offset + at(i));
             return __builtin_convertvector(v, F);
+        };
+        const auto load_row = [&](const void *p, int64_t offset, int i) {
+            if constexpr (PAST) return __builtin_convertvector(__builtin_nontemporal_load(reinterpret_cast<const V *>((const T *) p + offset + at(i))), F);
+            else return load(p, offset, i);
+        };
+        const auto store_row = [&](void *p, int64_t offset, int i) {
+            const V v = __builtin_convertvector(z[i], V);
+            if constexpr (PAST) __builtin_nontemporal_store(v, reinterpret_cast<V *>((T *) p + offset + at(i)));
+            else *reinterpret_cast<V *>((T *) p + offset + at(i)) = v;
         };
         const auto norm = [&](int kind, float eps, const float *w, const float *b) {
             if (kind == VKHIP_NORM_NONE) return;
@@ -93,10 +102,10 @@ namespace vkhip {
             for (int j = 0; j < VEC; ++j) z[i][j] = 0.f, r[i][j] = 0.f;
 #pragma unroll
         for (int i = 0; i < N; ++i)
-            if (a.x && in(i)) z[i] = load(a.x, row * a.x_row, i);
+            if (a.x && in(i)) z[i] = load_row(a.x, row * a.x_row, i);
 #pragma unroll
         for (int i = 0; i < N; ++i)
-            if (a.r && in(i)) r[i] = load(a.r, row * a.r_row, i);
+            if (a.r && in(i)) r[i] = load_row(a.r, row * a.r_row, i);
         if (a.x) {
             norm(a.post, a.post_eps, a.post_w, a.post_b);
 #pragma unroll
@@ -115,7 +124,7 @@ namespace vkhip {
         if (a.h)
 #pragma unroll
             for (int i = 0; i < N; ++i)
-                if (in(i)) *reinterpret_cast<V *>((T *) a.h + row * a.h_row + at(i)) = __builtin_convertvector(z[i], V);
+                if (in(i)) store_row(a.h, row * a.h_row, i);
         if (!a.y) return;
         norm(a.pre, a.pre_eps, a.pre_w, a.pre_b);
 #pragma unroll
@@ -127,7 +136,7 @@ namespace vkhip {
                 for (int j = 0; j < VEC; ++j) z[i][j] = __builtin_fmaf(z[i][j], s[j], z[i][j]);
             }
             if (a.shift) z[i] += load(a.shift, m * a.mod_row, i);
-            *reinterpret_cast<V *>((T *) a.y + row * a.y_row + at(i)) = __builtin_convertvector(z[i], V);
+            store_row(a.y, row * a.y_row, i);
         }
     }
 
@@ -143,23 +152,42 @@ namespace vkhip {
         return nullptr;
     }
 
+    constexpr int     kNormWave = 1280, kNormWide = 4096;
+    constexpr int64_t kNormPast = (int64_t) 64 << 20; // bytes of x from which rows pass the caches
+
     template <typename T, int VEC, int N, int GT>
     static void residual_norm_start(const NormArgs &a, hipStream_t s) {
         constexpr int RPB = GT < 256 ? 256 / GT : 1, THREADS = GT < 256 ? 256 : GT;
         const int64_t blocks = ceil_div(a.rows, RPB), layers = ceil_div(blocks, 0xFFFFFFFF / THREADS);
-        residual_norm_kernel<T, VEC, N, GT><<<dim3((unsigned) ceil_div(blocks, layers), (unsigned) layers), THREADS, 0, s>>>(a);
+        const dim3    grid((unsigned) ceil_div(blocks, layers), (unsigned) layers);
+        if ((int64_t) a.rows * a.dim * (int64_t) sizeof(T) >= kNormPast) residual_norm_kernel<T, VEC, N, GT, true><<<grid, THREADS, 0, s>>>(a);
+        else residual_norm_kernel<T, VEC, N, GT, false><<<grid, THREADS, 0, s>>>(a);
     }
-    // Threads of a row: a wave up to 2048 values, 256 threads up to 8192, 1024 above; 8, 16 or 32 values a thread.
+    // Vectors of a thread: as many as its row has, up to 32 values.
     template <typename T, int VEC, int GT>
     static void residual_norm_width(const NormArgs &a, hipStream_t s) {
-        if (a.dim <= GT * 8) residual_norm_start<T, VEC, 8 / VEC, GT>(a, s);
-        else if (a.dim <= GT * 16) residual_norm_start<T, VEC, 16 / VEC, GT>(a, s);
-        else residual_norm_start<T, VEC, 32 / VEC, GT>(a, s);
+        const int n = (int) ceil_div(a.dim, GT * VEC);
+        if constexpr (VEC == 1) {
+            if (n <= 8) residual_norm_start<T, VEC, 8, GT>(a, s);
+            else if (n <= 16) residual_norm_start<T, VEC, 16, GT>(a, s);
+            else residual_norm_start<T, VEC, 32, GT>(a, s);
+        } else if (n == 1) residual_norm_start<T, VEC, 1, GT>(a, s);
+        else if (n == 2) residual_norm_start<T, VEC, 2, GT>(a, s);
+        else if (n == 3) residual_norm_start<T, VEC, 3, GT>(a, s);
+        else if (n == 4) residual_norm_start<T, VEC, 4, GT>(a, s);
+        else if constexpr (VEC == 4) {
+            if (n == 5) residual_norm_start<T, VEC, 5, GT>(a, s);
+            else if (n == 6) residual_norm_start<T, VEC, 6, GT>(a, s);
+            else residual_norm_start<T, VEC, 8, GT>(a, s);
+        }
     }
+    // Threads of a row: a wave up to 1280 values, 256 threads up to 4096, 1024 above; a vector or two a thread is what keeps
+    // many rows under way (bf16, us at 411 MB of rows, x, r, h and y: 2048 values in a wave 206, in 256 threads 164; 8192 in 256, 512,
+    // 1024 threads 211, 196, 172; 12800 x 1100 fp16 with gate, scale and shift 35 and 38).
     template <typename T, int VEC>
     static void residual_norm_threads(const NormArgs &a, hipStream_t s) {
-        if (a.dim <= 2048) residual_norm_width<T, VEC, 64>(a, s);
-        else if (a.dim <= 8192) residual_norm_width<T, VEC, 256>(a, s);
+        if (a.dim <= kNormWave) residual_norm_width<T, VEC, 64>(a, s);
+        else if (a.dim <= kNormWide) residual_norm_width<T, VEC, 256>(a, s);
         else residual_norm_width<T, VEC, 1024>(a, s);
     }
     template <typename T>
