@@ -479,7 +479,10 @@ namespace vkhip {
         a.groups     = p->groups;
         a.max_prefix = p->max_tokens > 0 && p->max_tokens < whole.max_len ? p->max_tokens : whole.max_len;
         const int64_t each = p->groups > 0 ? (int64_t) c->batch * a.rows / p->groups : 0; // rows of a group
-        a.wide            = each > 192 && a.c.row == 128 ? 2 : each > 32;
+        // Tiles of 128 or 256 rows (kv_prefix.hip) from about 2^20 rows x tokens on; below, their start, about 10 us, is what
+        // counts (32 heads on 8, D = 128, prefix pass and join in us, 32-row tiles / wide ones: 64 sequences behind 4096
+        // tokens 28 / 29, 128 behind 1024 22 / 24, 16 behind 4096 17 / 19; 256 behind 32768 590 / 170).
+        a.wide            = each <= 64 || (int64_t) c->batch * a.rows * a.max_prefix <= 1 << 20 ? 0 : each > 192 && a.c.row == 128 ? 2 : 1;
         const int height  = a.wide ? a.wide * kWideRows : 32;
         a.shared_blocks   = (int) ((int64_t) c->batch * a.rows / height + p->groups);
         const int wide_tiles = kWideUnits / (c->page_tokens == 32 ? 2 : 1);
