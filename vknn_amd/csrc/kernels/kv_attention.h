@@ -20,6 +20,7 @@ namespace vkhip {
         const int32_t *cu, *prefix;           // groups of neighbouring sequences, tokens that each shares
         int            groups, max_prefix;
         int            shared_span, shared_splits, shared_blocks; // tokens a workgroup, splits (the first of a row's), blocks of rows
+        int            prefix_blocks;                             // workgroups of the prefixes, in blocks of 32 rows
         int            wide;                                      // blocks of 1 or 2 times kWideRows rows; 0: of 32
     };
 

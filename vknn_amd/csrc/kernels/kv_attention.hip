@@ -21,27 +21,34 @@
 
 namespace vkhip {
 
-
     // DJ = row / 64 channels, RT tiles of 16 rows, P32: pages of 32 tokens (two to a step), NW waves.
     // Two row tiles of 64 channels are compiled for two waves a SIMD: 16 x 5000 tokens, 32 rows, 31.7 -> 29.1 us; of 128
     // channels that costs more than it gives (4 x 40000, 64 rows, 132 -> 160 us), one row tile gains nothing.
     // MODE: a sequence's tokens (kAll), those behind the prefix that it shares (kTail), or a group's prefix (kPrefix), whose
     // rows are those of all its sequences; the last two leave parts for the join.
     enum { kAll, kTail, kPrefix };
+    template <int DJ, int RT, int NW>
+    struct KvAttnLds {
+        static constexpr int NL = NW < 4 ? NW : 4; // waves whose products lie here at a time
+        float wave_m[NW][RT * 16], wave_l[NW][RT * 16];
+        float acc[NL][16][DJ * 64 + 4];
+    };
+    // x, y, z: the workgroup's place in a grid of heads x blocks of rows, sequences and splits, or heads, splits and blocks
+    // of the groups' rows (kPrefix).
     template <typename T, int DJ, int RT, bool P32, int NW, int MODE>
-    __global__ __launch_bounds__(NW * 64, DJ == 1 && RT == 2 ? 2 : 1) void kv_attention_kernel(KvAttnArgs a) {
-        constexpr int Dp = DJ * 64, DT = DJ * 4, NL = NW < 4 ? NW : 4; // NL: waves whose products lie in LDS at a time
-        __shared__ float wave_m[NW][RT * 16], wave_l[NW][RT * 16];
-        __shared__ float acc_lds[NL][16][Dp + 4];
+    __device__ __forceinline__ void kv_attention_body(const KvAttnArgs &a, int bx, int by, int bz, KvAttnLds<DJ, RT, NW> &lds) {
+        constexpr int Dp = DJ * 64, DT = DJ * 4, NL = KvAttnLds<DJ, RT, NW>::NL;
+        auto &wave_m = lds.wave_m, &wave_l = lds.wave_l;
+        auto &acc_lds = lds.acc;
         const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, nn = lane & 15;
         // heads, then sequences, then splits: workgroups go to the 8 XCDs in turn, and with splits first the later ones,
         // which short sequences do not have, would all meet on some of them
-        const int head = MODE == kPrefix ? blockIdx.x : blockIdx.x / a.blocks, split = MODE == kPrefix ? blockIdx.y : blockIdx.z;
+        const int head = MODE == kPrefix ? bx : bx / a.blocks, split = MODE == kPrefix ? by : bz;
         const int P   = a.c.page_tokens, D = a.c.head_dim;
-        int       b = blockIdx.y, row0 = blockIdx.x % a.blocks * (16 * RT), rows = a.rows, len, t0, t1; // kPrefix: b is the group's first sequence
+        int       b = by, row0 = bx % a.blocks * (16 * RT), rows = a.rows, len, t0, t1; // kPrefix: b is the group's first sequence
         if constexpr (MODE == kPrefix) {
             const auto    bound = [&](int i) { return clampi(a.cu[i], 0, a.c.batch); };
-            const SeqTile w = find_tile(blockIdx.z, a.groups, [&](int g) { return prefix_of(a, g) > 0 ? (max(0, bound(g + 1) - bound(g)) * a.rows + 16 * RT - 1) / (16 * RT) : 0; });
+            const SeqTile w = find_tile(bz, a.groups, [&](int g) { return prefix_of(a, g) > 0 ? (max(0, bound(g + 1) - bound(g)) * a.rows + 16 * RT - 1) / (16 * RT) : 0; });
             if (w.b < 0) return;
             const int g = __builtin_amdgcn_readfirstlane(w.b);
             b = bound(g), rows = (bound(g + 1) - b) * a.rows, row0 = __builtin_amdgcn_readfirstlane(w.tile) * (16 * RT);
@@ -301,6 +308,23 @@ namespace vkhip {
         }
     }
 
+    template <typename T, int DJ, int RT, bool P32, int NW, int MODE>
+    __global__ __launch_bounds__(NW * 64, DJ == 1 && RT == 2 ? 2 : 1) void kv_attention_kernel(KvAttnArgs a) {
+        __shared__ KvAttnLds<DJ, RT, NW> lds;
+        kv_attention_body<T, DJ, RT, P32, NW, MODE>(a, blockIdx.x, blockIdx.y, blockIdx.z, lds);
+    }
+    // Prefixes, in blocks of 32 rows, and tails side by side: the first a.prefix_blocks workgroups take the prefixes.
+    template <typename T, int DJ, int RT, bool P32>
+    __global__ __launch_bounds__(256, DJ == 1 ? 2 : 1) void kv_shared_kernel(KvAttnArgs a) {
+        __shared__ union {
+            KvAttnLds<DJ, 2, 4>  prefix;
+            KvAttnLds<DJ, RT, 4> tail;
+        } lds;
+        const int id = (int) (blockIdx.y * gridDim.x + blockIdx.x), i = id - a.prefix_blocks, x = a.c.heads * a.blocks;
+        if (i < 0) kv_attention_body<T, DJ, 2, P32, 4, kPrefix>(a, id % a.c.heads, id / a.c.heads % a.shared_splits, id / a.c.heads / a.shared_splits, lds.prefix);
+        else if (i / x < a.c.batch * a.splits) kv_attention_body<T, DJ, RT, P32, 4, kTail>(a, i % x, i / x % a.c.batch, i / x / a.c.batch, lds.tail);
+    }
+
     // Joins the splits of a row: WPR waves each, two channels a lane; the splits' weights are formed a lane each, so
     // that the products' loads wait for nothing.
     template <typename T, int WPR, bool SHARED>
@@ -434,14 +458,16 @@ namespace vkhip {
 
     constexpr int kWideLeast = 4; // tiles of a workgroup, if the prefix has them
 
-    // Groups of sequences: the prefixes for all rows of a group, then every sequence's tail, then the join.
+    // Groups of sequences: the prefixes for all rows of a group and every sequence's tail, then the join.
     template <typename T, int DJ, int RT, bool P32>
     static int kv_shared_launch(const KvAttnArgs &a, hipStream_t s) {
-        if (!a.wide) kv_attention_kernel<T, DJ, 2, P32, 4, kPrefix><<<dim3((unsigned) a.c.heads, (unsigned) a.shared_splits, (unsigned) a.shared_blocks), 256, 0, s>>>(a);
-        if (int rc = a.wide ? kv_wide_run(a, !__is_same(T, half_t), s) : check_launch("kv_attention_shared prefix")) return rc;
-        const dim3 grid((unsigned) (a.c.heads * a.blocks), (unsigned) a.c.batch, (unsigned) a.splits);
-        if (a.waves == 2) kv_attention_kernel<T, DJ, RT, P32, 2, kTail><<<grid, 128, 0, s>>>(a);
-        else kv_attention_kernel<T, DJ, RT, P32, 4, kTail><<<grid, 256, 0, s>>>(a);
+        if (a.wide) {
+            if (int rc = kv_wide_run(a, !__is_same(T, half_t), s)) return rc;
+            kv_attention_kernel<T, DJ, RT, P32, 4, kTail><<<dim3((unsigned) (a.c.heads * a.blocks), (unsigned) a.c.batch, (unsigned) a.splits), 256, 0, s>>>(a);
+        } else {
+            const int64_t all = a.prefix_blocks + (int64_t) a.c.heads * a.blocks * a.c.batch * a.splits, layers = ceil_div(all, 0xFFFFFF);
+            kv_shared_kernel<T, DJ, RT, P32><<<dim3((unsigned) ceil_div(all, layers), (unsigned) layers), 256, 0, s>>>(a);
+        }
         return check_launch("kv_attention_shared");
     }
     template <typename T, int DJ>
@@ -474,7 +500,7 @@ namespace vkhip {
         vkhip_kv_attention_desc tail = *d;
         tail.max_len = p->max_tail > 0 && p->max_tail < whole.max_len ? p->max_tail : whole.max_len;
         KvAttnArgs a = kv_attention_cut(&tail, c);
-        if (a.waves == 8) a.waves = 4; // the span of 8 is one of 4's, twice as often
+        a.waves = 4; // spans are whole rounds of 2, 4 or 8
         a.max_len    = whole.max_len;
         a.groups     = p->groups;
         a.max_prefix = p->max_tokens > 0 && p->max_tokens < whole.max_len ? p->max_tokens : whole.max_len;
@@ -497,6 +523,8 @@ namespace vkhip {
         if (a.wide && splits < ceil_div(rounds, wide_tiles)) splits = ceil_div(rounds, wide_tiles);
         a.shared_span   = (int) (ceil_div(rounds, splits) * round);
         a.shared_splits = (int) ceil_div(a.max_prefix > 0 ? a.max_prefix : 1, a.shared_span);
+        const int64_t prefixes = (int64_t) c->kv_heads * a.shared_splits * a.shared_blocks, tails = (int64_t) c->kv_heads * a.blocks * c->batch * a.splits;
+        a.prefix_blocks = prefixes + tails < 0x7FFF0000 ? (int) prefixes : -1; // -1: more than a launch numbers
         return a;
     }
     static bool kv_nothing_shared(const KvAttnArgs &a) { return a.groups == 0 || a.max_prefix < a.c.page_tokens; }
@@ -550,7 +578,7 @@ int vkhip_kv_attention_shared(const vkhip_kv_attention_desc *d, const vkhip_kv_c
     if (kv_nothing_shared(a)) return vkhip_kv_attention(d, c, q, lens, o, workspace, s);
     if (c->pages == 0) a.max_len = a.max_prefix = 0; // no block has memory: every query gives zeros
     if (!workspace) return set_error(VKHIP_ERR_INVALID, what, "null pointer");
-    if ((int64_t) c->kv_heads * a.blocks > 65535 || a.shared_blocks > 65535) return set_error(VKHIP_ERR_INVALID, what, "too many heads, sequences and query tokens");
+    if ((int64_t) c->kv_heads * a.blocks > 65535 || a.shared_blocks > 65535 || a.prefix_blocks < 0) return set_error(VKHIP_ERR_INVALID, what, "too many heads, sequences and query tokens");
     a.q = q, a.o = o, a.lens = lens, a.part_o = (float *) workspace, a.scale = d->scale, a.cu = p->cu, a.prefix = p->tokens;
     a.part_s = a.part_o + (size_t) c->batch * c->kv_heads * a.rows * (a.shared_splits + a.splits) * c->head_dim;
     a.q_row = d->q_row, a.q_head = d->q_head, a.o_row = d->o_row, a.o_head = d->o_head;
