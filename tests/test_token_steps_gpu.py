@@ -665,6 +665,19 @@ def test_residual_norm_many_rows(gpu, dim, dtype):
     assert torch.equal(h, h[at]) and torch.equal(y, y[at])
 
 
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("rows,dim", [(700, 9), (300, 515), (300, 1029), (300, 1541), (200, 2302), (200, 3100), (100, 5003), (60, 7001), (40, 8193), (20, 16389), (9, 24581)])
+def test_residual_norm_odd_rows_in_place(gpu, rows, dim, dtype):
+    """Rows whose last vector begins inside the one before, in place: bit for bit as elsewhere, with and without a norm between loads and stores."""
+    x, r, g = rand(1, rows, dim), rand(2, rows, dim), rand(3, 1, dim)
+    for how in (dict(post="none", pre="none", gate=g), dict(post="layer", pre="layer")):
+        apart = residual_norm(x, r, dtype=dtype, **how)
+        check_norm(apart, x, r, dtype=dtype, **how)
+        for place in ("x", "r"):
+            for one, two in zip(apart, residual_norm(x, r, dtype=dtype, place=place, pad=1, **how)):
+                assert torch.equal(one, two)
+
+
 # ------------------------------------------------------------------------------------ together
 def test_step_on_a_stream_of_its_own_and_as_a_graph(gpu):
     """Two steps of several requests behind a shared prefix as they would be used: norm, pages, positions, rows into the

@@ -13,6 +13,7 @@ namespace vkhip {
         const int32_t *mod;
         void          *h, *y;
         int            rows, dim, post, pre, mods, mod_rows;
+        bool           in_place;
         float          alpha, post_eps, pre_eps;
         int64_t        x_row, r_row, h_row, y_row, mod_row;
     };
@@ -33,21 +34,25 @@ namespace vkhip {
         return v;
     }
 
-    // GT threads a row, N vectors of VEC values each, vector i of thread t at (i GT + t) VEC. PAST: rows pass the caches.
-    template <typename T, int VEC, int N, int GT, bool PAST>
-    __global__ __launch_bounds__(GT < 256 ? 256 : GT) void residual_norm_kernel(NormArgs a) {
-        typedef T     V __attribute__((ext_vector_type(VEC)));
-        typedef float F __attribute__((ext_vector_type(VEC)));
+    // GT threads a row, N vectors of VEC values each, vector i of thread t at (i GT + t) VEC. RAGGED: a row's last vector begins
+    // at dim - VEC; its first values, of the vector before, count once, and are stored twice, or once in place, where its owner
+    // may be a wave that has yet to read them. PAST: rows pass the caches.
+    template <typename T, int VEC, int N, int GT, bool RAGGED, bool PAST>
+    __global__ __launch_bounds__(GT == 64 ? 256 : GT) void residual_norm_kernel(NormArgs a) {
+        typedef T     V __attribute__((ext_vector_type(VEC), aligned(sizeof(T)))); // of any alignment: one instruction
+        typedef float F __attribute__((ext_vector_type(VEC), aligned(4)));
         __shared__ float waves[GT / 64];
-        constexpr int RPB = GT < 256 ? 256 / GT : 1; // rows of a workgroup
-        const int     t = (int) threadIdx.x % GT;
-        const int64_t row = ((int64_t) blockIdx.y * gridDim.x + blockIdx.x) * RPB + (int) threadIdx.x / GT;
+        constexpr int RPB = GT == 64 ? 4 : 1; // rows of a workgroup
+        const int     t = RPB > 1 ? (int) threadIdx.x % GT : (int) threadIdx.x;
+        const int64_t row = ((int64_t) blockIdx.y * gridDim.x + blockIdx.x) * RPB + (RPB > 1 ? (int) threadIdx.x / GT : 0);
         if (row >= a.rows) return; // the whole group
         const int64_t m = a.mod ? clampi(a.mod[row], 0, a.mods - 1) : (a.mod_rows ? row / a.mod_rows : 0);
         const float   count = (float) a.dim;
         F             z[N];
-        const auto    at = [&](int i) { return (i * GT + t) * VEC; };
-        const auto    in = [&](int i) { return at(i) < a.dim; };
+        const auto    whole = [&](int i) { return (i * GT + t) * VEC; };
+        const auto    in = [&](int i) { return whole(i) < a.dim; };
+        const auto    at = [&](int i) { return RAGGED ? min(whole(i), a.dim - VEC) : whole(i); };
+        const auto    own = [&](int i, int j) { return RAGGED && j < whole(i) - at(i) ? 0.f : z[i][j]; }; // what counts
         const auto    load = [&](const void *p, int64_t offset, int i) {
             const V v = *reinterpret_cast<const V *>((const T *) p + offset + at(i));
             return __builtin_convertvector(v, F);
@@ -58,7 +63,11 @@ namespace vkhip {
         };
         const auto store_row = [&](void *p, int64_t offset, int i) {
             const V v = __builtin_convertvector(z[i], V);
-            if constexpr (PAST) __builtin_nontemporal_store(v, reinterpret_cast<V *>((T *) p + offset + at(i)));
+            if (RAGGED && a.in_place && whole(i) > at(i)) {
+#pragma unroll
+                for (int j = 1; j < VEC; ++j)
+                    if (j >= whole(i) - at(i)) ((T *) p + offset + at(i))[j] = v[j];
+            } else if constexpr (PAST) __builtin_nontemporal_store(v, reinterpret_cast<V *>((T *) p + offset + at(i)));
             else *reinterpret_cast<V *>((T *) p + offset + at(i)) = v;
         };
         const auto norm = [&](int kind, float eps, const float *w, const float *b) {
@@ -68,7 +77,7 @@ namespace vkhip {
 #pragma unroll
                 for (int i = 0; i < N; ++i)
 #pragma unroll
-                    for (int j = 0; j < VEC; ++j) sum += z[i][j];
+                    for (int j = 0; j < VEC; ++j) sum += own(i, j);
                 const float mean = row_sum<GT>(sum, waves) / count; // a row of one value has it as its mean, and no variance
 #pragma unroll
                 for (int i = 0; i < N; ++i)
@@ -79,7 +88,7 @@ namespace vkhip {
 #pragma unroll
             for (int i = 0; i < N; ++i)
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) sum = __builtin_fmaf(z[i][j], z[i][j], sum);
+                for (int j = 0; j < VEC; ++j) sum = __builtin_fmaf(own(i, j), own(i, j), sum);
             const float rstd = 1.f / __builtin_sqrtf(row_sum<GT>(sum, waves) / count + eps);
 #pragma unroll
             for (int i = 0; i < N; ++i) {
@@ -152,49 +161,35 @@ namespace vkhip {
         return nullptr;
     }
 
-    constexpr int     kNormWave = 1280, kNormWide = 4096;
     constexpr int64_t kNormPast = (int64_t) 64 << 20; // bytes of x from which rows pass the caches
 
     template <typename T, int VEC, int N, int GT>
     static void residual_norm_start(const NormArgs &a, hipStream_t s) {
-        constexpr int RPB = GT < 256 ? 256 / GT : 1, THREADS = GT < 256 ? 256 : GT;
+        constexpr int RPB = GT == 64 ? 4 : 1, THREADS = RPB * GT;
         const int64_t blocks = ceil_div(a.rows, RPB), layers = ceil_div(blocks, 0xFFFFFFFF / THREADS);
         const dim3    grid((unsigned) ceil_div(blocks, layers), (unsigned) layers);
-        if ((int64_t) a.rows * a.dim * (int64_t) sizeof(T) >= kNormPast) residual_norm_kernel<T, VEC, N, GT, true><<<grid, THREADS, 0, s>>>(a);
-        else residual_norm_kernel<T, VEC, N, GT, false><<<grid, THREADS, 0, s>>>(a);
+        const bool    past = (int64_t) a.rows * a.dim * (int64_t) sizeof(T) >= kNormPast;
+        if (a.dim % VEC) past ? residual_norm_kernel<T, VEC, N, GT, VEC != 1, true><<<grid, THREADS, 0, s>>>(a) : residual_norm_kernel<T, VEC, N, GT, VEC != 1, false><<<grid, THREADS, 0, s>>>(a);
+        else past ? residual_norm_kernel<T, VEC, N, GT, false, true><<<grid, THREADS, 0, s>>>(a) : residual_norm_kernel<T, VEC, N, GT, false, false><<<grid, THREADS, 0, s>>>(a);
     }
-    // Vectors of a thread: as many as its row has, up to 32 values.
-    template <typename T, int VEC, int GT>
-    static void residual_norm_width(const NormArgs &a, hipStream_t s) {
-        const int n = (int) ceil_div(a.dim, GT * VEC);
-        if constexpr (VEC == 1) {
-            if (n <= 8) residual_norm_start<T, VEC, 8, GT>(a, s);
-            else if (n <= 16) residual_norm_start<T, VEC, 16, GT>(a, s);
-            else residual_norm_start<T, VEC, 32, GT>(a, s);
-        } else if (n == 1) residual_norm_start<T, VEC, 1, GT>(a, s);
-        else if (n == 2) residual_norm_start<T, VEC, 2, GT>(a, s);
-        else if (n == 3) residual_norm_start<T, VEC, 3, GT>(a, s);
-        else if (n == 4) residual_norm_start<T, VEC, 4, GT>(a, s);
-        else if constexpr (VEC == 4) {
-            if (n == 5) residual_norm_start<T, VEC, 5, GT>(a, s);
-            else if (n == 6) residual_norm_start<T, VEC, 6, GT>(a, s);
-            else residual_norm_start<T, VEC, 8, GT>(a, s);
-        }
-    }
-    // Threads of a row: a wave up to 1280 values, 256 threads up to 4096, 1024 above; a vector or two a thread is what keeps
-    // many rows under way (bf16, us at 411 MB of rows, x, r, h and y: 2048 values in a wave 206, in 256 threads 164; 8192 in 256, 512,
-    // 1024 threads 211, 196, 172; 12800 x 1100 fp16 with gate, scale and shift 35 and 38).
-    template <typename T, int VEC>
-    static void residual_norm_threads(const NormArgs &a, hipStream_t s) {
-        if (a.dim <= kNormWave) residual_norm_width<T, VEC, 64>(a, s);
-        else if (a.dim <= kNormWide) residual_norm_width<T, VEC, 256>(a, s);
-        else residual_norm_width<T, VEC, 1024>(a, s);
-    }
+    // Threads of a row: one for each vector of 8, in whole waves, up to 1024 threads. bf16, us with several vectors a thread, and with
+    // one: 25088 rows of 2500 values 170 (four), 142 (two), 122; 12500 of 4096 104, 84, 86; 64 of 4096 6.8, 5.4, 4.6; 12800 of 1100 fp16
+    // with gate, scale and shift 33.1 (three, a wave a row) and 28.5. A vector of 8 at any alignment, the last one overlapping: 12800 of
+    // 1101 values 141.6 (value by value) and 28.6.
     template <typename T>
-    static void residual_norm_vectors(const NormArgs &a, int vec, hipStream_t s) {
-        if (vec == 8) residual_norm_threads<T, 8>(a, s);
-        else if (vec == 4) residual_norm_threads<T, 4>(a, s);
-        else residual_norm_threads<T, 1>(a, s);
+    static void residual_norm_threads(const NormArgs &a, hipStream_t s) {
+        if (a.dim < 8) residual_norm_start<T, 1, 1, 64>(a, s);
+        else if (a.dim <= 512) residual_norm_start<T, 8, 1, 64>(a, s);
+        else if (a.dim <= 1024) residual_norm_start<T, 8, 1, 128>(a, s);
+        else if (a.dim <= 1536) residual_norm_start<T, 8, 1, 192>(a, s);
+        else if (a.dim <= 2048) residual_norm_start<T, 8, 1, 256>(a, s);
+        else if (a.dim <= 6 * 512) residual_norm_start<T, 8, 1, 384>(a, s);
+        else if (a.dim <= 4096) residual_norm_start<T, 8, 1, 512>(a, s);
+        else if (a.dim <= 6144) residual_norm_start<T, 8, 1, 768>(a, s);
+        else if (a.dim <= 8192) residual_norm_start<T, 8, 1, 1024>(a, s);
+        else if (a.dim <= 16384) residual_norm_start<T, 8, 2, 1024>(a, s);
+        else if (a.dim <= 24576) residual_norm_start<T, 8, 3, 1024>(a, s);
+        else residual_norm_start<T, 8, 4, 1024>(a, s);
     }
 
 } // namespace vkhip
@@ -228,17 +223,11 @@ int vkhip_residual_norm(const vkhip_residual_norm_desc *d, const void *x, const 
     a.rows = d->rows, a.dim = d->dim, a.post = d->post, a.pre = d->pre, a.mods = d->mods, a.mod_rows = with_mod ? d->mod_rows : 0;
     a.alpha = d->alpha, a.post_eps = d->post_eps, a.pre_eps = d->pre_eps;
     a.x_row = d->x_row, a.r_row = d->r_row, a.h_row = d->h_row, a.y_row = d->y_row, a.mod_row = d->mod_row;
-    // vectors of 8 or 4 values where rows come in such
-    const int64_t all = d->dim | (x ? d->x_row : 0) | (r ? d->r_row : 0) | (h ? d->h_row : 0) | (y ? d->y_row : 0) | (with_mod ? d->mod_row : 0);
-    const auto    fits = [&](int vec) {
-        const uintptr_t bytes = (uintptr_t) vec * elem;
-        return all % vec == 0 && rows % (bytes < 16 ? bytes : 16) == 0 && weights % 16 == 0;
-    };
-    const int   vec = fits(8) ? 8 : fits(4) ? 4 : 1;
-    hipStream_t st  = resolve_stream(s);
-    if (d->dtype == VKHIP_DT_F16) residual_norm_vectors<half_t>(a, vec, st);
-    else if (d->dtype == VKHIP_DT_BF16) residual_norm_vectors<bf16_t>(a, vec, st);
-    else residual_norm_vectors<float>(a, vec, st);
+    a.in_place = (h && (h == x || h == r)) || (y && (y == x || y == r));
+    hipStream_t st = resolve_stream(s);
+    if (d->dtype == VKHIP_DT_F16) residual_norm_threads<half_t>(a, st);
+    else if (d->dtype == VKHIP_DT_BF16) residual_norm_threads<bf16_t>(a, st);
+    else residual_norm_threads<float>(a, st);
     return check_launch("residual_norm");
 }
 
