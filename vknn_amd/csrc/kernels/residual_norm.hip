@@ -22,7 +22,7 @@ namespace vkhip {
     template <int GT>
     __device__ __forceinline__ float row_sum(float v, float *waves) {
 #pragma unroll
-        for (int o = 1; o < 64; o <<= 1) v += __shfl_xor(v, o);
+        for (int o = 1; o < (GT < 64 ? GT : 64); o <<= 1) v += __shfl_xor(v, o);
         if constexpr (GT > 64) {
             __syncthreads(); // the last sum has been read
             if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = v;
@@ -38,11 +38,11 @@ namespace vkhip {
     // at dim - VEC; its first values, of the vector before, count once, and are stored twice, or once in place, where its owner
     // may be a wave that has yet to read them. PAST: rows pass the caches.
     template <typename T, int VEC, int N, int GT, bool RAGGED, bool PAST>
-    __global__ __launch_bounds__(GT == 64 ? 256 : GT) void residual_norm_kernel(NormArgs a) {
+    __global__ __launch_bounds__(GT <= 64 ? 256 : GT) void residual_norm_kernel(NormArgs a) {
         typedef T     V __attribute__((ext_vector_type(VEC), aligned(sizeof(T)))); // of any alignment: one instruction
         typedef float F __attribute__((ext_vector_type(VEC), aligned(4)));
-        __shared__ float waves[GT / 64];
-        constexpr int RPB = GT == 64 ? 4 : 1; // rows of a workgroup
+        __shared__ float waves[GT <= 64 ? 1 : GT / 64];
+        constexpr int RPB = GT <= 64 ? 256 / GT : 1; // rows of a workgroup
         const int     t = RPB > 1 ? (int) threadIdx.x % GT : (int) threadIdx.x;
         const int64_t row = ((int64_t) blockIdx.y * gridDim.x + blockIdx.x) * RPB + (RPB > 1 ? (int) threadIdx.x / GT : 0);
         if (row >= a.rows) return; // the whole group
@@ -165,7 +165,7 @@ namespace vkhip {
 
     template <typename T, int VEC, int N, int GT>
     static void residual_norm_start(const NormArgs &a, hipStream_t s) {
-        constexpr int RPB = GT == 64 ? 4 : 1, THREADS = RPB * GT;
+        constexpr int RPB = GT <= 64 ? 256 / GT : 1, THREADS = RPB * GT;
         const int64_t blocks = ceil_div(a.rows, RPB), layers = ceil_div(blocks, 0xFFFFFFFF / THREADS);
         const dim3    grid((unsigned) ceil_div(blocks, layers), (unsigned) layers);
         const bool    past = (int64_t) a.rows * a.dim * (int64_t) sizeof(T) >= kNormPast;
@@ -175,10 +175,14 @@ namespace vkhip {
     // Threads of a row: one for each vector of 8, in whole waves, up to 1024 threads. bf16, us with several vectors a thread, and with
     // one: 25088 rows of 2500 values 170 (four), 142 (two), 122; 12500 of 4096 104, 84, 86; 64 of 4096 6.8, 5.4, 4.6; 12800 of 1100 fp16
     // with gate, scale and shift 33.1 (three, a wave a row) and 28.5. A vector of 8 at any alignment, the last one overlapping: 12800 of
-    // 1101 values 141.6 (value by value) and 28.6.
+    // 1101 values 141.6 (value by value) and 30.7.
+    // Several rows share a wave up to 256 values: 500000 of 88 bf16 283 a wave each, 84 in 16 threads.
     template <typename T>
     static void residual_norm_threads(const NormArgs &a, hipStream_t s) {
-        if (a.dim < 8) residual_norm_start<T, 1, 1, 64>(a, s);
+        if (a.dim < 8) residual_norm_start<T, 1, 1, 8>(a, s);
+        else if (a.dim <= 64) residual_norm_start<T, 8, 1, 8>(a, s);
+        else if (a.dim <= 128) residual_norm_start<T, 8, 1, 16>(a, s);
+        else if (a.dim <= 256) residual_norm_start<T, 8, 1, 32>(a, s);
         else if (a.dim <= 512) residual_norm_start<T, 8, 1, 64>(a, s);
         else if (a.dim <= 1024) residual_norm_start<T, 8, 1, 128>(a, s);
         else if (a.dim <= 1536) residual_norm_start<T, 8, 1, 192>(a, s);
