@@ -123,6 +123,30 @@ def test_rotary(gpu, case, dtype, near, interleaved, spectra):
             check_rotary(b, k, pos, **how)
 
 
+# pairs and copied channels that end inside a vector of 8 or 4: both, one alone, fewer than a vector
+ODD = [dict(rows=400, hq=3, hk=2, d=26, sections=[13]), dict(rows=300, hq=2, hk=1, d=59, rot=58, sections=[15, 14]), dict(rows=200, hq=2, hk=2, d=67, rot=46, sections=[20, 3]),
+       dict(rows=300, hq=1, hk=1, d=19, rot=16, sections=[8]), dict(rows=500, hq=1, hk=1, d=15, rot=10, sections=[5]), dict(rows=500, hq=2, hk=0, d=13, rot=8, sections=[4]),
+       dict(rows=500, hq=2, hk=0, d=9, rot=4, sections=[1, 1]), dict(rows=100, hq=2, hk=1, d=255, rot=250, sections=[60, 65])]
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("near", [False, True])
+@pytest.mark.parametrize("case", ODD)
+def test_rotary_odd_heads(gpu, case, near, dtype):
+    """Every layout, and bit for bit the same in place."""
+    rows, d, how = case["rows"], case["d"], dict(sections=case["sections"], rot=case.get("rot"), dtype=dtype, near=near)
+    q, k = rand(d, rows, case["hq"], d) * 3, rand(d + 1, rows, case["hk"], d) if case["hk"] else None
+    pos = np.random.default_rng(rows).integers(-50, 5000, (len(case["sections"]), rows))
+    first = None
+    for layout in ("slices", "place", "heads", "odd"):
+        got = rotary(q, k, pos, layout=layout, **how)
+        first = first or got
+        for x, one, two in zip((q, k), first, got):
+            if x is not None:
+                check_rotary(two, x, pos, **how)
+                assert torch.equal(one, two)
+
+
 def test_rotary_far_positions_and_given_frequencies(gpu):
     """Both ends of the positions' range, and frequencies of any sign and size, whole turns and none among them."""
     q, k = rand(1, 8, 2, 64), rand(2, 8, 1, 64)
@@ -654,7 +678,7 @@ def test_residual_norm_spoiled_row(gpu):
         assert torch.equal(a[keep], b[keep]) and torch.isnan(b[4]).all()
 
 
-@pytest.mark.parametrize("dim,dtype", [(8, "bf16"), (2048, "bf16")])
+@pytest.mark.parametrize("dim,dtype", [(5, "bf16"), (8, "bf16"), (88, "bf16"), (200, "f16"), (2048, "bf16")])
 def test_residual_norm_many_rows(gpu, dim, dtype):
     """More rows than run at once: every one is written, as its own."""
     rows = 20011
@@ -666,7 +690,7 @@ def test_residual_norm_many_rows(gpu, dim, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["f16", "f32"])
-@pytest.mark.parametrize("rows,dim", [(700, 9), (300, 515), (300, 1029), (300, 1541), (200, 2302), (200, 3100), (100, 5003), (60, 7001), (40, 8193), (20, 16389), (9, 24581)])
+@pytest.mark.parametrize("rows,dim", [(700, 9), (333, 67), (333, 131), (301, 259), (300, 515), (300, 1029), (300, 1541), (200, 2302), (200, 3100), (100, 5003), (60, 7001), (40, 8193), (20, 16389), (9, 24581)])
 def test_residual_norm_odd_rows_in_place(gpu, rows, dim, dtype):
     """Rows whose last vector begins inside the one before, in place: bit for bit as elsewhere, with and without a norm between loads and stores."""
     x, r, g = rand(1, rows, dim), rand(2, rows, dim), rand(3, 1, dim)

@@ -21,6 +21,7 @@ namespace vkhip {
         int            units, turned;   // pieces of a head; the first `turned` are pairs, the others copied
         int            slots, per;      // threads that share a row's unit, heads of each
         int            block_rows;      // rows of a workgroup, where several fit
+        bool           in_place;
         int64_t        pos_axis, q_row, q_head, k_row, k_head, qo_row, qo_head, ko_row, ko_head;
         uint64_t       freq[kRotaryPairs]; // turns * 2^64 per position
         uint8_t        axis[kRotaryPairs];
@@ -44,23 +45,17 @@ namespace vkhip {
         if (quarter & 2) s = -s;
     }
 
-    template <bool PAST, typename V>
-    __device__ __forceinline__ V rotary_load(const void *p) {
-        if constexpr (PAST) return __builtin_nontemporal_load(reinterpret_cast<const V *>(p));
-        else return *reinterpret_cast<const V *>(p);
-    }
-    template <bool PAST, typename V>
-    __device__ __forceinline__ void rotary_store(V v, void *p) {
-        if constexpr (PAST) __builtin_nontemporal_store(v, reinterpret_cast<V *>(p));
-        else *reinterpret_cast<V *>(p) = v;
-    }
+    // Rows in the caches, past them in stores, or past them altogether.
+    enum { kCached, kStoresPast, kPast };
 
     // A thread takes one unit of a row in several heads. A unit of halves is VEC pairs, two vectors of VEC channels that lie
     // half of the rotated channels apart; of neighbours VEC channels, or a pair; behind the rotated channels as many that
-    // are copied. PAST: rows pass the caches.
-    template <typename T, int VEC, bool NEAR, bool PAST>
+    // are copied. RAGGED: the last vectors begin that much earlier that they end with their channels; the channels of the
+    // vector before are stored twice, or once where their owner turns them, or in place, where it may be a wave that has yet to
+    // read them.
+    template <typename T, int VEC, bool NEAR, bool RAGGED, int PAST>
     __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
-        typedef T V __attribute__((ext_vector_type(VEC)));
+        typedef T V __attribute__((ext_vector_type(VEC), aligned(sizeof(T)))); // of any alignment: one instruction
         constexpr int  PAIRS = NEAR ? (VEC > 1 ? VEC / 2 : 1) : VEC;
         constexpr bool TWO   = !NEAR || VEC == 1; // vectors of a unit
         const int      each  = a.units * a.slots;
@@ -68,16 +63,43 @@ namespace vkhip {
         const int      r = (int) threadIdx.x / each;
         const int64_t  row = block * a.block_rows + r;
         if (r >= a.block_rows || row >= a.rows) return;
+        const auto load = [](const T *p) {
+            if constexpr (PAST == kPast) return __builtin_nontemporal_load(reinterpret_cast<const V *>(p));
+            else return *reinterpret_cast<const V *>(p);
+        };
+        const auto store = [&](V v, T *p, int skip, bool once) {
+            if (RAGGED && skip > 0 && once) {
+#pragma unroll
+                for (int j = 1; j < VEC; ++j)
+                    if (j >= skip) p[j] = v[j];
+            } else if constexpr (PAST != kCached) __builtin_nontemporal_store(v, reinterpret_cast<V *>(p));
+            else *reinterpret_cast<V *>(p) = v;
+        };
         for (int i = (int) threadIdx.x - r * each; i < each; i += 256) {
             const int  unit = i % a.units, h0 = i / a.units * a.per, h1 = min(a.heads, h0 + a.per);
             const bool turned = unit < a.turned;
-            const int  c0 = turned && !NEAR ? unit * VEC : unit * 2 * PAIRS, c1 = turned && !NEAR ? a.pairs + unit * VEC : c0 + VEC;
-            const bool second = TWO && c1 < a.head_dim;
+            // the first channel of each vector, and how many of its channels are another's
+            int        c0, c1, s0 = 0, s1 = 0, p0 = unit * PAIRS;
+            if (turned) {
+                if constexpr (RAGGED) {
+                    s0 = max(0, p0 + PAIRS - a.pairs);
+                    p0 -= s0;
+                    s1 = s0 = NEAR ? 2 * s0 : s0;
+                }
+                c0 = NEAR ? 2 * p0 : p0, c1 = NEAR ? c0 + VEC : a.pairs + p0;
+            } else {
+                c0 = 2 * a.pairs + (unit - a.turned) * 2 * PAIRS, c1 = c0 + VEC;
+                if constexpr (RAGGED) {
+                    s0 = max(0, c0 + VEC - a.head_dim), s1 = max(0, c1 + VEC - a.head_dim);
+                    c0 -= s0, c1 -= s1;
+                }
+            }
+            const bool second = TWO && s1 < VEC && c1 < a.head_dim;
             float      c[PAIRS], s[PAIRS];
             if (turned)
 #pragma unroll
                 for (int j = 0; j < PAIRS; ++j) {
-                    const int p = unit * PAIRS + j;
+                    const int p = p0 + j;
                     turn_of(a.freq[p], a.pos[a.axis[p] * a.pos_axis + row], c[j], s[j]);
                 }
 #pragma unroll 4
@@ -88,18 +110,18 @@ namespace vkhip {
                 const int64_t to = key ? row * a.ko_row + n * a.ko_head : row * a.qo_row + n * a.qo_head;
                 const T      *x = (const T *) (key ? a.k : a.q) + from;
                 T            *y = (T *) (key ? a.ko : a.qo) + to;
-                V             u = rotary_load<PAST, V>(x + c0), w = u;
-                if (second) w = rotary_load<PAST, V>(x + c1);
+                V             u = load(x + c0), w = u;
+                if (second) w = load(x + c1);
                 if (turned)
 #pragma unroll
                     for (int j = 0; j < PAIRS; ++j) {
                         const float p = (float) (TWO ? u[j] : u[2 * j]), q = (float) (TWO ? w[j] : u[2 * j + (VEC > 1)]);
-                        const T     p1 = (T) (p * c[j] - q * s[j]), q1 = (T) (q * c[j] + p * s[j]);
+                        const T     p1 = (T) __builtin_fmaf(p, c[j], -(q * s[j])), q1 = (T) __builtin_fmaf(q, c[j], p * s[j]); // the same in each of two threads
                         if constexpr (TWO) u[j] = p1, w[j] = q1;
                         else u[2 * j] = p1, u[2 * j + (VEC > 1)] = q1;
                     }
-                rotary_store<PAST>(u, y + c0);
-                if (second) rotary_store<PAST>(w, y + c1);
+                store(u, y + c0, s0, a.in_place || (!turned && c0 < 2 * a.pairs));
+                if (second) store(w, y + c1, s1, a.in_place || (!turned && c1 < 2 * a.pairs));
             }
         }
     }
@@ -164,10 +186,10 @@ namespace vkhip {
         return nullptr;
     }
 
-    template <typename T, int VEC>
+    template <typename T, int VEC, bool RAGGED>
     static void rotary_launch(const vkhip_rotary_desc *d, RotaryArgs &a, hipStream_t s) {
         const int pairs = d->neighbours ? (VEC > 1 ? VEC / 2 : 1) : VEC; // of a unit
-        a.turned = a.pairs / pairs;
+        a.turned = (int) ceil_div(a.pairs, pairs);
         a.units  = a.turned + (int) ceil_div(d->head_dim - d->rotary_dim, 2 * pairs);
         // Heads of a thread: as many as leave the card full, at most 4 (50176 rows of 40 heads of 128, bf16, 2, 4, 8, 10 of them: 201,
         // 193, 197, 206 us; neighbours 210, 187, 181, 186).
@@ -178,9 +200,29 @@ namespace vkhip {
         a.block_rows   = each >= 256 ? 1 : 256 / each;
         const int64_t blocks = ceil_div(a.rows, a.block_rows), layers = ceil_div(blocks, 0xFFFFFF);
         const dim3    grid((unsigned) ceil_div(blocks, layers), (unsigned) layers);
-        const bool past = (int64_t) a.rows * a.heads * d->head_dim * (int64_t) sizeof(T) >= kRotaryPast;
-        if (d->neighbours) past ? rotary_kernel<T, VEC, true, true><<<grid, 256, 0, s>>>(a) : rotary_kernel<T, VEC, true, false><<<grid, 256, 0, s>>>(a);
-        else past ? rotary_kernel<T, VEC, false, true><<<grid, 256, 0, s>>>(a) : rotary_kernel<T, VEC, false, false><<<grid, 256, 0, s>>>(a);
+        // Past the caches go only heads of whole lines, and in loads only whole lines at a time. 45000 rows of 32 heads, fp16, halves, us with
+        // both past, stores past, all cached: heads of 64 100, 66, 86; of 40 180, 127, 83; ragged (52 of 64) 183, 135, 93.
+        const int elem = (int) sizeof(T);
+        if constexpr (!RAGGED)
+            if ((int64_t) a.rows * a.heads * d->head_dim * elem >= kRotaryPast && d->head_dim * elem % 128 == 0) {
+                if (d->neighbours) rotary_kernel<T, VEC, true, false, kPast><<<grid, 256, 0, s>>>(a);
+                else if (a.pairs * elem % 128 == 0) rotary_kernel<T, VEC, false, false, kPast><<<grid, 256, 0, s>>>(a);
+                else rotary_kernel<T, VEC, false, false, kStoresPast><<<grid, 256, 0, s>>>(a);
+                return;
+            }
+        if (d->neighbours) rotary_kernel<T, VEC, true, RAGGED, kCached><<<grid, 256, 0, s>>>(a);
+        else rotary_kernel<T, VEC, false, RAGGED, kCached><<<grid, 256, 0, s>>>(a);
+    }
+    // Vectors of 8 channels, or of 4 where these come out even or there is no full one of 8; single ones below that. 45000 rows of 32 heads
+    // of 64, fp16, halves, us: 56 turned 60 in even vectors of 4, 92 in ragged ones of 8; 52 turned 183 (single), 107 (4), 93 (8).
+    template <typename T>
+    static void rotary_vectors(const vkhip_rotary_desc *d, RotaryArgs &a, hipStream_t s) {
+        const int turned = d->neighbours ? d->rotary_dim : a.pairs, both = turned | (d->head_dim - d->rotary_dim);
+        if (turned >= 8 && both % 8 == 0) rotary_launch<T, 8, false>(d, a, s);
+        else if (both % 4 == 0) rotary_launch<T, 4, false>(d, a, s);
+        else if (turned >= 8) rotary_launch<T, 8, true>(d, a, s);
+        else if (turned >= 4) rotary_launch<T, 4, true>(d, a, s);
+        else rotary_launch<T, 1, false>(d, a, s);
     }
 
 } // namespace vkhip
@@ -209,17 +251,11 @@ int vkhip_rotary(const vkhip_rotary_desc *d, const int32_t *pos, const double *f
     a.q_row = d->q_row, a.q_head = d->q_head, a.qo_row = d->qo_row, a.qo_head = d->qo_head;
     a.k_row = d->k_row, a.k_head = d->k_head, a.ko_row = d->ko_row, a.ko_head = d->ko_head;
     rotary_pairs(d, freq, a);
-    // vectors of 8 or 4 channels where pairs, rows, heads and pointers come in such
-    int64_t all = d->q_row | d->q_head | d->qo_row | d->qo_head | (with_k ? d->k_row | d->k_head | d->ko_row | d->ko_head : 0);
-    const auto fits = [&](int vec) {
-        const int64_t bytes = (int64_t) vec * (int64_t) elem;
-        return (d->neighbours ? d->rotary_dim : a.pairs) % vec == 0 && d->head_dim % vec == 0 && all % vec == 0 && places % (uintptr_t) (bytes < 16 ? bytes : 16) == 0;
-    };
-    const int   vec = fits(8) ? 8 : fits(4) ? 4 : 1;
-    hipStream_t st  = resolve_stream(s);
-    if (d->dtype == VKHIP_DT_F16) vec == 8 ? rotary_launch<half_t, 8>(d, a, st) : vec == 4 ? rotary_launch<half_t, 4>(d, a, st) : rotary_launch<half_t, 1>(d, a, st);
-    else if (d->dtype == VKHIP_DT_BF16) vec == 8 ? rotary_launch<bf16_t, 8>(d, a, st) : vec == 4 ? rotary_launch<bf16_t, 4>(d, a, st) : rotary_launch<bf16_t, 1>(d, a, st);
-    else vec == 8 ? rotary_launch<float, 8>(d, a, st) : vec == 4 ? rotary_launch<float, 4>(d, a, st) : rotary_launch<float, 1>(d, a, st);
+    a.in_place = q == qo || (with_k && k == ko);
+    hipStream_t st = resolve_stream(s);
+    if (d->dtype == VKHIP_DT_F16) rotary_vectors<half_t>(d, a, st);
+    else if (d->dtype == VKHIP_DT_BF16) rotary_vectors<bf16_t>(d, a, st);
+    else rotary_vectors<float>(d, a, st);
     return check_launch("rotary");
 }
 
