@@ -406,12 +406,13 @@ def test_shared_many_rows(gpu, sizes, hq, hkv, t, page, prefixes):
         both_checks(c, q, lens, cu, prefixes, dtype, d ** -0.5, max_tokens=max(prefixes), max_tail=max(tails))
 
 
-@pytest.mark.parametrize("many", [5, 60])
-def test_shared_lengths_inside_the_prefix(gpu, many):
+# Prefixes of more than 2^20 rows x tokens, as far as the host knows, go to other kernels: a wide table is enough for it.
+@pytest.mark.parametrize("many,blocks,page,d", [(5, None, 64, 128), (60, None, 64, 128), (60, 40, 64, 128), (9, 120, 64, 128), (60, 40, 64, 64), (60, 80, 32, 128), (60, 80, 32, 72)])
+def test_shared_lengths_inside_the_prefix(gpu, many, blocks, page, d):
     """Sequences that have not reached their prefix's end, the first one's table naming it: they see what their length
     lets them. A length of nothing gives zeros, more query tokens than tokens give rows that see nothing."""
-    page, heads, d, t = 64, 2, 128, 4
-    c, lens, cu = shared_cache([many], [512], [t] * many, page, heads, d)
+    heads, t = 2, 4
+    c, lens, cu = shared_cache([many], [512], [t] * many, page, heads, d, blocks=blocks)
     for b in range(many):
         c.table[b] = c.table[0]  # all are the first's prefix
     c.gpu_table.put(c.table)
@@ -422,12 +423,12 @@ def test_shared_lengths_inside_the_prefix(gpu, many):
     assert (out[2] == 0).all() and (out[3][:3] == 0).all()
 
 
-@pytest.mark.parametrize("many", [4, 64])
-def test_shared_spoiled_and_missing_pages(gpu, many):
+@pytest.mark.parametrize("many,blocks,d", [(4, None, 64), (64, None, 64), (64, 40, 64), (64, 40, 128), (20, 120, 128)])
+def test_shared_spoiled_and_missing_pages(gpu, many, blocks, d):
     """A prefix page of NaN scale reaches the queries that see it and no other; one without memory is seen by none; the
     tails' and the other group's pages stay their own."""
-    page, heads, d = 64, 1, 64
-    c, lens, cu = shared_cache([many, many], [256, 192], [5] * (2 * many), page, heads, d, seed=3)
+    page, heads = 64, 1
+    c, lens, cu = shared_cache([many, many], [256, 192], [5] * (2 * many), page, heads, d, seed=3, blocks=blocks)
     q = rand(12, 2 * many, 1, 4, d).half().float()
     clean = shared_attention(c, q, lens, cu, [256, 192], "f16", 0.125)
     for scales in (c.ks, c.vs):
@@ -451,12 +452,14 @@ def test_shared_spoiled_and_missing_pages(gpu, many):
         T.check_attention(out[b], q[b].double(), k, v, [1], [int(keep.sum())], True, "f16", 0.125)
 
 
-def test_shared_hints_and_odd_prefixes(gpu):
+@pytest.mark.parametrize("sizes,hq", [([3, 20], 4), ([30, 200], 16)])
+def test_shared_hints_and_odd_prefixes(gpu, sizes, hq):
     """Prefixes are whole pages; a smaller max_tokens leaves the rest to the tails, a smaller max_tail costs time alone,
     max_len cuts sequences; a wide table changes nothing."""
     page, heads, d = 64, 2, 128
-    c, lens, cu = shared_cache([3, 20], [640, 192], list(range(10, 33)), page, heads, d, seed=6, blocks=40)
-    q = rand(13, 23, 1, 4, d).half().float()
+    many = sum(sizes)
+    c, lens, cu = shared_cache(sizes, [640, 192], [10 + b % 23 for b in range(many)], page, heads, d, seed=6, blocks=40)
+    q = rand(13, many, 1, hq, d).half().float()
     for how in (dict(), dict(max_tokens=640, max_tail=32), dict(max_tokens=300), dict(max_tokens=64), dict(max_tokens=63), dict(max_tail=1), dict(max_len=700), dict(max_tokens=1 << 20)):
         for given in ([640, 192], [703, 193], [641, 255]):
             both_checks(c, q, lens, cu, given, "f16", 0.09, **how)
@@ -470,6 +473,11 @@ def test_shared_groups_out_of_range(gpu):
     """Ranges and prefixes that make no sense stay within the arrays, and sequences in no group are right."""
     c, lens, cu = shared_cache([4], [128], [20] * 4, 64, 1, 64, seed=7)
     q = rand(14, 4, 1, 2, 64).half().float()
+    wide, many, wcu = shared_cache([70], [128], [20] * 70, 64, 1, 64, seed=7, blocks=130)  # the same in wide tiles
+    wq = rand(14, 70, 1, 2, 64).half().float()
+    for given in ([0, 1 << 30], [-7, 70], [5, 66]):
+        for prefix in (128, 0, -64):
+            both_checks(wide, wq, many, given, [prefix], "f16", 0.125)
     both_checks(c, q, lens, [0, 1 << 30], [128], "f16", 0.125)
     both_checks(c, q, lens, [-7, 4], [128], "f16", 0.125)
     both_checks(c, q, lens, [2, 2, 2], [128, 1 << 30], "f16", 0.125)
@@ -487,11 +495,11 @@ def test_shared_many_groups(gpu):
     both_checks(c, q, lens, cu, prefixes, "f16", 0.125)
 
 
-@pytest.mark.parametrize("many", [2, 40])
-def test_shared_large_scores(gpu, many):
+@pytest.mark.parametrize("many,blocks,d", [(2, None, 64), (40, None, 64), (40, 110, 64), (130, 40, 64), (60, 80, 128)])
+def test_shared_large_scores(gpu, many, blocks, d):
     """bf16 queries beyond fp16's range, scores in the thousands, keys that grow along the prefix: maxima that move late."""
-    page, heads, d = 64, 2, 64
-    c, lens, cu = shared_cache([many], [1024], [30] * many, page, heads, d, seed=9)
+    page, heads = 64, 2
+    c, lens, cu = shared_cache([many], [1024], [30] * many, page, heads, d, seed=9, blocks=blocks)
     ks = c.ks.get()
     ks[c.table[0, :16].long()] *= torch.linspace(0.1, 8, 16)[:, None]
     c.ks.put(ks)
@@ -500,12 +508,12 @@ def test_shared_large_scores(gpu, many):
         both_checks(c, q, lens, cu, [1024], "bf16", scale)
 
 
-@pytest.mark.parametrize("many", [2, 40])
-def test_shared_value_scales_far_apart(gpu, many):
+@pytest.mark.parametrize("many,blocks,page,d", [(2, None, 64, 64), (40, None, 64, 64), (40, 110, 64, 64), (60, 80, 64, 128), (40, 220, 32, 64), (60, 160, 32, 128)])
+def test_shared_value_scales_far_apart(gpu, many, blocks, page, d):
     """Pages of values many powers of two apart, and one of zeros: a small page that owns the weights keeps its digits
     beside a large one that has none."""
-    page, heads, d = 64, 1, 64
-    c, lens, cu = shared_cache([many], [512], [3] * many, page, heads, d, seed=10)
+    heads = 1
+    c, lens, cu = shared_cache([many], [512], [3] * many, page, heads, d, seed=10, blocks=blocks)
     vs, ks = c.vs.get(), c.ks.get()
     for i, f in enumerate([1.0, 2.0 ** -30, 2.0 ** 20, 0.0, 2.0 ** -60, 1.0, 2.0 ** 10, 1.0]):
         vs[int(c.table[0, i])] *= f
@@ -527,6 +535,21 @@ def test_shared_value_scales_far_apart(gpu, many):
                 e = (d + 16) * F32 * qk + 2.0 ** -20
                 bound = 2.0 ** -11 * want.abs() * 1.01 + TINY["f16"] + (2.0 ** -11 * 1.02 + 2 * e) * pv + p.clamp(max=2.0 ** -38) @ v[:, 0].abs()
                 assert ((out[b, :, h] - want).abs() / bound).max().item() <= 1, (own, b, h)
+
+
+@pytest.mark.parametrize("many,blocks,page,d", [(5, None, 64, 64), (40, 110, 64, 64), (60, 80, 64, 128), (40, 220, 32, 64)])
+def test_shared_pages_of_zeros(gpu, many, blocks, page, d):
+    """Pages whose keys, values or both are zeros: scores of nothing that still take their weight, and a prefix of such alone."""
+    c, lens, cu = shared_cache([many], [512], [3] * many, page, 1, d, seed=18, blocks=blocks)
+    vs, ks = c.vs.get(), c.ks.get()
+    q = rand(19, many, 1, 4, d).half().float()
+    for keys, values in (([1, 2, 7], [2, 5]), (range(512 // page), []), (range(512 // page), range(512 // page))):
+        a, b = ks.clone(), vs.clone()
+        a[[int(c.table[0, i]) for i in keys]] = 0.0
+        b[[int(c.table[0, i]) for i in values]] = 0.0
+        c.ks.put(a)
+        c.vs.put(b)
+        both_checks(c, q, lens, cu, [512], "f16", 0.125)
 
 
 def test_shared_long_prefix(gpu):
