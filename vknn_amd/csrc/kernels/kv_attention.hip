@@ -501,6 +501,14 @@ namespace vkhip {
         tail.max_len = p->max_tail > 0 && p->max_tail < whole.max_len ? p->max_tail : whole.max_len;
         KvAttnArgs a = kv_attention_cut(&tail, c);
         a.waves = 4; // spans are whole rounds of 2, 4 or 8
+        // Tails are joined in any case: a second workgroup a compute unit and half of a third costs no launch (124 sequences of 4
+        // heads, up to 800 tokens, 15.4 / 11.6 us; of 512 workgroups with 3 rounds each 34.4 either way, 200 x 8 in halves slower).
+        const int64_t tail_rounds = ceil_div(a.max_len, 4 * kStep), tail_base = (int64_t) c->batch * c->kv_heads * a.blocks;
+        const int64_t more = tail_base > 0 && 1024 / tail_base < tail_rounds ? 1024 / tail_base : tail_rounds;
+        if (more > a.splits) {
+            a.span   = (int) (ceil_div(tail_rounds, more) * 4 * kStep);
+            a.splits = (int) ceil_div(a.max_len, a.span);
+        }
         a.max_len    = whole.max_len;
         a.groups     = p->groups;
         a.max_prefix = p->max_tokens > 0 && p->max_tokens < whole.max_len ? p->max_tokens : whole.max_len;
@@ -516,7 +524,9 @@ namespace vkhip {
         const int     round = (a.wide ? 1 : 4) * kStep; // tokens that a workgroup takes at a time
         const int64_t rounds = ceil_div(a.max_prefix > 0 ? a.max_prefix : 1, round), full = ceil_div((int64_t) c->batch * a.rows, height);
         const int64_t base = (full > p->groups ? full : p->groups) * c->kv_heads; // blocks, if groups fill theirs
-        const int64_t places = a.wide == 2 ? 256 : 512;
+        // blocks of uneven groups outnumber that, and two workgroups a compute unit make good for each other's ends (7 groups of 124
+        // sequences, 8, 10, 12 splits: 40, 46 (which begin a second turn), 39 us; one group of 128, 10 and 13: 27, 29)
+        const int64_t places = a.wide == 2 ? 256 : a.wide == 1 && p->groups > 1 ? 640 : 512;
         int64_t       splits = base >= places || base == 0 ? 1 : places / base;
         const int64_t most = a.wide ? rounds / kWideLeast : rounds;
         if (splits > most) splits = most > 0 ? most : 1;
