@@ -501,10 +501,10 @@ namespace vkhip {
         tail.max_len = p->max_tail > 0 && p->max_tail < whole.max_len ? p->max_tail : whole.max_len;
         KvAttnArgs a = kv_attention_cut(&tail, c);
         a.waves = 4; // spans are whole rounds of 2, 4 or 8
-        // Tails are joined in any case: a second workgroup a compute unit and half of a third costs no launch (124 sequences of 4
-        // heads, up to 800 tokens, 15.4 / 11.6 us; of 512 workgroups with 3 rounds each 34.4 either way, 200 x 8 in halves slower).
+        // Tails are joined in any case, so that two workgroups a sequence cost no launch where four fit a compute unit, as with 64
+        // channels (124 sequences of 4 heads, up to 800 tokens, 15.4 / 11.6 us; of 128 channels two fit: 35 x 8 of 40 rows 19.5 / 22.1).
         const int64_t tail_rounds = ceil_div(a.max_len, 4 * kStep), tail_base = (int64_t) c->batch * c->kv_heads * a.blocks;
-        const int64_t more = tail_base > 0 && 1024 / tail_base < tail_rounds ? 1024 / tail_base : tail_rounds;
+        const int64_t more = tail_base == 0 || a.c.row != 64 ? 1 : 1024 / tail_base < tail_rounds ? 1024 / tail_base : tail_rounds;
         if (more > a.splits) {
             a.span   = (int) (ceil_div(tail_rounds, more) * 4 * kStep);
             a.splits = (int) ceil_div(a.max_len, a.span);
