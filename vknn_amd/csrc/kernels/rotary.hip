@@ -10,7 +10,7 @@
 
 namespace vkhip {
 
-    constexpr int     kRotaryPairs = 128;
+    constexpr int     kRotaryPairs = 128, kRotaryHeads = 4; // of a head; of a thread
     constexpr int64_t kRotaryPast = (int64_t) 64 << 20; // bytes of rows from which they pass the caches
 
     struct RotaryArgs {
@@ -95,34 +95,47 @@ namespace vkhip {
                 }
             }
             const bool second = TWO && s1 < VEC && c1 < a.head_dim;
-            float      c[PAIRS], s[PAIRS];
+            const auto place = [&](const void *q, const void *k, int64_t q_row, int64_t q_head, int64_t k_row, int64_t k_head, int h) {
+                return h < a.q_heads ? (T *) q + (row * q_row + h * q_head) : (T *) k + (row * k_row + (h - a.q_heads) * k_head);
+            };
+            // All heads are on their way while the angles are, but for whole heads of neighbours past the caches, which go one by one (50176
+            // rows of 40 heads of 128, bf16, at once and one by one: halves 182, 192 us, neighbours 205, 185; 45000 x 32 of 40 channels,
+            // fp16, 59, 81).
+            constexpr bool ALL = !NEAR || PAST != kPast;
+            V              u[kRotaryHeads], w[kRotaryHeads];
+            const auto     head = [&](int n) {
+                const T *x = place(a.q, a.k, a.q_row, a.q_head, a.k_row, a.k_head, h0 + n);
+                u[n] = load(x + c0);
+                if (second) w[n] = load(x + c1);
+            };
+            if constexpr (ALL)
+#pragma unroll
+                for (int n = 0; n < kRotaryHeads; ++n)
+                    if (h0 + n < h1) head(n);
+            float c[PAIRS], s[PAIRS];
             if (turned)
 #pragma unroll
                 for (int j = 0; j < PAIRS; ++j) {
                     const int p = p0 + j;
                     turn_of(a.freq[p], a.pos[a.axis[p] * a.pos_axis + row], c[j], s[j]);
                 }
-#pragma unroll 4
-            for (int h = h0; h < h1; ++h) {
-                const bool    key = h >= a.q_heads;
-                const int     n = key ? h - a.q_heads : h;
-                const int64_t from = key ? row * a.k_row + n * a.k_head : row * a.q_row + n * a.q_head;
-                const int64_t to = key ? row * a.ko_row + n * a.ko_head : row * a.qo_row + n * a.qo_head;
-                const T      *x = (const T *) (key ? a.k : a.q) + from;
-                T            *y = (T *) (key ? a.ko : a.qo) + to;
-                V             u = load(x + c0), w = u;
-                if (second) w = load(x + c1);
-                if (turned)
 #pragma unroll
-                    for (int j = 0; j < PAIRS; ++j) {
-                        const float p = (float) (TWO ? u[j] : u[2 * j]), q = (float) (TWO ? w[j] : u[2 * j + (VEC > 1)]);
-                        const T     p1 = (T) __builtin_fmaf(p, c[j], -(q * s[j])), q1 = (T) __builtin_fmaf(q, c[j], p * s[j]); // the same in each of two threads
-                        if constexpr (TWO) u[j] = p1, w[j] = q1;
-                        else u[2 * j] = p1, u[2 * j + (VEC > 1)] = q1;
-                    }
-                store(u, y + c0, s0, a.in_place || (!turned && c0 < 2 * a.pairs));
-                if (second) store(w, y + c1, s1, a.in_place || (!turned && c1 < 2 * a.pairs));
-            }
+            for (int n = 0; n < kRotaryHeads; ++n)
+                if (h0 + n < h1) {
+                    if constexpr (!ALL) head(n);
+                    V &v = u[n], &z = w[n];
+                    if (turned)
+#pragma unroll
+                        for (int j = 0; j < PAIRS; ++j) {
+                            const float p = (float) (TWO ? v[j] : v[2 * j]), q = (float) (TWO ? z[j] : v[2 * j + (VEC > 1)]);
+                            const T     p1 = (T) __builtin_fmaf(p, c[j], -(q * s[j])), q1 = (T) __builtin_fmaf(q, c[j], p * s[j]); // the same in each of two threads
+                            if constexpr (TWO) v[j] = p1, z[j] = q1;
+                            else v[2 * j] = p1, v[2 * j + (VEC > 1)] = q1;
+                        }
+                    T *y = place(a.qo, a.ko, a.qo_row, a.qo_head, a.ko_row, a.ko_head, h0 + n);
+                    store(v, y + c0, s0, a.in_place || (!turned && c0 < 2 * a.pairs));
+                    if (second) store(z, y + c1, s1, a.in_place || (!turned && c1 < 2 * a.pairs));
+                }
         }
     }
 
@@ -194,7 +207,7 @@ namespace vkhip {
         // Heads of a thread: as many as leave the card full, at most 4 (50176 rows of 40 heads of 128, bf16, 2, 4, 8, 10 of them: 201,
         // 193, 197, 206 us; neighbours 210, 187, 181, 186).
         const int64_t items = (int64_t) a.rows * a.heads * a.units, fill = 256 * 2048;
-        a.per   = (int) (items / fill < 1 ? 1 : items / fill > 4 ? 4 : items / fill);
+        a.per   = (int) (items / fill < 1 ? 1 : items / fill > kRotaryHeads ? kRotaryHeads : items / fill);
         a.slots = (int) ceil_div(a.heads, a.per);
         const int each = a.units * a.slots;
         a.block_rows   = each >= 256 ? 1 : 256 / each;
