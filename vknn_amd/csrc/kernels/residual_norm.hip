@@ -14,15 +14,25 @@ namespace vkhip {
         void          *h, *y;
         int            rows, dim, post, pre, mods, mod_rows;
         bool           in_place;
-        float          alpha, post_eps, pre_eps;
+        float          alpha, post_eps, pre_eps, each; // each: 1 / dim
         int64_t        x_row, r_row, h_row, y_row, mod_row;
     };
 
+    // A lane's number and its partner's: quad_perm of 1 and of 2 apart, then the other half of 8 and of 16 lanes mirrored.
+    template <int CTRL>
+    __device__ __forceinline__ float add_partner(float x) {
+        return x + __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), CTRL, 0xF, 0xF, true));
+    }
     // The sum over the threads of a row, in each of them.
     template <int GT>
     __device__ __forceinline__ float row_sum(float v, float *waves) {
-#pragma unroll
-        for (int o = 1; o < (GT < 64 ? GT : 64); o <<= 1) v += __shfl_xor(v, o);
+        v = add_partner<0x141>(add_partner<0x4E>(add_partner<0xB1>(v)));
+        if constexpr (GT > 8) v = add_partner<0x140>(v);
+        if constexpr (GT == 32) v += __shfl_xor(v, 16);
+        if constexpr (GT >= 64) {
+            const auto row = [&](int lane) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), lane)); };
+            v = (row(0) + row(16)) + (row(32) + row(48));
+        }
         if constexpr (GT > 64) {
             __syncthreads(); // the last sum has been read
             if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = v;
@@ -46,7 +56,7 @@ namespace vkhip {
         const int     t = RPB > 1 ? (int) threadIdx.x % GT : (int) threadIdx.x;
         const int64_t row = ((int64_t) blockIdx.y * gridDim.x + blockIdx.x) * RPB + (RPB > 1 ? (int) threadIdx.x / GT : 0);
         if (row >= a.rows) return; // the whole group
-        const int64_t m = a.mod ? clampi(a.mod[row], 0, a.mods - 1) : (a.mod_rows ? row / a.mod_rows : 0);
+        const int64_t m = a.mod ? clampi(a.mod[row], 0, a.mods - 1) : (a.mod_rows ? (int64_t) ((unsigned) row / (unsigned) a.mod_rows) : 0);
         const float   count = (float) a.dim;
         F             z[N];
         const auto    whole = [&](int i) { return (i * GT + t) * VEC; };
@@ -89,7 +99,7 @@ namespace vkhip {
             for (int i = 0; i < N; ++i)
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) sum = __builtin_fmaf(own(i, j), own(i, j), sum);
-            const float rstd = 1.f / __builtin_sqrtf(row_sum<GT>(sum, waves) / count + eps);
+            const float rstd = 1.f / __builtin_sqrtf(__builtin_fmaf(row_sum<GT>(sum, waves), a.each, eps));
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 F g, c;
@@ -225,7 +235,7 @@ int vkhip_residual_norm(const vkhip_residual_norm_desc *d, const void *x, const 
     a.x = x, a.r = r, a.gate = gate, a.scale = scale, a.shift = shift, a.mod = with_mod ? mod : nullptr, a.h = h, a.y = y;
     a.post_w = post_w, a.post_b = post_b, a.pre_w = pre_w, a.pre_b = pre_b;
     a.rows = d->rows, a.dim = d->dim, a.post = d->post, a.pre = d->pre, a.mods = d->mods, a.mod_rows = with_mod ? d->mod_rows : 0;
-    a.alpha = d->alpha, a.post_eps = d->post_eps, a.pre_eps = d->pre_eps;
+    a.alpha = d->alpha, a.post_eps = d->post_eps, a.pre_eps = d->pre_eps, a.each = 1.f / (float) d->dim;
     a.x_row = d->x_row, a.r_row = d->r_row, a.h_row = d->h_row, a.y_row = d->y_row, a.mod_row = d->mod_row;
     a.in_place = (h && (h == x || h == r)) || (y && (y == x || y == r));
     hipStream_t st = resolve_stream(s);
