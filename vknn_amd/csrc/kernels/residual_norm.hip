@@ -62,7 +62,13 @@ namespace vkhip {
         const auto    whole = [&](int i) { return (i * GT + t) * VEC; };
         const auto    in = [&](int i) { return whole(i) < a.dim; };
         const auto    at = [&](int i) { return RAGGED ? min(whole(i), a.dim - VEC) : whole(i); };
-        const auto    own = [&](int i, int j) { return RAGGED && j < whole(i) - at(i) ? 0.f : z[i][j]; }; // what counts
+        const auto    own = [&](int i) { // what counts of z[i]: by a branch, which few waves take
+            F c = z[i];
+            if (whole(i) + VEC > a.dim)
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) c[j] = RAGGED && j >= whole(i) - at(i) ? c[j] : 0.f;
+            return c;
+        };
         const auto    load = [&](const void *p, int64_t offset, int i) {
             const V v = *reinterpret_cast<const V *>((const T *) p + offset + at(i));
             return __builtin_convertvector(v, F);
@@ -85,20 +91,24 @@ namespace vkhip {
             if (kind == VKHIP_NORM_LAYER) {
                 float sum = 0.f;
 #pragma unroll
-                for (int i = 0; i < N; ++i)
+                for (int i = 0; i < N; ++i) {
+                    const F c = own(i);
 #pragma unroll
-                    for (int j = 0; j < VEC; ++j) sum += own(i, j);
+                    for (int j = 0; j < VEC; ++j) sum += c[j];
+                }
                 const float mean = row_sum<GT>(sum, waves) / count; // a row of one value has it as its mean, and no variance
 #pragma unroll
                 for (int i = 0; i < N; ++i)
 #pragma unroll
-                    for (int j = 0; j < VEC; ++j) z[i][j] = in(i) ? z[i][j] - mean : 0.f;
+                    for (int j = 0; j < VEC; ++j) z[i][j] -= mean;
             }
             float sum = 0.f;
 #pragma unroll
-            for (int i = 0; i < N; ++i)
+            for (int i = 0; i < N; ++i) {
+                const F c = own(i);
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) sum = __builtin_fmaf(own(i, j), own(i, j), sum);
+                for (int j = 0; j < VEC; ++j) sum = __builtin_fmaf(c[j], c[j], sum);
+            }
             const float rstd = 1.f / __builtin_sqrtf(__builtin_fmaf(row_sum<GT>(sum, waves), a.each, eps));
 #pragma unroll
             for (int i = 0; i < N; ++i) {
@@ -134,7 +144,7 @@ namespace vkhip {
                 for (int j = 0; j < VEC; ++j) g[j] = 1.f;
                 if (a.gate && in(i)) g = load(a.gate, m * a.mod_row, i);
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) z[i][j] = in(i) ? __builtin_fmaf(z[i][j] * a.alpha, g[j], r[i][j]) : 0.f;
+                for (int j = 0; j < VEC; ++j) z[i][j] = __builtin_fmaf(z[i][j] * a.alpha, g[j], r[i][j]);
             }
         } else {
 #pragma unroll
