@@ -601,7 +601,8 @@ int vkhip_kv_release(const vkhip_kv_cache *c, const vkhip_kv_pool *p, const int3
  * int32 [groups + 1], rising, clamped to [0, batch]) share the pages of the first tokens[g] tokens (device int32
  * [groups], rounded down to whole pages), which are read once for all of them, through the table of the first.
  * Sequences in no group share nothing. The result is that of vkhip_kv_attention but for rounding: what a query may
- * see goes by its own sequence's length, also inside the prefix.
+ * see goes by its own sequence's length, also inside the prefix. Value scales are 0 or more, as kv_append makes them
+ * (a NaN reaches the queries that see its page; a negative one may give NaN).
  * max_tokens: no prefix is longer (0: max_len); longer ones are read sequence by sequence from there on. max_tail: no
  * sequence has more tokens behind its prefix (0: max_len); it only sizes the launch. workspace as for
  * vkhip_kv_attention, from vkhip_kv_attention_shared_workspace_bytes. */

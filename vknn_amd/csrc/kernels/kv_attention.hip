@@ -313,7 +313,8 @@ namespace vkhip {
         __shared__ KvAttnLds<DJ, RT, NW> lds;
         kv_attention_body<T, DJ, RT, P32, NW, MODE>(a, blockIdx.x, blockIdx.y, blockIdx.z, lds);
     }
-    // Prefixes, in blocks of 32 rows, and tails side by side: the first a.prefix_blocks workgroups take the prefixes.
+    // Prefixes, in blocks of 32 rows, and tails side by side: the first a.prefix_blocks workgroups take the prefixes. 4 sequences
+    // behind 1024 tokens 9.1 us, 8.3 and 5.2 in two launches; 64 behind 4096 34.3, 21.6 and 14.3.
     template <typename T, int DJ, int RT, bool P32>
     __global__ __launch_bounds__(256, DJ == 1 ? 2 : 1) void kv_shared_kernel(KvAttnArgs a) {
         __shared__ union {

@@ -9,6 +9,11 @@
 // Weights are up to 2^15, as they are in the attention of one sequence, and rescaled where a row's maximum grows by more
 // than 2; a page's value scale goes into its weights' exponents, relative to the largest one so far, so that the products
 // of all pages add up in place (a page under 2^-8 of that, or not finite, takes a product of its own).
+//
+// Bound by instruction issue beside the products: 1024 rows behind 32768 tokens, 8 heads of 128, 155 us, 890 TFLOP/s (a
+// library product of 16384^3 1340); matrix units busy 42% of the time, vector units 48%, two waves a SIMD; start and end
+// of a workgroup, queries in and parts out, take about 10 us of it. Value scales are 0 or more, as kv_append makes them:
+// of a negative one the weights' exponents have no logarithm.
 #include "kv_attention.h"
 #include <type_traits>
 

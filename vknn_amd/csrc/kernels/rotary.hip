@@ -5,6 +5,9 @@
 // are lost at far positions, and no 64-bit floats are needed. The upper 32 bits go on to cosine and sine: the nearest
 // quarter turn is taken off as a whole number, the rest, within an eighth of a turn, goes into Taylor's series up to x^11
 // (its next terms are below 2^-34). One pair's sine and cosine serve all heads that a thread takes.
+//
+// Bound by memory where rows are many: 50176 rows of 40 heads of 128 bf16 183 us, 5.6 TB/s in and out; 45000 rows of 32 heads
+// of 64 fp16, neighbours, 65 us, 5.7 TB/s (partly from the caches). 64 rows 8.2 us, a launch and two loads in a row.
 #include "tokens.h"
 #include <math.h>
 
