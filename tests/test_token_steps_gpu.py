@@ -355,6 +355,16 @@ def shared_cache(sizes, prefixes, tails, page, heads, d, outside=0, seed=0, bloc
     return c, lens, cu
 
 
+def widen(c, rows, tiles):
+    """A table so wide that, as far as the host knows, prefixes of that many tokens times `rows` rows a sequence are worth tiles
+    of 128 or 256 rows (None: as it is)."""
+    if tiles:
+        work = 3 << 24 if c.d <= 64 else 3 << 22 if tiles == 128 else 1 << 24
+        c.blocks = max(c.blocks, work // (c.heads * c.batch * rows * c.page) + 1)
+        c.table = torch.cat([c.table, torch.full((c.batch, c.blocks - c.table.shape[1]), -1, dtype=torch.int32)], 1).contiguous()
+        c.gpu_table = Dev(c.table)
+
+
 def shared_attention(c, q, lens, cu, prefixes, dtype, scale, max_len=0, max_tokens=0, max_tail=0, stream=None, o_pad=0):
     """q [batch, t, heads, d]"""
     lib, (dt, code, _) = V.vkhip(), DT[dtype]
@@ -403,19 +413,21 @@ def test_shared_many_rows(gpu, sizes, hq, hkv, t, page, prefixes):
     for d, dtype in ((128, "f16"), (64, "bf16"), (88, "bf16")):
         c, lens, cu = shared_cache(sizes, prefixes, tails, page, hkv, d, seed=t)
         q = rand(10, len(lens), t, hq, d).to(DT[dtype][0]).float()
-        both_checks(c, q, lens, cu, prefixes, dtype, d ** -0.5, max_tokens=max(prefixes), max_tail=max(tails))
+        for tiles in (None, 128, 256) if d == 128 else (256,):
+            widen(c, hq // hkv * t, tiles)
+            both_checks(c, q, lens, cu, prefixes, dtype, d ** -0.5, max_tokens=0 if tiles else max(prefixes), max_tail=max(tails))
 
 
-# Prefixes of more than 2^20 rows x tokens, as far as the host knows, go to other kernels: a wide table is enough for it.
-@pytest.mark.parametrize("many,blocks,page,d", [(5, None, 64, 128), (60, None, 64, 128), (60, 40, 64, 128), (9, 120, 64, 128), (60, 40, 64, 64), (60, 80, 32, 128), (60, 80, 32, 72)])
-def test_shared_lengths_inside_the_prefix(gpu, many, blocks, page, d):
+@pytest.mark.parametrize("many,tiles,page,d", [(5, None, 64, 128), (60, None, 64, 128), (60, 256, 64, 128), (9, 128, 64, 128), (60, 128, 64, 64), (60, 256, 32, 128), (60, 128, 32, 72)])
+def test_shared_lengths_inside_the_prefix(gpu, many, tiles, page, d):
     """Sequences that have not reached their prefix's end, the first one's table naming it: they see what their length
     lets them. A length of nothing gives zeros, more query tokens than tokens give rows that see nothing."""
     heads, t = 2, 4
-    c, lens, cu = shared_cache([many], [512], [t] * many, page, heads, d, blocks=blocks)
+    c, lens, cu = shared_cache([many], [512], [t] * many, page, heads, d)
     for b in range(many):
         c.table[b] = c.table[0]  # all are the first's prefix
     c.gpu_table.put(c.table)
+    widen(c, t * 4, tiles)
     lens = [[512, 511, 0, 1, 3, 64, 65, 300, 449, 2][b % 10] for b in range(many)]
     q = rand(11, many, t, 8, d).half().float()
     out = shared_attention(c, q, lens, cu, [512], "f16", 0.09)
@@ -423,12 +435,13 @@ def test_shared_lengths_inside_the_prefix(gpu, many, blocks, page, d):
     assert (out[2] == 0).all() and (out[3][:3] == 0).all()
 
 
-@pytest.mark.parametrize("many,blocks,d", [(4, None, 64), (64, None, 64), (64, 40, 64), (64, 40, 128), (20, 120, 128)])
-def test_shared_spoiled_and_missing_pages(gpu, many, blocks, d):
+@pytest.mark.parametrize("many,tiles,d", [(4, None, 64), (64, None, 64), (64, 128, 64), (64, 256, 128), (20, 128, 128)])
+def test_shared_spoiled_and_missing_pages(gpu, many, tiles, d):
     """A prefix page of NaN scale reaches the queries that see it and no other; one without memory is seen by none; the
     tails' and the other group's pages stay their own."""
     page, heads = 64, 1
-    c, lens, cu = shared_cache([many, many], [256, 192], [5] * (2 * many), page, heads, d, seed=3, blocks=blocks)
+    c, lens, cu = shared_cache([many, many], [256, 192], [5] * (2 * many), page, heads, d, seed=3)
+    widen(c, 4, tiles)
     q = rand(12, 2 * many, 1, 4, d).half().float()
     clean = shared_attention(c, q, lens, cu, [256, 192], "f16", 0.125)
     for scales in (c.ks, c.vs):
@@ -452,14 +465,15 @@ def test_shared_spoiled_and_missing_pages(gpu, many, blocks, d):
         T.check_attention(out[b], q[b].double(), k, v, [1], [int(keep.sum())], True, "f16", 0.125)
 
 
-@pytest.mark.parametrize("sizes,hq", [([3, 20], 4), ([30, 200], 16)])
-def test_shared_hints_and_odd_prefixes(gpu, sizes, hq):
+@pytest.mark.parametrize("sizes,hq,tiles", [([3, 20], 4, None), ([20, 30], 16, 128), ([20, 30], 16, 256)])
+def test_shared_hints_and_odd_prefixes(gpu, sizes, hq, tiles):
     """Prefixes are whole pages; a smaller max_tokens leaves the rest to the tails, a smaller max_tail costs time alone,
     max_len cuts sequences; a wide table changes nothing."""
     page, heads, d = 64, 2, 128
     many = sum(sizes)
     c, lens, cu = shared_cache(sizes, [640, 192], [10 + b % 23 for b in range(many)], page, heads, d, seed=6, blocks=40)
     q = rand(13, many, 1, hq, d).half().float()
+    widen(c, hq // heads, tiles)
     for how in (dict(), dict(max_tokens=640, max_tail=32), dict(max_tokens=300), dict(max_tokens=64), dict(max_tokens=63), dict(max_tail=1), dict(max_len=700), dict(max_tokens=1 << 20)):
         for given in ([640, 192], [703, 193], [641, 255]):
             both_checks(c, q, lens, cu, given, "f16", 0.09, **how)
@@ -473,7 +487,8 @@ def test_shared_groups_out_of_range(gpu):
     """Ranges and prefixes that make no sense stay within the arrays, and sequences in no group are right."""
     c, lens, cu = shared_cache([4], [128], [20] * 4, 64, 1, 64, seed=7)
     q = rand(14, 4, 1, 2, 64).half().float()
-    wide, many, wcu = shared_cache([70], [128], [20] * 70, 64, 1, 64, seed=7, blocks=130)  # the same in wide tiles
+    wide, many, wcu = shared_cache([70], [128], [20] * 70, 64, 1, 64, seed=7)  # the same in wide tiles
+    widen(wide, 2, 128)
     wq = rand(14, 70, 1, 2, 64).half().float()
     for given in ([0, 1 << 30], [-7, 70], [5, 66]):
         for prefix in (128, 0, -64):
@@ -495,25 +510,27 @@ def test_shared_many_groups(gpu):
     both_checks(c, q, lens, cu, prefixes, "f16", 0.125)
 
 
-@pytest.mark.parametrize("many,blocks,d", [(2, None, 64), (40, None, 64), (40, 110, 64), (130, 40, 64), (60, 80, 128)])
-def test_shared_large_scores(gpu, many, blocks, d):
+@pytest.mark.parametrize("many,tiles,d", [(2, None, 64), (40, None, 64), (40, 128, 64), (130, 128, 64), (60, 256, 128)])
+def test_shared_large_scores(gpu, many, tiles, d):
     """bf16 queries beyond fp16's range, scores in the thousands, keys that grow along the prefix: maxima that move late."""
     page, heads = 64, 2
-    c, lens, cu = shared_cache([many], [1024], [30] * many, page, heads, d, seed=9, blocks=blocks)
+    c, lens, cu = shared_cache([many], [1024], [30] * many, page, heads, d, seed=9)
     ks = c.ks.get()
     ks[c.table[0, :16].long()] *= torch.linspace(0.1, 8, 16)[:, None]
     c.ks.put(ks)
+    widen(c, 4, tiles)
     q = (rand(16, many, 1, 8, d) * torch.tensor([1e-6, 1.0, 1e5, 1e9] * 2)[None, None, :, None]).bfloat16().float()
     for scale in (1e-9, 1e-5, 1.0):
         both_checks(c, q, lens, cu, [1024], "bf16", scale)
 
 
-@pytest.mark.parametrize("many,blocks,page,d", [(2, None, 64, 64), (40, None, 64, 64), (40, 110, 64, 64), (60, 80, 64, 128), (40, 220, 32, 64), (60, 160, 32, 128)])
-def test_shared_value_scales_far_apart(gpu, many, blocks, page, d):
+@pytest.mark.parametrize("many,tiles,page,d", [(2, None, 64, 64), (40, None, 64, 64), (40, 128, 64, 64), (60, 256, 64, 128), (40, 128, 32, 64), (60, 256, 32, 128), (20, 128, 32, 128)])
+def test_shared_value_scales_far_apart(gpu, many, tiles, page, d):
     """Pages of values many powers of two apart, and one of zeros: a small page that owns the weights keeps its digits
     beside a large one that has none."""
     heads = 1
-    c, lens, cu = shared_cache([many], [512], [3] * many, page, heads, d, seed=10, blocks=blocks)
+    c, lens, cu = shared_cache([many], [512], [3] * many, page, heads, d, seed=10)
+    widen(c, 4, tiles)
     vs, ks = c.vs.get(), c.ks.get()
     for i, f in enumerate([1.0, 2.0 ** -30, 2.0 ** 20, 0.0, 2.0 ** -60, 1.0, 2.0 ** 10, 1.0]):
         vs[int(c.table[0, i])] *= f
@@ -537,10 +554,11 @@ def test_shared_value_scales_far_apart(gpu, many, blocks, page, d):
                 assert ((out[b, :, h] - want).abs() / bound).max().item() <= 1, (own, b, h)
 
 
-@pytest.mark.parametrize("many,blocks,page,d", [(5, None, 64, 64), (40, 110, 64, 64), (60, 80, 64, 128), (40, 220, 32, 64)])
-def test_shared_pages_of_zeros(gpu, many, blocks, page, d):
+@pytest.mark.parametrize("many,tiles,page,d", [(5, None, 64, 64), (40, 128, 64, 64), (60, 256, 64, 128), (40, 128, 32, 64)])
+def test_shared_pages_of_zeros(gpu, many, tiles, page, d):
     """Pages whose keys, values or both are zeros: scores of nothing that still take their weight, and a prefix of such alone."""
-    c, lens, cu = shared_cache([many], [512], [3] * many, page, 1, d, seed=18, blocks=blocks)
+    c, lens, cu = shared_cache([many], [512], [3] * many, page, 1, d, seed=18)
+    widen(c, 4, tiles)
     vs, ks = c.vs.get(), c.ks.get()
     q = rand(19, many, 1, 4, d).half().float()
     for keys, values in (([1, 2, 7], [2, 5]), (range(512 // page), []), (range(512 // page), range(512 // page))):

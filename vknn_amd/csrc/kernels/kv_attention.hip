@@ -514,10 +514,13 @@ namespace vkhip {
         a.groups     = p->groups;
         a.max_prefix = p->max_tokens > 0 && p->max_tokens < whole.max_len ? p->max_tokens : whole.max_len;
         const int64_t each = p->groups > 0 ? (int64_t) c->batch * a.rows / p->groups : 0; // rows of a group
-        // Tiles of 128 or 256 rows (kv_prefix.hip) from about 2^20 rows x tokens on; below, their start, about 10 us, is what
-        // counts (32 heads on 8, D = 128, prefix pass and join in us, 32-row tiles / wide ones: 64 sequences behind 4096
-        // tokens 28 / 29, 128 behind 1024 22 / 24, 16 behind 4096 17 / 19; 256 behind 32768 590 / 170).
-        a.wide            = each <= 64 || (int64_t) c->batch * a.rows * a.max_prefix <= 1 << 20 ? 0 : each > 192 && a.c.row == 128 ? 2 : 1;
+        // Tiles of 128 or 256 rows (kv_prefix.hip) from 2^23 heads x rows x tokens on, of 64 channels, whose narrow tiles run twice as
+        // many at a time, from 3 * 2^24 on; below, their start, about 10 us, is what counts. Whole calls, us, 32-row tiles / wide ones: 8 x
+        // 256 x 4096 39.5 / 39.9, 1 x 400 x 16384 29 / 35, 8 x 512 x 4096 57 / 54; 64 channels, 4 x 768 x 8192 37 / 46, x 16384 55.2 /
+        // 55.5, 4 x 3072 x 4096 65 / 64, 1 x 12288 x 8192 112 / 79. 256 rows instead of 128 from 2^24 on: 8 x 256 x 4096 42.5 / 39.9, 8 x
+        // 512 x 4096 54.1 / 53.6, 8 x 1024 x 32768 157 / 166 (prefixes alone).
+        const int64_t work = (int64_t) c->kv_heads * c->batch * a.rows * a.max_prefix;
+        a.wide             = each <= 64 || work <= (a.c.row == 64 ? 3 << 24 : 1 << 23) ? 0 : each > 192 && a.c.row == 128 && work > 1 << 24 ? 2 : 1;
         const int height  = a.wide ? a.wide * kWideRows : 32;
         a.shared_blocks   = (int) ((int64_t) c->batch * a.rows / height + p->groups);
         const int wide_tiles = kWideUnits / (c->page_tokens == 32 ? 2 : 1);
