@@ -18,6 +18,7 @@
 // one's values: 64 x 2048 at D = 64, 80, 96, 128 27, 44, 43, 43 us. Loading the next step's keys and values while this
 // one's are multiplied gained nothing: it costs the registers of a third wave a SIMD, which does the same.
 #include "kv_attention.h"
+#include <type_traits>
 
 namespace vkhip {
 
@@ -355,6 +356,25 @@ namespace vkhip {
             const float  f = exp2_hw(s.x - base);
             sum += s.y * f;
             const int end = min(64, n - k0);
+            if constexpr (SHARED) {
+                // eight loads under way, of a rest four, the last ones of parts that are there already (5 parts of 720 rows 10.2 us with a
+                // loop's rest, 5.0; 28 of 2352 13.9, 9.0)
+                const auto some = [&](int i, auto n_c) __attribute__((always_inline)) {
+                    constexpr int SOME = decltype(n_c)::value;
+                    float2        y[SOME];
+#pragma unroll
+                    for (int j = 0; j < SOME; ++j) y[j] = *reinterpret_cast<const float2 *>(a.part_o + slot(k0 + min(i + j * WPR, end - 1)) * D + min(d, D - 2));
+#pragma unroll
+                    for (int j = 0; j < SOME; ++j) {
+                        const int   k = i + j * WPR;
+                        const float w = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), min(k, end - 1)));
+                        if (k < end) x.x += y[j].x * w, x.y += y[j].y * w;
+                    }
+                };
+                int i = part;
+                for (; i + 7 * WPR < end; i += 8 * WPR) some(i, std::integral_constant<int, 8>());
+                for (; i < end; i += 4 * WPR) some(i, std::integral_constant<int, 4>());
+            } else
 #pragma unroll 8
             for (int i = part; i < end; i += WPR) {
                 const float w = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), i));
