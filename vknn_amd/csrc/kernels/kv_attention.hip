@@ -537,7 +537,7 @@ namespace vkhip {
         // Tiles of 128 or 256 rows (kv_prefix.hip) from 2^23 heads x rows x tokens on, of 64 channels, whose narrow tiles run twice as
         // many at a time, from 3 * 2^24 on; below, their start, about 10 us, is what counts. Whole calls, us, 32-row tiles / wide ones: 8 x
         // 256 x 4096 39.5 / 39.9, 1 x 400 x 16384 29 / 35, 8 x 512 x 4096 57 / 54; 64 channels, 4 x 768 x 8192 37 / 46, x 16384 55.2 /
-        // 55.5, 4 x 3072 x 4096 65 / 64, 1 x 12288 x 8192 112 / 79. 256 rows instead of 128 from 2^24 on: 8 x 256 x 4096 42.5 / 39.9, 8 x
+        // 55.5, 4 x (256 sequences of 12) x 4096 65 / 64, 1 x 12288 x 8192 112 / 79. 256 rows instead of 128 from 2^24 on: 8 x 256 x 4096 42.5 / 39.9, 8 x
         // 512 x 4096 54.1 / 53.6, 8 x 1024 x 32768 157 / 166 (prefixes alone).
         const int64_t work = (int64_t) c->kv_heads * c->batch * a.rows * a.max_prefix;
         a.wide             = each <= 64 || work <= (a.c.row == 64 ? 3 << 24 : 1 << 23) ? 0 : each > 192 && a.c.row == 128 && work > 1 << 24 ? 2 : 1;
