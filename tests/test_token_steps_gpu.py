@@ -182,11 +182,11 @@ def test_rotary_special_values(gpu):
     assert torch.equal(out[~touched], clean[~touched]) and not torch.isfinite(out[touched]).any()
 
 
-@pytest.mark.parametrize("rows,hq,hk,d", [(70001, 6, 2, 64), (20000, 33, 0, 40)])
-def test_rotary_many_rows(gpu, rows, hq, hk, d):
-    """Enough rows for several heads a thread."""
+@pytest.mark.parametrize("rows,hq,hk,d,near", [(70001, 6, 2, 64, False), (20000, 33, 0, 40, False), (20000, 14, 2, 128, False), (20000, 14, 2, 128, True), (20000, 20, 1, 90, True)])
+def test_rotary_many_rows(gpu, rows, hq, hk, d, near):
+    """Enough rows for several heads a thread and, of whole lines, to pass the caches."""
     q, k = rand(6, rows, hq, d), rand(7, rows, hk, d) if hk else None
-    how = dict(sections=[d // 4, d // 4], dtype="bf16")
+    how = dict(sections=[d // 4, d // 2 - d // 4], dtype="bf16", near=near)
     pos = np.stack([np.arange(rows) // 100, np.arange(rows) % 100])
     a, b = rotary(q, k, pos, **how)
     check_rotary(a, q, pos, **how)
@@ -719,7 +719,7 @@ def test_residual_norm_spoiled_row(gpu):
         assert torch.equal(a[keep], b[keep]) and torch.isnan(b[4]).all()
 
 
-@pytest.mark.parametrize("dim,dtype", [(5, "bf16"), (8, "bf16"), (88, "bf16"), (200, "f16"), (2048, "bf16")])
+@pytest.mark.parametrize("dim,dtype", [(5, "bf16"), (8, "bf16"), (88, "bf16"), (200, "f16"), (2047, "f16"), (2048, "bf16")])
 def test_residual_norm_many_rows(gpu, dim, dtype):
     """More rows than run at once: every one is written, as its own."""
     rows = 20011
@@ -814,3 +814,50 @@ def test_step_on_a_stream_of_its_own_and_as_a_graph(gpu):
         T.check_kv_attention(got[0][2].view(n, many, hq, d).double(), c, got[0][3].view(n, many, hq, d).float(), [m + many for m in lens], "f16", 0.125)
     check(lib.vkhip_graph_destroy(g))
     check(lib.vkhip_stream_destroy(s))
+
+
+@pytest.mark.parametrize("tiles", [None, 256])
+def test_shared_calls_side_by_side_and_replayed(gpu, tiles):
+    """Two calls under way on streams of their own, and both as graphs, give bit for bit what each gives alone, with
+    workspaces that hold anything."""
+    lib, page, heads, d, many, t = V.vkhip(), 64, 2, 128, 60, 2
+    calls = []
+    for seed in (31, 32):
+        c, lens, cu = shared_cache([many], [1024], [t + b % 70 for b in range(many)], page, heads, d, seed=seed)
+        widen(c, 4 * t, tiles)
+        q = rand(seed, many, t, 4 * heads, d).half()
+        alone = shared_attention(c, q.float(), lens, cu, [1024], "f16", 0.09)
+        desc = V.KvAttentionDesc(q_heads=4 * heads, q_tokens=t, dtype=0, max_len=0, scale=0.09, q_row=4 * heads * d, q_head=d, o_row=4 * heads * d, o_head=d)
+        cd, dq, n, dc, dp, out = c.desc(), Dev(q), ints(lens), ints(cu), ints([1024]), full((many, t, 4 * heads, d), 7.0, torch.float16)
+        p = V.KvPrefix(cu=dc.data_ptr(), tokens=dp.data_ptr(), groups=1, max_tokens=0, max_tail=0)
+        ws, s, g = workspace(lib.vkhip_kv_attention_shared_workspace_bytes(R(desc), R(cd), R(p))), ctypes.c_void_p(), ctypes.c_void_p()
+        check(lib.vkhip_stream_create(ctypes.byref(s)))
+        calls.append((alone, desc, cd, p, dq, n, out, ws, s, g, (c, dc, dp)))
+    sync()
+
+    def launch(call):
+        _, desc, cd, p, dq, n, out, ws, s, _, _ = call
+        check(lib.vkhip_kv_attention_shared(R(desc), R(cd), R(p), dq.data_ptr(), n.data_ptr(), out.data_ptr(), ws.data_ptr(), s))
+
+    def same():
+        for call in calls:
+            check(lib.vkhip_stream_sync(call[8]))
+        for alone, *_, out, _, _, _, _ in calls:
+            assert torch.equal(out.get().double(), alone)
+            out.put(torch.full(out.shape, 7.0, dtype=torch.float16))
+        sync()
+    for _ in range(3):
+        for call in calls:
+            launch(call)
+        same()
+    for call in calls:
+        check(lib.vkhip_graph_begin(call[8]))
+        launch(call)
+        check(lib.vkhip_graph_end(call[8], ctypes.byref(call[9])))
+    for _ in range(4):
+        for call in calls:
+            check(lib.vkhip_graph_launch(call[9], call[8]))
+        same()
+    for call in calls:
+        check(lib.vkhip_graph_destroy(call[9]))
+        check(lib.vkhip_stream_destroy(call[8]))
