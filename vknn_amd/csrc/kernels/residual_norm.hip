@@ -183,7 +183,7 @@ namespace vkhip {
         return nullptr;
     }
 
-    constexpr int64_t kNormPast = (int64_t) 64 << 20; // bytes of x from which rows pass the caches
+    constexpr int64_t kNormPast = (int64_t) 64 << 20; // bytes of x from which rows pass the caches (50000 of 1101 bf16 128 us, in them 139)
 
     template <typename T, int VEC, int N, int GT>
     static void residual_norm_start(const NormArgs &a, hipStream_t s) {
