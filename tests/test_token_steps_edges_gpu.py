@@ -1,0 +1,69 @@
+"""The operators of a token step at their edges: workspaces past 2^31 parts, long prefixes in wide tiles, value scales at
+the ends of the number range, launches of very many groups, pages that several sequences name. Against float64, with the
+bounds of test_token_steps_gpu.py."""
+import copy
+import ctypes
+
+import pytest
+
+import test_token_steps_gpu as S
+import test_tokens_gpu as T
+import vknn_amd as V
+from test_tokens_gpu import Dev, full, ints, rand, sync
+from vknn_amd import DeviceBuffer, check
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+R = ctypes.byref
+
+
+class Shared:
+    """A call of the attention behind shared prefixes whose workspace says how the host has cut it."""
+
+    def __init__(self, c, q, lens, cu, prefixes, dtype, scale, **hints):
+        (self.dt, code, _), (b, t, hq, d) = T.DT[dtype], q.shape
+        self.c, self.q, self.lens, self.dtype, self.scale, self.shape = c, q, lens, dtype, scale, (b, t, hq, d)
+        self.desc = V.KvAttentionDesc(q_heads=hq, q_tokens=t, dtype=code, scale=scale, q_row=hq * d, q_head=d, o_row=hq * d, o_head=d)
+        self.cd, self.keep = c.desc(), [ints(cu), ints(prefixes)]
+        self.prefix = V.KvPrefix(cu=self.keep[0].data_ptr(), tokens=self.keep[1].data_ptr(), groups=len(cu) - 1, **hints)
+        self.bytes = V.vkhip().vkhip_kv_attention_shared_workspace_bytes(R(self.desc), R(self.cd), R(self.prefix))
+        self.rows = hq // c.heads * t
+        self.parts = self.bytes // (4 * (d + 2))
+        self.splits = self.parts // (b * c.heads * self.rows)  # of a row: of the prefix and of the tail
+
+    def run(self, workspace=None):
+        dq, n, out = Dev(self.q.to(self.dt)), ints(self.lens), full(self.shape, 7.0, self.dt)
+        ws = workspace or T.workspace(self.bytes)
+        sync()
+        check(V.vkhip().vkhip_kv_attention_shared(R(self.desc), R(self.cd), R(self.prefix), dq.data_ptr(), n.data_ptr(), out.data_ptr(), getattr(ws, "ptr", None) or ws.data_ptr(), None), "shared")
+        sync()
+        return out.get().double()
+
+    def check(self, out, ids=None):
+        """All sequences, or some of them."""
+        ids = list(range(len(self.lens))) if ids is None else ids
+        some = copy.copy(self.c)
+        some.table = self.c.table[ids]
+        T.check_kv_attention(out[ids], some, self.q[ids], [self.lens[i] for i in ids], self.dtype, self.scale)
+
+
+def widen_table(c, blocks):
+    """The same pages in a table of that many blocks a sequence."""
+    table = torch.full((c.batch, blocks), -1, dtype=torch.int32)
+    table[:, :c.blocks] = c.table
+    c.table, c.blocks, c.gpu_table = table, blocks, Dev(table)
+
+
+def test_shared_more_than_2_31_parts(gpu):
+    """A table so wide that a workspace holds more parts than 31 bits number: the last sequence's rows have theirs behind
+    the 2^31st. (The workspace, 86 GB, is not cleared: what is read of it has been written.)"""
+    many, t, hq, d = 128, 64, 64, 8
+    c, lens, cu = S.shared_cache([many], [128], [1 + b % 60 for b in range(many)], 64, 1, d, seed=21)
+    widen_table(c, 1 << 20)
+    q = rand(22, many, t, hq, d).half().float()
+    call = Shared(c, q, lens, cu, [128], "f16", 0.35, max_tail=64)
+    assert call.parts > 1 << 31 and (many - 1) * call.rows * call.splits < 1 << 31
+    ws = DeviceBuffer(call.bytes)
+    out = call.run(ws)
+    del ws
+    call.check(out, [0, 1, many - 2, many - 1])

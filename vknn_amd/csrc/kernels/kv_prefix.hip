@@ -384,8 +384,9 @@ namespace vkhip {
         l += __shfl_xor(l, 32);
         l *= 1.f / (1 << kWeightBits); // the products have it in their values
         const int3 me = row_of(again(lane));
-        const int  at = me.z ? (int) ((((int64_t) me.x * a.c.heads + head) * a.rows + me.y) * (a.shared_splits + a.splits) + split) : -1; // fewer than 2^31 parts
-        if (h == 0 && at >= 0) *reinterpret_cast<float2 *>(a.part_s + (int64_t) at * 2) = make_float2(m, l);
+        // 64 bits: a wide table alone makes 2^31 parts, however few of them a call has
+        const int64_t at = me.z ? (((int64_t) me.x * a.c.heads + head) * a.rows + me.y) * (a.shared_splits + a.splits) + split : -1;
+        if (h == 0 && at >= 0) *reinterpret_cast<float2 *>(a.part_s + at * 2) = make_float2(m, l);
         // through LDS, 64 channels at a time, so that rows leave in whole lines (4 of 11 us for a call of 4 tiles otherwise)
         __syncthreads();
         unsigned char *own = (wave < NW / 2 ? sm_k[0] : sm_v[0]) + wave % (NW / 2) * 8192;
@@ -401,8 +402,8 @@ namespace vkhip {
             for (int i = 0; i < 8; ++i) {
                 const int     row = 4 * i + (lane >> 4), piece = lane & 15, ch = 64 * e + 4 * piece;
                 const float4v x = *reinterpret_cast<const float4v *>(own + row * 256 + ((piece ^ (row & 15)) << 4));
-                const int     to = __shfl(at, row);
-                if (to >= 0 && ch < D) *reinterpret_cast<float4v *>(a.part_o + (int64_t) to * D + ch) = x;
+                const int64_t to = __shfl((long long) at, row);
+                if (to >= 0 && ch < D) *reinterpret_cast<float4v *>(a.part_o + to * D + ch) = x;
             }
         }
 #endif
