@@ -67,3 +67,32 @@ def test_shared_more_than_2_31_parts(gpu):
     out = call.run(ws)
     del ws
     call.check(out, [0, 1, many - 2, many - 1])
+
+
+@pytest.mark.parametrize("many,tiles,page,d", [(4, None, 64, 64), (60, 128, 64, 64), (60, 256, 64, 128), (60, 128, 32, 64), (20, 128, 32, 128), (60, 256, 32, 128), (20, 128, 64, 128)])
+@pytest.mark.parametrize("small,large", [(2.0 ** -60, 2.0 ** 30), (2.0 ** -70, 2.0 ** 70), (2.0 ** -100, 2.0 ** 90), (2.0 ** -100, 1.0), (1.0, 3e37 * 16)])
+def test_shared_value_scales_at_both_ends(gpu, many, tiles, page, d, small, large):
+    """A prefix whose pages have value scales 2^90 to 2^230 apart, all but the last the small ones: sequences that end in
+    front of the last page have what a call without it gives, and those that see it no NaN. Scales are put at most at 4e37
+    to 3e38, past 2^126 (values of which bf16 has no numbers: those sequences are compared in front of it alone)."""
+    c, lens, cu = S.shared_cache([many], [512], [3] * many, page, 1, d, seed=23)
+    for b in range(many):
+        c.table[b] = c.table[0]
+    c.gpu_table.put(c.table)
+    S.widen(c, 4, tiles)
+    vs = c.vs.get()
+    first, last = c.table[0, :512 // page - 1].long(), int(c.table[0, 512 // page - 1])
+    vs[first] *= small
+    vs[last] = (vs[last].clamp(max=0.5).double() * large).float()  # the factor alone may be past fp32's largest number
+    c.vs.put(vs)
+    assert (vs[first] > 2.0 ** -116).all() and torch.isfinite(vs[last]).all()
+    end = 512 - page
+    lens = [[end, end - 1, 1, 65, 300, 512, 500, 2][b % 8] for b in range(many)]
+    q = rand(24, many, 1, 4, d).bfloat16().float()
+    call = Shared(c, q, lens, cu, [512], "bf16", 0.125)
+    out = call.run()
+    seen = [b for b in range(many) if lens[b] > end]
+    call.check(out, [b for b in range(many) if b not in seen])
+    assert not torch.isnan(out[seen]).any()
+    if large < 1e30:
+        call.check(out, seen)

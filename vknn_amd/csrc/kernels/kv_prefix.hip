@@ -7,8 +7,10 @@
 // 0-3 8-11 | 4-7 12-15. Bytes become fp16 once for the four waves, on their way from memory through registers into LDS,
 // a tile of 64 tokens ahead.
 // Weights are up to 2^15, as they are in the attention of one sequence, and rescaled where a row's maximum grows by more
-// than 2; a page's value scale goes into its weights' exponents, relative to the largest one so far, so that the products
-// of all pages add up in place (a page under 2^-8 of that, or not finite, takes a product of its own).
+// than 2; a page's value scale goes into its weights' exponents, relative to a power of two at or above the largest of the
+// workgroup's span (2^10 at most, which scales of fp16 rows stay under), so that the products of all pages add up in place. A
+// page under 2^-8 of that, or above it, takes products of its own, which are multiplied by its scale in fp32. Weights of a
+// page are thus lost from 2^-30 of a row's largest on where its scale is 2^-8 of the span's, from 2^-38 on otherwise.
 //
 // Bound by instruction issue beside the products: 1024 rows behind 32768 tokens, 8 heads of 128, 155 us, 890 TFLOP/s (a
 // library product of 16384^3 1340); matrix units busy 42% of the time, vector units 48%, two waves a SIMD; start and end
@@ -40,7 +42,7 @@ namespace vkhip {
         constexpr int AHEAD = 6, ROWS = 32 * NW; // operands read in front of their products; rows of a workgroup
         constexpr int UNIT  = P32 ? 32 : kStep;                                  // tokens of one page, as many as a tile takes
         __shared__ __attribute__((aligned(1024))) unsigned char sm_k[2][kStep * ROW], sm_v[2][kStep * ROW];
-        __shared__ float4v unit[256]; // of a unit's page: key scale; vref to its unit (0: zeros, NaN: no number); log2 of its value scale to that, and back
+        __shared__ float4v unit[256]; // of a unit's page: key scale; factor of its products (NaN: its value scale is no number); log2 of the one of its weights, and back
         __shared__ int     unit_id[256];
         __shared__ float   wave_vs[NW];
         const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = lane >> 5, col = lane & 31, tid = threadIdx.x;
@@ -61,7 +63,7 @@ namespace vkhip {
         };
         // What the loop needs of pages it finds in LDS, for 256 units of tokens at a time (a tile, or half of one where pages
         // are smaller): a scalar load would make every wait for LDS a wait for memory.
-        float vref = 0x1p-126f; // the scale that O is in units of: a power of two, no page's so far was larger
+        float vref = 0x1p-126f; // the scale that O is in units of, a power of two
         float16v acc[DB];
         int   unit_page = -1; // this thread's unit
         float unit_ks = 0.f, unit_vs = 0.f;
@@ -78,22 +80,22 @@ namespace vkhip {
         };
         const auto settle = [&] {
             const float ks = unit_ks, vs = unit_vs;
-            float       larger = vs <= 0x1p126f ? vs : 0.f;
+            const bool  number = vs >= 0.f && vs < __builtin_inff();
+            float       larger = number ? vs : 0.f;
 #pragma unroll
             for (int o = 1; o < 64; o <<= 1) larger = fmaxf(larger, __shfl_xor(larger, o));
             if (lane == 0) wave_vs[wave] = larger;
             __syncthreads();
 #pragma unroll
             for (int i = 0; i < 4; ++i) larger = fmaxf(larger, wave_vs[i]);
-            vref = fmaxf(__uint_as_float((__float_as_uint(larger) + 0x7FFFFFu) & 0x7F800000u), 0x1p-126f);
-            // a page far below the largest has a unit of its own, a power of two under vref that O takes for its tile; a page
-            // of zeros or of a scale that is no number is dealt with there too
-            const bool none = vs == 0.f, lost = !(vs <= vref), plain = none || lost || vs >= vref * 0x1p-8f;
-            const float up = __uint_as_float((__float_as_uint(vs) + 0x7FFFFFu) & 0x7F800000u), under = plain ? 1.f : fminf(vref / up, 0x1p64f);
-            const float ratio = none || lost ? 1.f : vs / (vref / under);
+            vref = fminf(fmaxf(__uint_as_float((__float_as_uint(larger) + 0x7FFFFFu) & 0x7F800000u), 0x1p-126f), 0x1p10f);
+            // a page near it has its share in its weights, any other beside its products: vref is no more than 2^10, so that this
+            // factor is as good as the scale itself, however large the scale of a page is that some rows do not see
+            const float ratio = vs / vref;
+            const bool  near  = ratio >= 0x1p-8f && ratio <= 1.f;
             if (tid >= 256) return;
-            unit_id[tid] = unit_page < 0 ? -1 : none || lost || !plain || !(ks > 0.f) ? unit_page | 0x40000000 : unit_page;
-            unit[tid]    = float4v {ks, none ? 0.f : lost ? __builtin_nanf("") : under, __builtin_amdgcn_logf(ratio), 1.f / ratio};
+            unit_id[tid] = unit_page < 0 ? -1 : near && ks > 0.f ? unit_page : unit_page | 0x40000000;
+            unit[tid]    = float4v {ks, near ? 1.f : number ? ratio : __builtin_nanf(""), near ? __builtin_amdgcn_logf(ratio) : 0.f, near ? 1.f / ratio : 1.f};
         };
         // the names of the pages of tile i of those in LDS, the same in every lane
         const auto names = [&](int i) {
@@ -212,40 +214,37 @@ namespace vkhip {
 
         // Round i of a wave: the products O += V P of tile i - 1 and S = K Q of tile i, beside them K of tile i + 1 and V of
         // tile i into LDS, whose places tiles i - 1 and i - 2 have left; then the exponentials of tile i, and a barrier.
-        const auto in_units = [&](float by) __attribute__((always_inline)) {
-            __asm__ volatile("" : "+v"(by));
-#pragma unroll
-            for (int d = 0; d < DB; ++d)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) acc[d][r] *= by;
-        };
         const auto values = [&](int i, int2 n, int place) __attribute__((always_inline)) {
             const unsigned at = va + place * (kStep * 2 * DP);
-            const bool     odd = odd_page(n);
-            float          of = 1.f;
             const auto     product = [&](int k) __attribute__((always_inline)) {
 #pragma unroll
                 for (int d = 0; d < DB; ++d)
                     acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const half8 *>(sm_v[0] + (at ^ k << 5) + d * (32 * kStep * 2)), pf[k], acc[d], 0, 0, 0);
             };
-            const auto none = [&](int k) __attribute__((always_inline)) {
+            if (odd_page(n)) { // page by page, and nothing of them left for the others; a row that sees one of no number has weights of none
 #pragma unroll
-                for (int j = 0; j < 8; ++j) pf[k][j] = (half_t) 0.f;
-            };
-            if (odd) {
-                const float u0 = unit[i * (kStep / UNIT)][1], u1 = unit[P32 ? i * 2 + 1 : i][1], of0 = u0 > 0.f ? u0 : 1.f;
-                of = u1 > 0.f ? u1 : 1.f;
-                if (u0 == 0.f) none(0), none(1); // whatever the bytes of a page of zeros are
-                if (u1 == 0.f) none(2), none(3);
-                in_units(of0);
-                if (P32 && of0 != of) { // the first page by itself
-                    product(0), product(1), none(0), none(1);
-                    in_units(of / of0);
+                for (int u = 0; u < (P32 ? 2 : 1); ++u) {
+                    const float scale = unit[again(P32 ? i * 2 + u : i)][1], f = scale > 0.f ? scale : 0.f;
+#pragma unroll
+                    for (int d = 0; d < DB; ++d) {
+                        float16v x;
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) x[r] = 0.f;
+#pragma unroll
+                        for (int k = P32 ? 2 * u : 0; k < (P32 ? 2 * u + 2 : 4); ++k)
+                            x = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const half8 *>(sm_v[0] + (at ^ k << 5) + d * (32 * kStep * 2)), pf[k], x, 0, 0, 0);
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) acc[d][r] = __builtin_fmaf(x[r], f, acc[d][r]);
+                        __builtin_amdgcn_sched_barrier(0); // one product's registers at a time
+                    }
                 }
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) pf[k][j] = (half_t) 0.f;
             }
 #pragma unroll
             for (int k = 0; k < 4; ++k) product(k);
-            return 1.f / of;
         };
         const auto scores = [&](int place) __attribute__((always_inline)) {
             const unsigned at = ka + place * (kStep * ROW);
@@ -367,11 +366,10 @@ namespace vkhip {
                 constexpr int ODD = decltype(odd_c)::value;
                 weights(i, before);
                 barrier();
-                const float back = values(i, before, ODD);
+                values(i, before, ODD);
                 scores(ODD ^ 1); // behind the last tile its scores are formed again, for nobody
                 stage_k(sm_k[ODD], kr), stage_v(sm_v[ODD ^ 1]);
                 beside(std::integral_constant<int, 4 * DB + 2 * KS>());
-                if (odd_page(before)) in_units(back);
                 ahead(i + 1);
             };
 #pragma unroll 1
