@@ -96,3 +96,31 @@ def test_shared_value_scales_at_both_ends(gpu, many, tiles, page, d, small, larg
     assert not torch.isnan(out[seen]).any()
     if large < 1e30:
         call.check(out, seen)
+
+
+def filled(batch, blocks, page, d, seed):
+    """A cache of one head whose pages hold any bytes, with scales as of ordinary rows."""
+    c = T.Cache(batch, blocks, page, 1, d, seed)
+    for i, scales in enumerate((c.ks, c.vs)):
+        scales.put(torch.rand(scales.shape, generator=torch.Generator().manual_seed(seed + i)) * 0.02 + 0.005)
+    return c
+
+
+# groups that together have more than 65535 blocks of 32 rows, and ones whose wide tiles would be that many; more groups
+# than sequences: those of three have four empty ones behind them
+@pytest.mark.parametrize("batch,hq,t,sizes,height", [(32000, 1, 32, [1] * 7 + [3, 0, 0, 0, 0], 32), (16000, 8, 64, [8], 128)])
+def test_shared_very_many_groups(gpu, batch, hq, t, sizes, height):
+    page, d, cu = 32, 8, [0]
+    while cu[-1] < batch:
+        cu += [min(batch, cu[-1] + sum(sizes[:i + 1])) for i in range(len(sizes))]
+    c = filled(batch, 3, page, d, 25)
+    for lo, hi in zip(cu, cu[1:]):
+        if hi - lo > 1:
+            c.table[lo:hi, 0] = c.table[lo, 0]
+    c.gpu_table.put(c.table)
+    lens = [page + 1 + b % 63 for b in range(batch)]
+    q = rand(26, batch, t, hq, d).half().float()
+    call = Shared(c, q, lens, cu, [page * (g % 9 > 0) for g in range(len(cu) - 1)], "f16", 0.35, max_tokens=page, max_tail=70)
+    assert batch * hq * t // height + len(cu) - 1 > 65535
+    out = call.run(DeviceBuffer(call.bytes))
+    call.check(out, [0, 1, 7, 8, 9, 10, batch // 2, batch - 9, batch - 2, batch - 1])

@@ -541,8 +541,10 @@ namespace vkhip {
         // 512 x 4096 54.1 / 53.6, 8 x 1024 x 32768 157 / 166 (prefixes alone).
         const int64_t work = (int64_t) c->kv_heads * c->batch * a.rows * a.max_prefix;
         a.wide             = each <= 64 || work <= (a.c.row == 64 ? 3 << 24 : 1 << 23) ? 0 : each > 192 && a.c.row == 128 && work > 1 << 24 ? 2 : 1;
+        const auto blocks = [&](int height) { return (int64_t) c->batch * a.rows / height + p->groups; };
+        if (a.wide && blocks(a.wide * kWideRows) > 65535) a.wide = 0; // more than the third dimension of their grid; the narrow ones' has one
         const int height  = a.wide ? a.wide * kWideRows : 32;
-        a.shared_blocks   = (int) ((int64_t) c->batch * a.rows / height + p->groups);
+        a.shared_blocks   = (int) blocks(height);
         const int wide_tiles = kWideUnits / (c->page_tokens == 32 ? 2 : 1);
         if (a.wide && a.max_prefix > 4096 * wide_tiles * kStep) a.max_prefix = 4096 * wide_tiles * kStep; // 4096 splits; the rest with the tails
         const int     round = (a.wide ? 1 : 4) * kStep; // tokens that a workgroup takes at a time
@@ -557,9 +559,13 @@ namespace vkhip {
         if (a.wide && splits < ceil_div(rounds, wide_tiles)) splits = ceil_div(rounds, wide_tiles);
         a.shared_span   = (int) (ceil_div(rounds, splits) * round);
         a.shared_splits = (int) ceil_div(a.max_prefix > 0 ? a.max_prefix : 1, a.shared_span);
-        const int64_t prefixes = (int64_t) c->kv_heads * a.shared_splits * a.shared_blocks, tails = (int64_t) c->kv_heads * a.blocks * c->batch * a.splits;
-        a.prefix_blocks = prefixes + tails < 0x7FFF0000 ? (int) prefixes : -1; // -1: more than a launch numbers
+        const int64_t prefixes = (int64_t) c->kv_heads * a.shared_splits * blocks(height), tails = (int64_t) c->kv_heads * a.blocks * c->batch * a.splits;
+        a.prefix_blocks = a.wide ? 0 : prefixes + tails < 0x7FFF0000 ? (int) prefixes : -1; // -1: more than a launch numbers
         return a;
+    }
+    // What no launch holds, nor the rows of a group 31 bits.
+    static const char *kv_shared_too_many(const KvAttnArgs &a) {
+        return (int64_t) a.c.heads * a.blocks > 65535 || (int64_t) a.c.batch * a.rows > 0x7FFFFF00 || a.prefix_blocks < 0 ? "too many heads, sequences and query tokens" : nullptr;
     }
     static bool kv_nothing_shared(const KvAttnArgs &a) { return a.groups == 0 || a.max_prefix < a.c.page_tokens; }
 
@@ -595,6 +601,7 @@ size_t vkhip_kv_attention_shared_workspace_bytes(const vkhip_kv_attention_desc *
     if (kv_shared_refusal(d, c, p)) return 0;
     const KvAttnArgs a = kv_shared_cut(d, c, p);
     if (kv_nothing_shared(a)) return vkhip_kv_attention_workspace_bytes(d, c);
+    if (kv_shared_too_many(a)) return 0;
     return (size_t) c->batch * c->kv_heads * a.rows * (a.shared_splits + a.splits) * (c->head_dim + 2) * sizeof(float);
 }
 
@@ -610,9 +617,9 @@ int vkhip_kv_attention_shared(const vkhip_kv_attention_desc *d, const vkhip_kv_c
     if (!q || !lens || !o) return set_error(VKHIP_ERR_INVALID, what, "null pointer");
     if (misaligned16(q) || misaligned16(o) || misaligned16(workspace) || ((uintptr_t) lens) % 4) return set_error(VKHIP_ERR_INVALID, what, "misaligned pointer");
     if (kv_nothing_shared(a)) return vkhip_kv_attention(d, c, q, lens, o, workspace, s);
+    if (const char *why = kv_shared_too_many(a)) return set_error(VKHIP_ERR_INVALID, what, why);
     if (c->pages == 0) a.max_len = a.max_prefix = 0; // no block has memory: every query gives zeros
     if (!workspace) return set_error(VKHIP_ERR_INVALID, what, "null pointer");
-    if ((int64_t) c->kv_heads * a.blocks > 65535 || a.shared_blocks > 65535 || a.prefix_blocks < 0) return set_error(VKHIP_ERR_INVALID, what, "too many heads, sequences and query tokens");
     a.q = q, a.o = o, a.lens = lens, a.part_o = (float *) workspace, a.scale = d->scale, a.cu = p->cu, a.prefix = p->tokens;
     a.part_s = a.part_o + (size_t) c->batch * c->kv_heads * a.rows * (a.shared_splits + a.splits) * c->head_dim;
     a.q_row = d->q_row, a.q_head = d->q_head, a.o_row = d->o_row, a.o_head = d->o_head;
