@@ -124,3 +124,16 @@ def test_shared_very_many_groups(gpu, batch, hq, t, sizes, height):
     assert batch * hq * t // height + len(cu) - 1 > 65535
     out = call.run(DeviceBuffer(call.bytes))
     call.check(out, [0, 1, 7, 8, 9, 10, batch // 2, batch - 9, batch - 2, batch - 1])
+
+
+def test_reserve_of_no_sequences(gpu):
+    """The sums have one entry, which is 0; the list, where there is one, stays."""
+    for pool in (V.KvPool(), None):
+        free, state, cu, pos = ints([3, 1, 2, 0]), ints([4, 9]), ints([-9, -9]), ints([-9])
+        pool = pool or V.KvPool(free=free.data_ptr(), state=state.data_ptr(), capacity=4)
+        cache = V.KvCache(pages=4, page_tokens=64, kv_heads=1, head_dim=64, batch=0, max_blocks=2)
+        sync()
+        check(V.vkhip().vkhip_kv_reserve(R(cache), R(pool), None, None, 1, cu.data_ptr(), None, pos.data_ptr(), None, None))
+        sync()
+        assert cu.get().tolist() == [0, -9] and pos.get().tolist() == [-9]
+        assert free.get().tolist() == [3, 1, 2, 0] and state.get().tolist() == [4, 9]

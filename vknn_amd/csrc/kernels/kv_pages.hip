@@ -55,9 +55,10 @@ namespace vkhip {
     __global__ __launch_bounds__(kSeqs) void kv_reserve_kernel(KvPageArgs a) {
         __shared__ int waves[kSeqs / 64], row_from[kSeqs], block_from[kSeqs], first_block[kSeqs], held[kSeqs];
         const int tid = threadIdx.x, most = a.max_blocks << a.page_shift;
+        if (tid == 0) a.cu[0] = 0;
+        if (a.batch == 0) return; // there may be no list either
         const int left = clampi(a.state[0], 0, a.capacity);
         int       rows = 0, taken = 0; // of the sequences before
-        if (tid == 0) a.cu[0] = 0;
         for (int b0 = 0; b0 < a.batch; b0 += kSeqs) {
             const int b = b0 + tid, n = min(kSeqs, a.batch - b0);
             // what does not fit the remaining rows is cut, here by halves, so that the sum stays within 32 bits
@@ -168,13 +169,13 @@ int vkhip_kv_reserve(const vkhip_kv_cache *c, const vkhip_kv_pool *p, const int3
                      int32_t *pos, int64_t *slot, vkhip_stream_t s) {
     if (const char *why = kv_pages_refusal(c, p, lens, add)) return set_error(VKHIP_ERR_INVALID, "kv_reserve: %s", why);
     if (total < 0 || total >= 1 << 30) return set_error(VKHIP_ERR_INVALID, "kv_reserve: total is not 0 .. 2^30 - 1");
-    if (c->batch == 0) return VKHIP_OK;
+    if (c->batch == 0 && !cu) return VKHIP_OK;
     if (!cu) return set_error(VKHIP_ERR_INVALID, "kv_reserve: null pointer");
     if (((uintptr_t) cu | (uintptr_t) now | (uintptr_t) pos) % 4 || (uintptr_t) slot % 8) return set_error(VKHIP_ERR_INVALID, "kv_reserve: misaligned pointer");
-    if (now == lens || now == add || cu == lens || cu == add) return set_error(VKHIP_ERR_INVALID, "kv_reserve: an output is an input");
+    if (c->batch > 0 && (now == lens || now == add || cu == lens || cu == add)) return set_error(VKHIP_ERR_INVALID, "kv_reserve: an output is an input");
     KvPageArgs a = kv_page_args(c, p, lens, add);
     a.cu = cu, a.now = now, a.pos = pos, a.slot = slot, a.total = total;
-    const bool rows = (pos || slot) && total > 0;
+    const bool rows = (pos || slot) && total > 0 && c->batch > 0;
     a.few           = rows && total <= 8 * kSeqs;
     kv_reserve_kernel<<<1, kSeqs, 0, resolve_stream(s)>>>(a);
     int rc = check_launch("kv_reserve");
