@@ -9,6 +9,7 @@
 // Bound by memory where rows are many: 50176 rows of 40 heads of 128 bf16 183 us, 5.6 TB/s in and out; 45000 rows of 32 heads
 // of 64 fp16, neighbours, 65 us, 5.7 TB/s (partly from the caches). 64 rows 8.2 us, a launch and two loads in a row.
 #include "tokens.h"
+#include <algorithm>
 #include <math.h>
 
 namespace vkhip {
@@ -171,6 +172,16 @@ namespace vkhip {
         }
     }
 
+    // Frequencies that rotary_pairs takes: of 10^6 and more the whole turns would leave its digits too few of the rest.
+    constexpr double kRotaryFreq = 1e6;
+
+    // The largest frequency that theta gives: with a theta under 1 the last pair's of its axis.
+    static double rotary_largest(const vkhip_rotary_desc *d) {
+        int n = d->rotary_dim / 2;
+        if (d->spectra) n = *std::max_element(d->sections, d->sections + d->axes);
+        return d->theta >= 1.0 ? 1.0 : pow(d->theta, -(n - 1.0) / n);
+    }
+
     static bool rotary_strides(int64_t row, int64_t head) { return row >= 0 && head >= 0 && row <= (int64_t) 1 << 31 && head <= (int64_t) 1 << 40; }
 
     // Whether an output's heads lie apart within its rows, or its rows within its heads.
@@ -252,9 +263,10 @@ int vkhip_rotary(const vkhip_rotary_desc *d, const int32_t *pos, const double *f
     RotaryArgs a {};
     a.pairs = d->rotary_dim / 2;
     if (!freq && !(d->theta > 0.0 && d->theta < 1e30)) return set_error(VKHIP_ERR_INVALID, "rotary: theta is not positive");
+    if (!freq && !(rotary_largest(d) < kRotaryFreq)) return set_error(VKHIP_ERR_INVALID, "rotary: theta gives a frequency of 10^6 or more");
     if (freq)
         for (int i = 0; i < a.pairs; ++i)
-            if (!(fabs(freq[i]) < 1e6)) return set_error(VKHIP_ERR_INVALID, "rotary: a frequency is not finite or 10^6 or more");
+            if (!(fabs(freq[i]) < kRotaryFreq)) return set_error(VKHIP_ERR_INVALID, "rotary: a frequency is not finite or 10^6 or more");
     if (d->rows == 0) return VKHIP_OK;
     const bool with_k = d->k_heads > 0;
     if (!pos || !q || !qo || (with_k && (!k || !ko))) return set_error(VKHIP_ERR_INVALID, "rotary: null pointer");
