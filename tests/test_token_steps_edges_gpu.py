@@ -137,3 +137,33 @@ def test_reserve_of_no_sequences(gpu):
         sync()
         assert cu.get().tolist() == [0, -9] and pos.get().tolist() == [-9]
         assert free.get().tolist() == [3, 1, 2, 0] and state.get().tolist() == [4, 9]
+
+
+@pytest.mark.parametrize("near", [False, True])
+def test_rotary_small_angles_keep_their_digits(gpu, near):
+    """The pair (1, 0) becomes (cos, sin): a slow pair's sine is good to a few units of itself, not of the turn. The float of
+    the angle is rounded from its halves, their factors and their sum (4 * 2^-24 of itself), the series in fp32 (another 3), its
+    product and the output (1 each); 9 * 2^-24 in all, beside what a frequency rounded to 2^-64 turns adds a position."""
+    at, n, theta = [1, -1, 3, 7, -20, 1000, 4096, -65537, 200000, 2 ** 24 + 1], 64, 1e6
+    q = torch.zeros(len(at), 1, 2 * n)
+    q[:, :, 0:2 * n:2 if near else 1][:, :, :n] = 1.0
+    out, _ = S.rotary(q, None, [at], sections=[n], dtype="f32", near=near, theta=theta)
+    sine = out[:, 0, 1::2] if near else out[:, 0, n:]
+    cosine = out[:, 0, 0::2] if near else out[:, 0, :n]
+    pos = torch.tensor(at, dtype=torch.float64)[:, None]
+    angle = pos * theta ** (-torch.arange(n, dtype=torch.float64) / n)
+    slow = angle.abs() < 0.75
+    assert slow.sum() > 300 and (angle[slow].abs() < 1e-5).any()
+    off = (sine.double() - torch.sin(angle)).abs() / (9 * S.F32 * torch.sin(angle).abs() + pos.abs() * 2.0 ** -62 + 1e-38)
+    assert off[slow].max() <= 1, off[slow].max()
+    assert ((cosine.double() - torch.cos(angle)).abs()[slow] <= 9 * S.F32).all()
+
+
+@pytest.mark.parametrize("theta", [0.5, 1e-3, 2e-6])
+def test_rotary_theta_under_one(gpu, theta):
+    """Frequencies that rise from 1: whole turns a position."""
+    q = rand(31, 70, 2, 64)
+    pos = [list(range(-20, 50)), list(range(3, 700, 10))]
+    how = dict(sections=[20, 12], dtype="f32", theta=theta)
+    out, _ = S.rotary(q, None, pos, **how)
+    S.check_rotary(out, q, pos, **how)

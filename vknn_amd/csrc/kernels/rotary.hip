@@ -1,10 +1,12 @@
 // Rotary positions with several axes: pairs of channels of query and key rows turned by the row's positions.
 //
 // Angles are kept as fractions of a turn in 64 bits: a pair's frequency is f 2^64 / 2 pi rounded to a whole number, the
-// angle its product with the position modulo 2^64, which is the fraction of the turn but for position * 2^-65: no bits
-// are lost at far positions, and no 64-bit floats are needed. The upper 32 bits go on to cosine and sine: the nearest
-// quarter turn is taken off as a whole number, the rest, within an eighth of a turn, goes into Taylor's series up to x^11
-// (its next terms are below 2^-34). One pair's sine and cosine serve all heads that a thread takes.
+// angle its product with the position modulo 2^64, which is the fraction of the turn but for position * 2^-65: whole
+// turns fall off by themselves, and no 64-bit floats are needed. The nearest quarter turn is taken off as a whole number; the
+// rest, within an eighth of a turn, becomes a float from both halves of its 64 bits, so that small angles keep their digits
+// (the upper half alone has 2^-32 of a turn: sines of the slowest pairs at theta 10^6 were off by 3e-4 of themselves), and
+// goes into Taylor's series, the sine's up to x^11 (next term 2^-37), the cosine's up to x^10 (next 2^-33). One pair's sine
+// and cosine serve all heads that a thread takes.
 //
 // Bound by memory where rows are many: 50176 rows of 40 heads of 128 bf16 183 us, 5.6 TB/s in and out; 45000 rows of 32 heads
 // of 64 fp16, neighbours, 65 us, 5.7 TB/s (partly from the caches). 64 rows 8.2 us, a launch and two loads in a row.
@@ -32,8 +34,10 @@ namespace vkhip {
     };
 
     __device__ __forceinline__ void turn_of(uint64_t freq, int pos, float &c, float &s) {
-        const unsigned at = (unsigned) (freq * (uint64_t) (int64_t) pos >> 32), quarter = (at + 0x20000000u) >> 30;
-        const float    x = (float) (int) (at - (quarter << 30)) * (6.283185307179586f / 4294967296.f), z = x * x;
+        const uint64_t turn = freq * (uint64_t) (int64_t) pos;
+        const int      low = (int) (unsigned) turn; // as a number of its own, so that it takes nothing from a small high half
+        const unsigned high = (unsigned) (turn >> 32) + ((unsigned) low >> 31), quarter = (high + 0x20000000u) >> 30;
+        const float    x = __builtin_fmaf((float) low, 0x1.921fb6p+2f * 0x1p-64f, (float) (int) (high - (quarter << 30)) * (0x1.921fb6p+2f * 0x1p-32f)), z = x * x;
         float          sx = __builtin_fmaf(z, -1.f / 39916800, 1.f / 362880), cx = __builtin_fmaf(z, -1.f / 3628800, 1.f / 40320);
         sx = __builtin_fmaf(sx, z, -1.f / 5040);
         cx = __builtin_fmaf(cx, z, -1.f / 720);
