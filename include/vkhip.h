@@ -593,8 +593,11 @@ int vkhip_kv_reserve(const vkhip_kv_cache *c, const vkhip_kv_pool *p, const int3
 /* The pages behind the first keep[b] of the lens[b] tokens of each sequence go back to the list (all with keep 0;
  * rejected drafts; what lies behind a shared prefix): blocks ceil(keep / page_tokens) .. ceil(lens / page_tokens),
  * the first of them on top, so that a reserve of the same takes them back. Their table entries become -1; entries
- * that name no page are passed over, and pages that the list has no room for are dropped. A page goes back
- * once: where several sequences name it, one of them gives it. */
+ * that name no page are passed over, and pages that the list has no room for are dropped.
+ * The call does not look for a page that several sequences name, nor whether it is on the list already: giving it
+ * back once is the caller's duty, or the list holds it twice and two sequences get it. Of those that share a prefix all
+ * but the last that ends keep it (keep at least its tokens); the entries that stay in an ended one's row are the
+ * others', and a sequence that begins there with a length of 0 writes over them. */
 int vkhip_kv_release(const vkhip_kv_cache *c, const vkhip_kv_pool *p, const int32_t *lens, const int32_t *keep, vkhip_stream_t s);
 
 /* vkhip_kv_attention where sequences share their first tokens' pages: neighbouring sequences cu[g] .. cu[g+1] (device

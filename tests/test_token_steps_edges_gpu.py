@@ -167,3 +167,93 @@ def test_rotary_theta_under_one(gpu, theta):
     how = dict(sections=[20, 12], dtype="f32", theta=theta)
     out, _ = S.rotary(q, None, pos, **how)
     S.check_rotary(out, q, pos, **how)
+
+
+def test_pages_of_a_shared_prefix_go_back_once(gpu):
+    """Members of a group end one after the other, the first one first, and draft tokens are taken back between: all but the
+    last keep the shared prefix, whose pages then come back with the last one, and the list never names a page twice."""
+    page, shared, batch = 32, 3, 5
+    p = S.Pool(batch, 8, page, 40, seed=9)
+    prefix = shared * page
+    now = p.reserve([0] * batch, [prefix] + [0] * (batch - 1), prefix)
+    for b in range(1, batch):  # the program names the first one's pages for the others
+        p.table[b][:shared] = p.table[0][:shared]
+    p.gpu_table.put(torch.tensor(p.table, dtype=torch.int32))
+    lens = p.reserve([prefix] * batch, [5, 70, 33, 1, 64], 173)
+    left = list(range(batch))
+    for b in (0, 3, 1, 4, 2):
+        drafts = [3 if i in left else 0 for i in range(batch)]
+        now = p.reserve(lens, drafts, sum(drafts))
+        p.release(now, lens)
+        left.remove(b)
+        keep = [n if i != b else prefix if left else 0 for i, n in enumerate(lens)]
+        p.release(lens, keep)
+        lens = [n if i in left else 0 for i, n in enumerate(keep)]  # what is kept of an ended one's row is the others'
+        held = {e for i in left for e in p.table[i] if e >= 0}
+        assert len(set(p.free)) == len(p.free) and not held & set(p.free) and len(held) + len(p.free) == 40
+    # the rows of the table are free for others, whatever they still name
+    now = p.reserve([0] * batch, [2 * page] * batch, 2 * page * batch)
+    taken = [e for row in p.table for e in row[:2]]
+    assert len(set(taken)) == 2 * batch and not set(taken) & set(p.free)
+
+
+def test_steps_of_drafts_behind_a_shared_prefix(gpu):
+    """Steps of drafted tokens as they would be run: pages, rows into the cache, attention, the rejected tokens' pages back;
+    the first two eager, the others replays of one graph, with the program's lengths and rows put in between."""
+    lib, page, hkv, hq, d, n, drafts, pre = V.vkhip(), 64, 2, 4, 64, 5, 4, 128
+    c, lens, cu = S.shared_cache([n], [pre], [63, 1, 62, 100, 125], page, hkv, d, seed=12, blocks=8)
+    count = [-(-m // page) for m in lens]
+    used = {int(v) for b in range(n) for v in c.table[b, :count[b]]}
+    free = [i for i in range(c.pages) if i not in used][:14]
+    for b in range(n):
+        c.table[b, count[b]:] = -1
+    c.gpu_table.put(c.table)
+    rows = n * drafts
+    q, att = full((rows, hq * d), 0.0, torch.float16), full((rows, hq * d), 9.0, torch.float16)
+    k, v = (full((rows, hkv * d), 0.0, torch.float16) for _ in range(2))
+    was, add, now, keep, dcu = ints(lens), ints([drafts] * n), ints([0] * n), ints([0] * n), ints([0] * (n + 1))
+    dfree, state, dc, dp = ints(free), ints([len(free), 0]), ints(cu), ints([pre])
+    pool, cd = V.KvPool(free=dfree.data_ptr(), state=state.data_ptr(), capacity=len(free)), c.desc()
+    kr = V.KvRows(dtype=0, total=rows, k_row=hkv * d, k_head=d, v_row=hkv * d, v_head=d)
+    ad = V.KvAttentionDesc(q_heads=hq, q_tokens=drafts, dtype=0, max_len=page * 8, scale=0.125, q_row=hq * d, q_head=d, o_row=hq * d, o_head=d)
+    pf = V.KvPrefix(cu=dc.data_ptr(), tokens=dp.data_ptr(), groups=1, max_tokens=pre, max_tail=300)
+    ws, s, g = T.workspace(lib.vkhip_kv_attention_shared_workspace_bytes(R(ad), R(cd), R(pf))), ctypes.c_void_p(), ctypes.c_void_p()
+    check(lib.vkhip_stream_create(ctypes.byref(s)))
+
+    def chain():
+        check(lib.vkhip_kv_reserve(R(cd), R(pool), was.data_ptr(), add.data_ptr(), rows, dcu.data_ptr(), now.data_ptr(), None, None, s))
+        check(lib.vkhip_kv_append(R(cd), R(kr), k.data_ptr(), v.data_ptr(), dcu.data_ptr(), was.data_ptr(), s))
+        check(lib.vkhip_kv_attention_shared(R(ad), R(cd), R(pf), q.data_ptr(), now.data_ptr(), att.data_ptr(), ws.data_ptr(), s))
+        check(lib.vkhip_kv_release(R(cd), R(pool), now.data_ptr(), keep.data_ptr(), s))
+    check(lib.vkhip_graph_begin(s))
+    chain()
+    check(lib.vkhip_graph_end(s, ctypes.byref(g)))
+    for i in range(7):
+        taken = [(b + i) % (drafts + 1) for b in range(n)]  # none, some or all of the drafts
+        kept = [m + t for m, t in zip(lens, taken)]
+        was.put(torch.tensor(lens, dtype=torch.int32))
+        keep.put(torch.tensor(kept, dtype=torch.int32))
+        for t, salt in ((q, 1), (k, 2), (v, 3)):
+            t.put(rand(40 + 3 * i + salt, *t.shape).half())
+        sync()
+        if i < 2:
+            chain()
+        else:
+            check(lib.vkhip_graph_launch(g, s))
+        check(lib.vkhip_stream_sync(s))
+        table = c.table.clone()
+        for b in range(n):  # the pages as the attention had them
+            for j in range(-(-lens[b] // page), -(-(lens[b] + drafts) // page)):
+                table[b, j] = free.pop()
+        c.table = table.clone()
+        T.check_kv_attention(att.get().view(n, drafts, hq, d).double(), c, q.get().view(n, drafts, hq, d).float(), [m + drafts for m in lens], "f16", 0.125)
+        back = []
+        for b in range(n):
+            for j in range(-(-kept[b] // page), -(-(lens[b] + drafts) // page)):
+                back.append(int(table[b, j]))
+                table[b, j] = -1
+        free += back[::-1]
+        c.table, lens = table, kept
+        assert torch.equal(c.gpu_table.get(), table) and state.get().tolist() == [len(free), 0] and dfree.get().tolist()[:len(free)] == free
+    check(lib.vkhip_graph_destroy(g))
+    check(lib.vkhip_stream_destroy(s))
