@@ -257,3 +257,74 @@ def test_steps_of_drafts_behind_a_shared_prefix(gpu):
         assert torch.equal(c.gpu_table.get(), table) and state.get().tolist() == [len(free), 0] and dfree.get().tolist()[:len(free)] == free
     check(lib.vkhip_graph_destroy(g))
     check(lib.vkhip_stream_destroy(s))
+
+
+def long_cache(heads, d, page, tokens, many, tail, seed):
+    """One prefix of that many tokens for all, a page or two behind it for each; any bytes, scales as of ordinary rows, so
+    that nothing is appended and the table alone is large."""
+    blocks = tokens // page + 2
+    c = T.Cache.__new__(T.Cache)
+    c.page, c.heads, c.d, c.dp, c.batch, c.blocks, c.pages = page, heads, d, V.vkhip().vkhip_kv_row(d), many, blocks, tokens // page + 2 * many
+    g = torch.Generator().manual_seed(seed)
+    names = torch.randperm(c.pages, generator=g).int()
+    c.table = torch.empty((many, blocks), dtype=torch.int32)
+    c.table[:, :-2] = names[:blocks - 2]
+    c.table[:, -2:] = names[blocks - 2:].view(many, 2)
+    c.gpu_table = Dev(c.table)
+    c.k, c.v = (Dev(torch.randint(-127, 128, (c.pages, heads) + shape, generator=g, dtype=torch.int8)) for shape in ((page, c.dp), (c.dp, page)))
+    c.ks, c.vs = (Dev(torch.rand((c.pages, heads), generator=g) * 0.02 + 0.005) for _ in range(2))
+    return c, [tokens + tail(b) for b in range(many)]
+
+
+# Tiles of 128 rows for 64 channels (512 places on the card) and of 256 for 128 (256): one workgroup takes 256 tiles of 64
+# tokens at most, 128 with pages of 32, and as many rows as fill the places leave it all that it may hold.
+LONG = [(128, 64, 16384, 1, "f16"), (128, 64, 16384 + 64, 2, "f16"), (128, 64, 32768 - 192, 2, "bf16"), (128, 32, 8192, 1, "f16"), (128, 32, 8192 + 32, 2, "bf16"), (128, 32, 16384 - 32, 2, "f16"),
+        (64, 64, 16384, 1, "bf16"), (64, 128, 32768 - 128, 2, "f16"), (64, 32, 8192, 1, "f16"), (64, 32, 16384 + 32, 3, "f16"), (96, 256, 16384, 1, "f16"), (40, 64, 16384 + 128, 2, "f16")]
+
+
+@pytest.mark.parametrize("d,page,tokens,splits,dtype", LONG)
+def test_shared_long_spans_in_wide_tiles(gpu, d, page, tokens, splits, dtype):
+    """Workgroups that hold as many tiles as they can: full lists of pages, accumulation over hundreds of tiles, and spans that
+    the limit splits although the rows alone fill the card. Some sequences end inside the prefix, at the last tile's first
+    and last token among them."""
+    heads, many, hq, t = 4, 32, 64, 32  # 512 rows a sequence, 16384 of a group and head
+    c, lens = long_cache(heads, d, page, tokens, many, lambda b: 30 + b, d + page)
+    span = -(-(tokens // 64) // splits) * 64
+    lens[3:9] = [t, tokens, tokens - 1, tokens - 63, min(tokens, span + 5), min(tokens, span) - 1]
+    q = rand(41, many, t, hq, d).to(T.DT[dtype][0]).float()
+    call = Shared(c, q, lens, [0, many], [tokens], dtype, d ** -0.5, max_tokens=tokens, max_tail=80)
+    assert call.splits == splits + 1  # the tail has one
+    out = call.run(DeviceBuffer(call.bytes))
+    # a few heads and rows of some sequences, the keys' sum being long: the bound's terms for weights under fp16's smallest go
+    # by the number of tokens, as everywhere
+    for b in (0, 3, 4, 5, 6, 7, 8, many - 1):
+        (kq, ks), (vq, vs) = c.bytes_of(b, lens[b])
+        for h in (0, hq - 1):
+            one = h * heads // hq
+            k, v = ((x[:, one:one + 1].double() * s[:, one:one + 1, None]) for x, s in ((kq, ks), (vq, vs)))
+            extra = 0.0 if dtype == "f16" else d * 2.0 ** -25
+            T.check_attention(out[b][:, h:h + 1], q[b][:, h:h + 1].double(), k, v, [t], [lens[b]], True, dtype, d ** -0.5, weights_dtype="f16", extra=extra)
+
+
+@pytest.mark.parametrize("d,hq", [(128, 64), (64, 512)])
+def test_shared_wide_tiles_of_a_cut_prefix(gpu, d, hq):
+    """max_tokens under the prefix, on a page's border and not: wide tiles take it up to there, each sequence the rest."""
+    heads, many, tokens = 8, 64, 4096
+    c, lens = long_cache(heads, d, 64, tokens, many, lambda b: 1 + b, 42)
+    q = rand(43, many, 1, hq, d).half().float()
+    for most in (tokens - 64, tokens - 1, tokens // 2 + 640 + 31):
+        assert heads * many * hq // heads * (most // 64 * 64) > (1 << 23 if d == 128 else 3 << 24)
+        call = Shared(c, q, lens, [0, many], [tokens], "f16", d ** -0.5, max_tokens=most, max_tail=tokens - most + 64 + many)
+        call.check(call.run(), [0, 17, many - 1])
+
+
+def test_shared_wide_tiles_of_many_groups(gpu):
+    """More groups than a wave has lanes, each with rows for wide tiles, empty ones between them."""
+    heads, d, hq, t, page = 4, 128, 32, 4, 64
+    sizes = [0 if g % 11 == 5 else 1 + g % 6 for g in range(90)]
+    prefixes = [page * (1 + g % 9) for g in range(90)]
+    c, lens, cu = S.shared_cache(sizes, prefixes, [t + b % 60 for b in range(sum(sizes))], page, heads, d, seed=44)
+    assert heads * sum(sizes) * hq // heads * t * max(prefixes) > 1 << 24 and sum(sizes) * hq // heads * t // 90 > 64
+    q = rand(45, len(lens), t, hq, d).half().float()
+    call = Shared(c, q, lens, cu, prefixes, "f16", d ** -0.5, max_tokens=max(prefixes), max_tail=64)
+    call.check(call.run(), list(range(0, len(lens), 7)) + [len(lens) - 1])
