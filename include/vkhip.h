@@ -545,7 +545,8 @@ int    vkhip_kv_attention(const vkhip_kv_attention_desc *d, const vkhip_kv_cache
 /* ---------------------------------------------------------------- a token step of many requests
  * What stands between the products and the cache of a step: positions of rows, pages for them, attention
  * that reads a shared prompt once, and the norms around a block. No counterpart in the reference's
- * backends; forward only; strides in elements; arithmetic in fp32, outputs rounded once, to nearest even. */
+ * backends; forward only; strides in elements; positions and norms in fp32 arithmetic, outputs rounded once, to nearest
+ * even; what else the attention rounds stands with it. */
 
 /* Rotary positions with up to four axes (time, height, width): the first rotary_dim channels of every head
  * of q and k, in pairs, are turned by an angle that belongs to the row and the pair:
@@ -556,11 +557,12 @@ int    vkhip_kv_attention(const vkhip_kv_attention_desc *d, const vkhip_kv_cache
  *           interleaved, dealt to the axes in turn, past those that have theirs.
  *   freq:   host doubles, one a pair, read before the call returns; NULL: theta^(-i / n) over all n pairs or, with
  *           spectra, theta^(-j / n_axis) for pair j of its axis. theta is not used beside freq.
- *   pos:    device int32 [axes][rows], pos_axis elements from one axis to the next; any value (angles are
- *           reduced exactly: they are as good at 2^31 as at 0).
- * F16, BF16 or F32; head_dim up to 256, rotary_dim even; any strides that keep the rows of qo and ko apart, so that
- * rows may be slices of wider ones. qo may be q and ko k where their strides agree; otherwise nothing may
- * overlap. k_heads of 0: no k. */
+ *   pos:    device int32 [axes][rows], pos_axis elements from one axis to the next; any value: whole turns come off
+ *           without error. An angle is off by a few 2^-24 of what is left of it within an eighth of a turn; each
+ *           position adds up to 2^-62 of a turn and, without freq, 2^-57 of the angle that it takes.
+ * Frequencies are under 10^6, given or, with a theta under 1, made. F16, BF16 or F32; head_dim up to 256, rotary_dim
+ * even; rows may be slices of wider ones: of qo and ko the heads lie apart within a row's place, or the rows within a
+ * head's. qo may be q and ko k where their strides agree; otherwise nothing may overlap. k_heads of 0: no k. */
 typedef struct vkhip_rotary_desc {
     int32_t rows, q_heads, k_heads, head_dim, rotary_dim, dtype;
     int32_t neighbours, axes, sections[4], interleaved, spectra;
@@ -582,7 +584,8 @@ typedef struct vkhip_kv_pool {
  *   table: the blocks that the new tokens begin, ceil(lens / page_tokens) .. ceil((lens + add) / page_tokens),
  *          sequence by sequence, take the list's pages from its end; those that find none become -1 (a
  *          block without memory). Other entries stay. The table is written although the struct has it const.
- *   cu:    int32 [batch + 1], sums of add up to `total`: the rows of each sequence, as kv_append takes them.
+ *   cu:    int32 [batch + 1], sums of add up to `total`: the rows of each sequence, as kv_append takes them (cu[0] = 0 also
+ *          with a batch of 0, where it may be NULL).
  *   now:   int32 [batch], lens + rows: what kv_attention takes behind kv_append. Not lens itself.
  *   pos, slot: of each row its token's position, int32 [total], and its place in the cache, int64 [total],
  *          page * page_tokens + token in the page (-1: no memory). Rows from cu[batch] on are not written.
@@ -604,11 +607,17 @@ int vkhip_kv_release(const vkhip_kv_cache *c, const vkhip_kv_pool *p, const int3
  * int32 [groups + 1], rising, clamped to [0, batch]) share the pages of the first tokens[g] tokens (device int32
  * [groups], rounded down to whole pages), which are read once for all of them, through the table of the first.
  * Sequences in no group share nothing. The result is that of vkhip_kv_attention but for rounding: what a query may
- * see goes by its own sequence's length, also inside the prefix. Value scales are 0 or more, as kv_append makes them
- * (a NaN reaches the queries that see its page; a negative one may give NaN).
+ * see goes by its own sequence's length, also inside the prefix. In both, scores, weights' sums and products add up in
+ * fp32; a weight is rounded to fp16 before it multiplies values (their sum is not), and lost under 2^-38 of its row's
+ * largest, or 2^-30 in a page whose value scale is 2^-8 of those beside it; of a bf16 query what lies under 2^-24 of its
+ * largest channel is lost. Value scales are 0 or more and finite, as kv_append makes them (a NaN reaches the queries that
+ * see its page; a negative or infinite one may give NaN).
  * max_tokens: no prefix is longer (0: max_len); longer ones are read sequence by sequence from there on. max_tail: no
  * sequence has more tokens behind its prefix (0: max_len); it only sizes the launch. workspace as for
- * vkhip_kv_attention, from vkhip_kv_attention_shared_workspace_bytes. */
+ * vkhip_kv_attention, from vkhip_kv_attention_shared_workspace_bytes (0 also for a call that is refused: more than 2^31
+ * rows a head, 65535 blocks of heads and rows, or 65535 groups).
+ * The prefix costs two launches at least: up to about 4000 tokens of 4 sequences, or 1000 of 64, vkhip_kv_attention on the
+ * same tables takes less time. */
 typedef struct vkhip_kv_prefix {
     const int32_t *cu, *tokens;
     int32_t        groups, max_tokens, max_tail;
@@ -621,6 +630,7 @@ int    vkhip_kv_attention_shared(const vkhip_kv_attention_desc *d, const vkhip_k
  *   h = r + alpha * gate[m] * N_post(x),  y = N_pre(h) * (1 + scale[m]) + shift[m]
  * N_post and N_pre: VKHIP_NORM_NONE (the values), _RMS (z / sqrt(mean z^2 + eps) * w + b) or _LAYER ((z - mean) /
  * sqrt(var + eps) * w + b, biased variance); w and b fp32 [dim], NULL = 1 and 0. N_pre takes h before it is rounded.
+ * Squares are formed and added in fp32: the values of a normed row stay under about 2^63 / sqrt(dim).
  *   x NULL: h = r; r NULL: h = the block's part alone (not both). h or y may be NULL: not written (not both).
  *   gate, scale, shift: vectors of dtype, `mods` of them, mod_row elements apart, or NULL: 1, 0, 0. Row i uses
  *           vector m = mod[i] (device int32 [rows], clamped to the vectors) or, with mod NULL, i / mod_rows.

@@ -9,7 +9,10 @@
 // int8 becomes fp16 exactly; a page's key scale multiplies its scores, its value scale the fp32 product of the
 // page. Weights are rounded to fp16, whose smallest step is 2^-24: a row's reference is 14 below its largest exponent,
 // so that its largest weight is 2^14 and what is lost lies under 2^-39 of it (a row of many small weights beside one
-// large one keeps them), and values come as multiples of 2^-14 in return, at no cost.
+// large one keeps them), and values come as multiples of 2^-14 in return, at no cost. This rounding is the largest beside
+// that of the output, half a step of fp16 a weight: 64 sequences on 4096 shared tokens are off by 2.6e-4 (norm of the error
+// to the result's) in fp16, where fp32 weights leave 2.1e-4; 256 on 32768 in bf16 by 1.67e-3, and 1.66e-3. Both products in
+// fp32 would run at a sixteenth of the matrix units' rate, a second product for the weights' rest at half of it.
 // The tokens of a sequence are split over workgroups and a workgroup's four waves; partial results
 // (reference, sum, product) join in LDS and, across workgroups, in a second kernel.
 //
@@ -374,12 +377,12 @@ namespace vkhip {
                 int i = part;
                 for (; i + 7 * WPR < end; i += 8 * WPR) some(i, std::integral_constant<int, 8>());
                 for (; i < end; i += 4 * WPR) some(i, std::integral_constant<int, 4>());
-            } else
-#pragma unroll 8
-            for (int i = part; i < end; i += WPR) {
-                const float w = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), i));
-                const float2 y = *reinterpret_cast<const float2 *>(a.part_o + slot(k0 + i) * D + min(d, D - 2));
-                x.x += y.x * w, x.y += y.y * w;
+            } else {
+                for (int i = part; i < end; i += WPR) {
+                    const float  w = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), i));
+                    const float2 y = *reinterpret_cast<const float2 *>(a.part_o + slot(k0 + i) * D + min(d, D - 2));
+                    x.x += y.x * w, x.y += y.y * w;
+                }
             }
         }
 #pragma unroll
@@ -479,6 +482,19 @@ namespace vkhip {
 
     constexpr int kWideLeast = 4; // tiles of a workgroup, if the prefix has them
 
+    // A prefix takes tiles of 128 or 256 rows (kv_prefix.hip) where groups have more than kWideGroup rows a head on average and
+    // heads x rows x tokens are more than this; below, the start of a wide tile's workgroup, about 10 us, is what counts, and
+    // of 64 channels narrow tiles run twice as many at a time. Whole calls, us, 32-row tiles / wide ones:
+    //   128 channels: 8 x 256 x 4096 (2^23) 39.5 / 39.9, 1 x 400 x 16384 29 / 35 (2^22.6), 8 x 512 x 4096 (2^24) 57 / 54
+    //   64 channels:  4 x 768 x 8192 (2^24.6) 37 / 46, x 16384 (3 * 2^24) 55.2 / 55.5, 4 x (256 sequences of 12) x 4096 65 / 64,
+    //                 1 x 12288 x 8192 (3 * 2^25) 112 / 79
+    // The host knows the groups' mean alone, and counts sequences outside every group to it: a large group beside many small
+    // ones takes 32-row tiles too (256 sequences on 8192 tokens 71 us, with 40 pairs beside them 140).
+    constexpr int64_t kWideGroup = 64, kWideWork128 = 1 << 23, kWideWork64 = 3 << 24;
+    // 256 rows instead of 128, with 128 channels: 8 x 256 x 4096 42.5 / 39.9, 8 x 512 x 4096 54.1 / 53.6, 8 x 1024 x 32768 157 / 166
+    // (prefixes alone).
+    constexpr int64_t kWideTallGroup = 192, kWideTallWork = 1 << 24;
+
     // Groups of sequences: the prefixes for all rows of a group and every sequence's tail, then the join.
     template <typename T, int DJ, int RT, bool P32>
     static int kv_shared_launch(const KvAttnArgs &a, hipStream_t s) {
@@ -534,13 +550,9 @@ namespace vkhip {
         a.groups     = p->groups;
         a.max_prefix = p->max_tokens > 0 && p->max_tokens < whole.max_len ? p->max_tokens : whole.max_len;
         const int64_t each = p->groups > 0 ? (int64_t) c->batch * a.rows / p->groups : 0; // rows of a group
-        // Tiles of 128 or 256 rows (kv_prefix.hip) from 2^23 heads x rows x tokens on, of 64 channels, whose narrow tiles run twice as
-        // many at a time, from 3 * 2^24 on; below, their start, about 10 us, is what counts. Whole calls, us, 32-row tiles / wide ones: 8 x
-        // 256 x 4096 39.5 / 39.9, 1 x 400 x 16384 29 / 35, 8 x 512 x 4096 57 / 54; 64 channels, 4 x 768 x 8192 37 / 46, x 16384 55.2 /
-        // 55.5, 4 x (256 sequences of 12) x 4096 65 / 64, 1 x 12288 x 8192 112 / 79. 256 rows instead of 128 from 2^24 on: 8 x 256 x 4096 42.5 / 39.9, 8 x
-        // 512 x 4096 54.1 / 53.6, 8 x 1024 x 32768 157 / 166 (prefixes alone).
         const int64_t work = (int64_t) c->kv_heads * c->batch * a.rows * a.max_prefix;
-        a.wide             = each <= 64 || work <= (a.c.row == 64 ? 3 << 24 : 1 << 23) ? 0 : each > 192 && a.c.row == 128 && work > 1 << 24 ? 2 : 1;
+        const bool    tall = a.c.row == 128 && each > kWideTallGroup && work > kWideTallWork;
+        a.wide             = each <= kWideGroup || work <= (a.c.row == 64 ? kWideWork64 : kWideWork128) ? 0 : tall ? 2 : 1;
         const auto blocks = [&](int height) { return (int64_t) c->batch * a.rows / height + p->groups; };
         if (a.wide && blocks(a.wide * kWideRows) > 65535) a.wide = 0; // more than the third dimension of their grid; the narrow ones' has one
         const int height  = a.wide ? a.wide * kWideRows : 32;
@@ -550,8 +562,10 @@ namespace vkhip {
         const int     round = (a.wide ? 1 : 4) * kStep; // tokens that a workgroup takes at a time
         const int64_t rounds = ceil_div(a.max_prefix > 0 ? a.max_prefix : 1, round), full = ceil_div((int64_t) c->batch * a.rows, height);
         const int64_t base = (full > p->groups ? full : p->groups) * c->kv_heads; // blocks, if groups fill theirs
-        // blocks of uneven groups outnumber that, and two workgroups a compute unit make good for each other's ends (7 groups of 124
-        // sequences, 8, 10, 12 splits: 40, 46 (which begin a second turn), 39 us; one group of 128, 10 and 13: 27, 29)
+        // blocks of uneven groups outnumber that, and two workgroups a compute unit make good for each other's ends, if not for
+        // every size: of 12 drawn sets of 3 to 12 groups of 1 to 54 sequences 7 take the same splits with 512, 640 and 768 places; the
+        // others, whole calls: 82, 92, 85 us; 119, 92, 107; 94, 84, 78; 56, 54, 50; 78, 68, 75. One group of 128 sequences, 512 and
+        // 640: 27, 29.
         const int64_t places = a.wide == 2 ? 256 : a.wide == 1 && p->groups > 1 ? 640 : 512;
         int64_t       splits = base >= places || base == 0 ? 1 : places / base;
         const int64_t most = a.wide ? rounds / kWideLeast : rounds;

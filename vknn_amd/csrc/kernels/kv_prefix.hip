@@ -1,10 +1,10 @@
 // A prefix of the 8-bit cache that many rows share (sequences x query heads x tokens): scores and values as products of
 // whole tiles.
 //
-// A wave owns 32 rows, a workgroup 128. As in the attention over packed sequences, scores come out transposed (S^T = K Q^T,
+// A wave owns 32 rows, a workgroup 128 (four waves) or 256 (eight). As in the attention over packed sequences, scores come out transposed (S^T = K Q^T,
 // 32x32x16) and the exponentials are, as they lie in the registers, the operand of O^T += V^T P^T; the cache keeps the
 // values by channel, so V^T needs no turning, only its tokens in the order in which a lane holds their weights: of each 16,
-// 0-3 8-11 | 4-7 12-15. Bytes become fp16 once for the four waves, on their way from memory through registers into LDS,
+// 0-3 8-11 | 4-7 12-15. Bytes become fp16 once for all waves, on their way from memory through registers into LDS,
 // a tile of 64 tokens ahead.
 // Weights are up to 2^15, as they are in the attention of one sequence, and rescaled where a row's maximum grows by more
 // than 2; a page's value scale goes into its weights' exponents, relative to a power of two at or above the largest of the
@@ -12,9 +12,9 @@
 // page under 2^-8 of that, or above it, takes products of its own, which are multiplied by its scale in fp32. Weights of a
 // page are thus lost from 2^-30 of a row's largest on where its scale is 2^-8 of the span's, from 2^-38 on otherwise.
 //
-// Bound by instruction issue beside the products: 1024 rows behind 32768 tokens, 8 heads of 128, 155 us, 890 TFLOP/s (a
-// library product of 16384^3 1340); matrix units busy 42% of the time, vector units 48%, two waves a SIMD; start and end
-// of a workgroup, queries in and parts out, take about 10 us of it. Value scales are 0 or more, as kv_append makes them:
+// Bound by instruction issue beside the products: 1024 rows behind 32768 tokens, 8 heads of 128, 157 to 168 us by the card, up to
+// 875 TFLOP/s (a library product of 16384^3 1340); matrix units busy 41% of the time, vector units 46%, two waves a SIMD; start
+// and end of a workgroup, queries in and parts out, take about 10 us of it. Value scales are 0 or more, as kv_append makes them:
 // of a negative one the weights' exponents have no logarithm.
 #include "kv_attention.h"
 #include <type_traits>
@@ -33,7 +33,8 @@ namespace vkhip {
         return x;
     }
 
-    // NW: waves of a workgroup, 4 (two of them a compute unit) or, where a group has the rows, 8, which share what is converted.
+    // NW: waves of a workgroup, 4 (two such a compute unit, with 64 channels three) or, where a group has the rows, 8, which share what
+    // is converted.
     template <typename T, int DP, bool P32, int NW>
     __global__ __launch_bounds__(NW * 64, 2) void kv_wide_kernel(KvAttnArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)

@@ -8,8 +8,9 @@
 // goes into Taylor's series, the sine's up to x^11 (next term 2^-37), the cosine's up to x^10 (next 2^-33). One pair's sine
 // and cosine serve all heads that a thread takes.
 //
-// Bound by memory where rows are many: 50176 rows of 40 heads of 128 bf16 183 us, 5.6 TB/s in and out; 45000 rows of 32 heads
-// of 64 fp16, neighbours, 65 us, 5.7 TB/s (partly from the caches). 64 rows 8.2 us, a launch and two loads in a row.
+// Bound by memory where rows are many: 50176 rows of 40 heads of 128 bf16 181 us, 5.7 TB/s in and out, fp32 422 us, 4.9 TB/s;
+// 45000 rows of 32 heads of 64 fp16, neighbours, 65 us, 5.7 TB/s (partly from the caches), fp32, halves, 163 us, 4.5 TB/s. 64 rows
+// 8.2 us, a launch and two loads in a row.
 #include "tokens.h"
 #include <algorithm>
 #include <math.h>
